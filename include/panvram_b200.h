@@ -420,6 +420,76 @@ int pv_windows_form(uint32_t cell, int64_t n, int64_t W, uint32_t flags, int* la
 /* message of the calling thread's last pv_windows / pv_windows_ex argument or launch failure */
 const char* pv_kernels_last_error(void);
 
+/* ---- device: the operators of a training step around a model fed from the cohort (no counterpart in the reference,
+ * which hands the batch out and leaves scoring, losses and clipping to the caller's framework). Device pointers;
+ * asynchronous on `stream`; work: device scratch of the stated size, 16-byte aligned. Failures: pv_kernels_last_error. */
+
+#define PV_T_BF16 0
+#define PV_T_FP16 1
+#define PV_T_FP32 2
+
+/* A batch of n windows of W positions under a model's logits over V words. Position t of window i is scored against
+ * the token at t + shift if that token is counted: t + shift < W, its mask (if any) is not zero, and it is in [0, V) and
+ * not `ignore`. Strides are in elements; the words of a position are contiguous. */
+typedef struct pv_scored {
+    const void* logits;       /* type[n, W, V] */
+    void* grad;               /* their gradient, same type and shape, or NULL: every element written (0 where not counted) */
+    const void* tokens;       /* uint8 or int64 [n, W] */
+    const void* mask;         /* uint8 or float [n, W], or NULL; lies at the tokens' positions */
+    int64_t n, W, V;
+    int64_t logits_n, logits_w, grad_n, grad_w, tokens_n, tokens_w, mask_n, mask_w;
+    int64_t ignore;
+    int32_t shift;
+    int32_t type;             /* PV_T_* */
+    int32_t token_bytes;      /* 1 (uint8) or 8 (int64) */
+    int32_t mask_bytes;       /* 0 (none), 1 (uint8) or 4 (float) */
+} pv_scored;
+
+/* scratch bytes of pv_logprobs / pv_preference / pv_policy on this batch (0: bad arguments or an empty batch) */
+size_t pv_score_work_bytes(const pv_scored* b);
+/* logp[i W + t] = log softmax(logits[i, t])[target], 0 where not counted; sums[i] = its sum over the window. Either may
+ * be NULL. b->grad is not used. */
+int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* work, size_t work_bytes, void* stream);
+/* b->grad[i, t] = up[i up_n + t up_w] * *scale * (one at the target - softmax). scale: a device float, or NULL for 1;
+ * with skip_one, a *scale of exactly 1 leaves b->grad as it is (it then holds that gradient already). */
+int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t up_w, const float* scale, int skip_one, void* stream);
+/* The preference loss: windows [0, n/2) preferred over windows [n/2, n), n even. With S the windows' sums of log
+ * probabilities and R = ref[i ref_n]: margins[k] = (S - R)[k] - (S - R)[k + n/2], h = beta margins[k],
+ * *loss = mean over k of -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h), and coef[i] its derivative by S[i].
+ * If b->grad is given it receives the loss's gradient; else pv_logprobs_grad(b, coef, 1, 0, ...) gives it later.
+ * margins (float [n/2]) may be NULL; coef float [n]. */
+int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float beta, float smoothing, float* loss, float* margins,
+                  float* coef, void* work, size_t work_bytes, void* stream);
+/* The clipped policy loss. Per counted position, r = exp(logp - old) and A = adv:
+ * -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1) with d = ref - logp. *loss is its mean over
+ * the batch's counted positions, or (by_window) the mean over the windows that have any of their own means; 0 if there
+ * are none. float arrays with strides in elements; ref may be NULL with kl 0. weight (double [n]) receives each window's
+ * weight of a position. If b->grad is given it receives the loss's gradient in the same pass. */
+typedef struct pv_policy_args {
+    const float *old, *adv, *ref;
+    int64_t old_n, old_w, adv_n, adv_w, ref_n, ref_w;
+    float clip_low, clip_high, kl;
+    int32_t by_window;
+} pv_policy_args;
+int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* weight, void* work, size_t work_bytes, void* stream);
+/* b->grad = *scale times the loss's gradient, with the weights that pv_policy left (scale, skip_one: pv_logprobs_grad) */
+int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* weight, const float* scale, int skip_one, void* stream);
+
+/* A list of dense tensors on one device, each contiguous in memory: host arrays of their device addresses, element
+ * counts and PV_T_* types. */
+typedef struct pv_tensors {
+    const uint64_t* ptr; const int64_t* numel; const uint8_t* type;
+    int64_t count;
+} pv_tensors;
+/* scratch bytes of pv_grad_norm / pv_clip_grads on this list */
+size_t pv_grads_work_bytes(const pv_tensors* g);
+/* *norm (device float) = the 2-norm over all elements of all tensors, summed in 64 bits */
+int pv_grad_norm(const pv_tensors* g, float* norm, void* work, size_t work_bytes, void* stream);
+/* the same, and every tensor scaled by f = min(1, max_norm / (norm + 1e-6)): into out (same counts; each tensor of its
+ * source's type or float), or with out == NULL in place (nothing is written where f is 1). No tensor that is written
+ * may share memory with another of the two lists, other than with its own source where out names the same one. */
+int pv_clip_grads(const pv_tensors* g, const pv_tensors* out, float max_norm, float* norm, void* work, size_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

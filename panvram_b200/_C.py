@@ -68,6 +68,23 @@ class AsmInfo(ctypes.Structure):
                 ("lower_case_runs", ctypes.c_uint64), ("fasta_xxh3", ctypes.c_uint64), ("bases_xxh3", ctypes.c_uint64)]
 
 
+class Scored(ctypes.Structure):
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("logits", "grad", "tokens", "mask")]
+                + [(k, ctypes.c_int64) for k in ("n", "W", "V", "logits_n", "logits_w", "grad_n", "grad_w", "tokens_n", "tokens_w", "mask_n",
+                                                 "mask_w", "ignore")]
+                + [(k, ctypes.c_int32) for k in ("shift", "type", "token_bytes", "mask_bytes")])
+
+
+class PolicyArgs(ctypes.Structure):
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("old", "adv", "ref")]
+                + [(k, ctypes.c_int64) for k in ("old_n", "old_w", "adv_n", "adv_w", "ref_n", "ref_w")]
+                + [(k, ctypes.c_float) for k in ("clip_low", "clip_high", "kl")] + [("by_window", ctypes.c_int32)])
+
+
+class Tensors(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("numel", ctypes.c_void_p), ("type", ctypes.c_void_p), ("count", ctypes.c_int64)]
+
+
 _P, _I64, _U64, _I32, _U32, _SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint64, ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t
 for _name, _res, _args in (
         ("pv_last_error", ctypes.c_char_p, []),
@@ -111,6 +128,15 @@ for _name, _res, _args in (
         ("pv_windows_items", _SZ, [ctypes.POINTER(DevCohort), _I64, _I64]),
         ("pv_rc_reference", _I32, [_P, _U64, _P, _P]),
         ("pv_windows_trace", _I32, [ctypes.POINTER(DevCohort), _P, _P, _I64, _I64, _P, _I32, _I32, _U32, _P, _P, _P, _SZ, _P, _SZ, _P]),
+        ("pv_score_work_bytes", _SZ, [ctypes.POINTER(Scored)]),
+        ("pv_logprobs", _I32, [ctypes.POINTER(Scored), _P, _P, _P, _SZ, _P]),
+        ("pv_logprobs_grad", _I32, [ctypes.POINTER(Scored), _P, _I64, _I64, _P, _I32, _P]),
+        ("pv_preference", _I32, [ctypes.POINTER(Scored), _P, _I64, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _SZ, _P]),
+        ("pv_policy", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _P, _SZ, _P]),
+        ("pv_policy_grad", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _I32, _P]),
+        ("pv_grads_work_bytes", _SZ, [ctypes.POINTER(Tensors)]),
+        ("pv_grad_norm", _I32, [ctypes.POINTER(Tensors), _P, _P, _SZ, _P]),
+        ("pv_clip_grads", _I32, [ctypes.POINTER(Tensors), ctypes.POINTER(Tensors), ctypes.c_float, _P, _P, _SZ, _P]),
         ("pv_index_build", _I32, [ctypes.POINTER(DevCohort), _U64, _U32, _P, _P, _P, _P, _P])):
     _f = getattr(_lib, _name)
     _f.restype, _f.argtypes = _res, _args

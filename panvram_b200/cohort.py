@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from . import _C
+from .train import window_logprobs
 
 DATASETS = ("q4k", "q16k")
 # torch releases (major.minor) whose randint / rand CUDA kernels (launch geometry, Philox state per thread, element
@@ -396,6 +397,14 @@ class Cohort:
             if s:
                 raise RuntimeError(STATUS_TEXT.format(s))
         return out
+
+    def score(self, model, asm, start, W, reverse_complement=None, token_ids=None, shift=1, check=True):
+        """How likely a model finds windows of the cohort: the windows' tokens (windows(tokens=True), or the five
+        token_ids) through model(tokens) -> logits [n, W, V], then each window's sum of log-probabilities of its bases
+        (train.window_logprobs with this shift; a base that is not A C G T is not counted) -> float32 [n]. No gradient."""
+        with torch.no_grad():
+            x = self.windows(asm, start, W, reverse_complement, tokens=True, check=check, token_ids=token_ids)
+            return window_logprobs(model(x), x, shift=shift, ignore=4 if token_ids is None else int(token_ids[4]), reduce="window")
 
     def trace_windows(self, asm, start, W, reverse_complement=None, tokens=False, flags=0):
         """windows() with a per-item trace of the kernels (pv_windows_trace: %globaltimer at every phase of every work

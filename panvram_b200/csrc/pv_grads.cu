@@ -1,0 +1,330 @@
+// pv_grads.cu - the 2-norm over many tensors and their scaling by min(1, max_norm / (norm + 1e-6))
+// (include/panvram_b200.h pv_grad_norm, pv_clip_grads).
+//
+// The tensors' addresses, counts and types travel as a kernel parameter, so a call copies no table to the device and
+// can be captured. A block takes chunks of CHUNK elements in turn, whatever tensor they lie in, and leaves one partial
+// sum in 64 bits; the scaling kernel's blocks each add those partial sums in the same order, so no launch is spent on
+// it and the result does not change from call to call. Squares are added eight (or four) at a time in 32 bits and then
+// in 64; where such a group leaves the range of 32 bits (elements beyond about 1e18 or all below 1e-13) it is squared
+// again in 64 bits, so the norm neither overflows nor underflows before it is rounded to float at the end.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "panvram_b200.h"
+
+namespace pvb { extern thread_local char g_cuda_err[256]; }
+
+namespace {
+
+using pvb::g_cuda_err;
+
+constexpr int CHUNK = 16384, THREADS = 256, SMS = 148, GRID = SMS * 8;
+
+template <int N>
+struct Table {
+    uint64_t ptr[N], out[N];
+    int64_t numel[N];
+    uint32_t first[N + 1];           // a tensor's first chunk
+    uint8_t type[N], otype[N];
+    int32_t count;
+};
+// two sizes of parameter: a launch copies all of it. 30 bytes per tensor, 32,764 bytes at most.
+constexpr int SMALL = 96, LARGE = 1024;
+static_assert(sizeof(Table<LARGE>) <= 32000, "a kernel's parameters");
+
+__device__ __forceinline__ float f32(float v) { return v; }
+__device__ __forceinline__ float f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from32(float v);
+template <> __device__ __forceinline__ float from32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int N> struct alignas(16) Vec { T v[N]; };
+
+template <int K>
+__device__ __forceinline__ double squares(const float (&x)[K]) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < K; j++) s = fmaf(x[j], x[j], s);
+    if (s > 1e-25f && s < 1e37f) return (double)s;
+    double d = 0;
+#pragma unroll
+    for (int j = 0; j < K; j++) d = fma((double)x[j], (double)x[j], d);
+    return d;
+}
+
+__device__ double block_sum(double v) {                      // every thread of the block gets it
+    __shared__ double sh[33];
+#pragma unroll
+    for (int s = 16; s; s >>= 1) v += __shfl_xor_sync(~0u, v, s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        double w = threadIdx.x < (blockDim.x >> 5) ? sh[threadIdx.x] : 0.0;
+#pragma unroll
+        for (int s = 16; s; s >>= 1) w += __shfl_xor_sync(~0u, w, s);
+        if (threadIdx.x == 0) sh[32] = w;
+    }
+    __syncthreads();
+    return sh[32];
+}
+
+// the tensor that chunk c lies in: the last whose first chunk is not after it (empty tensors share their successor's)
+template <int N>
+__device__ __forceinline__ int tensor_of(const Table<N>& t, uint32_t c) {
+    int lo = 0, hi = t.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.first[mid] <= c) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// elements from `p` to its next 16-byte boundary
+template <typename T>
+__device__ __forceinline__ int to_boundary(const T* p) { return (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T)); }
+
+template <typename T>
+__device__ double chunk_squares(const T* p, int count) {
+    constexpr int K = 16 / sizeof(T);
+    const int head = min(to_boundary(p), count), nv = (count - head) / K, tail = head + nv * K;
+    double s = 0;
+    float one[1];
+    if ((int)threadIdx.x < head) { one[0] = f32(p[threadIdx.x]); s += squares(one); }
+    if (tail + (int)threadIdx.x < count) { one[0] = f32(p[tail + threadIdx.x]); s += squares(one); }
+    const uint4* q = (const uint4*)(p + head);
+#pragma unroll 4
+    for (int j = threadIdx.x; j < nv; j += THREADS) {
+        const uint4 raw = q[j];
+        const Vec<T, K>& v = *(const Vec<T, K>*)&raw;
+        float x[K];
+#pragma unroll
+        for (int e = 0; e < K; e++) x[e] = f32(v.v[e]);
+        s += squares(x);
+    }
+    return s;
+}
+
+template <int N>
+__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ Table<N> t, double* part) {
+    double s = 0;
+    for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+        const int i = tensor_of(t, c);
+        const int64_t at = (int64_t)(c - t.first[i]) * CHUNK;
+        const int count = (int)min((int64_t)CHUNK, t.numel[i] - at);
+        switch (t.type[i]) {
+            case PV_T_BF16: s += chunk_squares((const __nv_bfloat16*)t.ptr[i] + at, count); break;
+            case PV_T_FP16: s += chunk_squares((const __half*)t.ptr[i] + at, count); break;
+            default: s += chunk_squares((const float*)t.ptr[i] + at, count);
+        }
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+__device__ double norm_of(const double* part, int64_t parts) {
+    double s = 0;
+    for (int64_t j = threadIdx.x; j < parts; j += blockDim.x) s += part[j];
+    return sqrt(block_sum(s));
+}
+
+__global__ void __launch_bounds__(THREADS) finish_norm_kernel(const double* part, int64_t parts, float* norm) {
+    const double s = norm_of(part, parts);
+    if (threadIdx.x == 0) *norm = (float)s;
+}
+
+template <typename T, typename O>
+__device__ void scale_chunk(const T* p, O* o, int count, float f) {
+    constexpr int K = 16 / sizeof(T);
+    int head = min(to_boundary(p), count), nv = (count - head) / K;
+    if (((uintptr_t)(o + head) & 15) != 0) { head = count; nv = 0; }     // the two differ in alignment: element by element
+    const int tail = head + nv * K;
+    for (int j = threadIdx.x; j < head; j += THREADS) o[j] = from32<O>(f32(p[j]) * f);
+    for (int j = tail + threadIdx.x; j < count; j += THREADS) o[j] = from32<O>(f32(p[j]) * f);
+    const uint4* q = (const uint4*)(p + head);
+#pragma unroll 4
+    for (int j = threadIdx.x; j < nv; j += THREADS) {
+        const uint4 raw = q[j];
+        const Vec<T, K>& v = *(const Vec<T, K>*)&raw;
+        Vec<O, K> w;
+#pragma unroll
+        for (int e = 0; e < K; e++) w.v[e] = from32<O>(f32(v.v[e]) * f);
+        *(Vec<O, K>*)(o + head + j * K) = w;
+    }
+}
+
+template <int N>
+__global__ void __launch_bounds__(THREADS) clip_kernel(const __grid_constant__ Table<N> t, const double* part, int64_t parts, float max_norm,
+                                                       int in_place, float* norm) {
+    const double s = norm_of(part, parts), r = (double)max_norm / (s + 1e-6);
+    const float f = r >= 1.0 ? 1.f : (float)r;               // NaN stays
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)s;
+    if (in_place && f == 1.f) return;
+    // last chunks first: the norm's pass left those in L2
+    for (int64_t q = (int64_t)t.first[t.count] - 1 - blockIdx.x; q >= 0; q -= gridDim.x) {
+        const uint32_t c = (uint32_t)q;
+        const int i = tensor_of(t, c);
+        const int64_t at = (int64_t)(c - t.first[i]) * CHUNK;
+        const int count = (int)min((int64_t)CHUNK, t.numel[i] - at);
+        const bool wide = t.otype[i] == PV_T_FP32;
+        switch (t.type[i]) {
+            case PV_T_BF16:
+                if (wide) scale_chunk((const __nv_bfloat16*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
+                else scale_chunk((const __nv_bfloat16*)t.ptr[i] + at, (__nv_bfloat16*)t.out[i] + at, count, f);
+                break;
+            case PV_T_FP16:
+                if (wide) scale_chunk((const __half*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
+                else scale_chunk((const __half*)t.ptr[i] + at, (__half*)t.out[i] + at, count, f);
+                break;
+            default: scale_chunk((const float*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host
+int fail(int code, const char* what) {
+    snprintf(g_cuda_err, sizeof g_cuda_err, "%s", what);
+    return code;
+}
+int launched() {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? PV_OK : fail(PV_ECUDA, cudaGetErrorString(e));
+}
+
+int elem(uint8_t type) { return type == PV_T_FP32 ? 4 : 2; }
+
+const char* bad_list(const pv_tensors* g) {
+    if (!g || g->count < 0 || (g->count && (!g->ptr || !g->numel || !g->type))) return "tensors: NULL list";
+    for (int64_t i = 0; i < g->count; i++) {
+        if (g->type[i] > PV_T_FP32) return "tensors: bf16, fp16 or fp32";
+        if (g->numel[i] < 0 || g->numel[i] > (1ll << 45)) return "tensors: a size is out of range";
+        if (g->numel[i] && (!g->ptr[i] || g->ptr[i] % elem(g->type[i]))) return "tensors: an address is NULL or not aligned to its type";
+    }
+    return nullptr;
+}
+
+// a tensor that is written shares memory with another
+struct Span { uint64_t a, b; bool written; };
+bool overlap(const pv_tensors* g, const pv_tensors* out) {
+    std::vector<Span> v;
+    v.reserve((size_t)g->count * (out ? 2 : 1));
+    for (int64_t i = 0; i < g->count; i++) {
+        if (!g->numel[i]) continue;
+        const uint64_t ga = g->ptr[i], gb = ga + (uint64_t)g->numel[i] * elem(g->type[i]);
+        if (!out || (out->ptr[i] == ga && out->type[i] == g->type[i])) { v.push_back({ga, gb, true}); continue; }
+        v.push_back({ga, gb, false});
+        v.push_back({out->ptr[i], out->ptr[i] + (uint64_t)g->numel[i] * elem(out->type[i]), true});
+    }
+    std::sort(v.begin(), v.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+    uint64_t end = 0, end_written = 0;
+    for (const Span& s : v) {
+        if (s.a < (s.written ? end : end_written)) return true;
+        end = std::max(end, s.b);
+        if (s.written) end_written = std::max(end_written, s.b);
+    }
+    return false;
+}
+
+int64_t launches_of(const pv_tensors* g) { return (g->count + LARGE - 1) / LARGE; }
+
+template <int N>
+int64_t fill(Table<N>& t, const pv_tensors* g, const pv_tensors* out, int64_t from, int64_t to) {
+    uint64_t c = 0;
+    t.count = (int32_t)(to - from);
+    for (int64_t i = from; i < to; i++) {
+        const int64_t k = i - from;
+        t.ptr[k] = g->ptr[i];
+        t.numel[k] = g->numel[i];
+        t.type[k] = g->type[i];
+        t.out[k] = out ? out->ptr[i] : g->ptr[i];
+        t.otype[k] = out ? out->type[i] : g->type[i];
+        t.first[k] = (uint32_t)c;
+        c += (uint64_t)((g->numel[i] + CHUNK - 1) / CHUNK);
+    }
+    t.first[t.count] = (uint32_t)c;
+    return c < (1ull << 32) ? (int64_t)c : -1;
+}
+
+// one launch over tensors [from, to): the norm's partial sums, or the scaling
+template <int N>
+int one(const pv_tensors* g, const pv_tensors* out, int64_t from, int64_t to, bool clip, double* part, int64_t* parts, float max_norm, bool in_place,
+        float* norm, cudaStream_t st) {
+    static thread_local Table<N> t;
+    const int64_t chunks = fill(t, g, out, from, to);
+    if (chunks < 0) return fail(PV_EARG, "tensors: too many elements in one list");
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks, GRID));
+    if (clip) {
+        clip_kernel<N><<<grid, THREADS, 0, st>>>(t, part, *parts, max_norm, in_place, norm);
+    } else {
+        norm_kernel<N><<<grid, THREADS, 0, st>>>(t, part + *parts);
+        *parts += grid;
+    }
+    return launched();
+}
+
+int all(const pv_tensors* g, const pv_tensors* out, bool clip, double* part, int64_t* parts, float max_norm, bool in_place, float* norm,
+        cudaStream_t st) {
+    for (int64_t from = 0; from < std::max<int64_t>(g->count, 1); from += LARGE) {
+        const int64_t to = std::min<int64_t>(g->count, from + LARGE);
+        float* nm = from == 0 ? norm : nullptr;
+        const int e = to - from <= SMALL ? one<SMALL>(g, out, from, to, clip, part, parts, max_norm, in_place, nm, st)
+                                         : one<LARGE>(g, out, from, to, clip, part, parts, max_norm, in_place, nm, st);
+        if (e) return e;
+    }
+    return PV_OK;
+}
+
+int norm_parts(const pv_tensors* g, float* norm, void* work, size_t work_bytes, int64_t* parts, cudaStream_t st) {
+    if (!norm) return fail(PV_EARG, "norm: NULL");
+    if (!work || work_bytes < pv_grads_work_bytes(g) || ((uintptr_t)work & 15)) return fail(PV_EARG, "scratch: too small, NULL or not 16-byte aligned");
+    *parts = 0;
+    return all(g, nullptr, false, (double*)work, parts, 0.f, false, nullptr, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pv_grads_work_bytes(const pv_tensors* g) {
+    if (!g || g->count < 0) return 0;
+    return (size_t)std::max<int64_t>(1, launches_of(g)) * GRID * sizeof(double);
+}
+
+int pv_grad_norm(const pv_tensors* g, float* norm, void* work, size_t work_bytes, void* stream) {
+    if (const char* why = bad_list(g)) return fail(PV_EARG, why);
+    int64_t parts = 0;
+    if (const int e = norm_parts(g, norm, work, work_bytes, &parts, (cudaStream_t)stream)) return e;
+    finish_norm_kernel<<<1, THREADS, 0, (cudaStream_t)stream>>>((const double*)work, parts, norm);
+    return launched();
+}
+
+int pv_clip_grads(const pv_tensors* g, const pv_tensors* out, float max_norm, float* norm, void* work, size_t work_bytes, void* stream) {
+    if (const char* why = bad_list(g)) return fail(PV_EARG, why);
+    if (!(max_norm >= 0.f)) return fail(PV_EARG, "max_norm: negative or NaN");
+    if (out) {
+        if (const char* why = bad_list(out)) return fail(PV_EARG, why);
+        if (out->count != g->count) return fail(PV_EARG, "out: another number of tensors");
+        for (int64_t i = 0; i < g->count; i++) {
+            if (out->numel[i] != g->numel[i]) return fail(PV_EARG, "out: a tensor of another size");
+            if (out->type[i] != g->type[i] && out->type[i] != PV_T_FP32) return fail(PV_EARG, "out: a tensor of neither its source's type nor float");
+        }
+    }
+    try {
+        if (overlap(g, out)) return fail(PV_EARG, "tensors: one that is written shares memory with another");
+    } catch (...) {
+        return fail(PV_EARG, "tensors: out of host memory");
+    }
+    int64_t parts = 0;
+    if (const int e = norm_parts(g, norm, work, work_bytes, &parts, (cudaStream_t)stream)) return e;
+    return all(g, out, true, (double*)work, &parts, max_norm, !out, norm, (cudaStream_t)stream);
+}
+
+}  // extern "C"

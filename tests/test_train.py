@@ -1,0 +1,166 @@
+"""The training-step operators' refusals and argument checks, without a GPU (nothing is launched: every call here is
+refused before its first CUDA call)."""
+import ctypes
+
+import pytest
+import torch
+
+import panvram_b200 as P
+from panvram_b200 import _C
+
+X = torch.zeros(2, 3, 4)
+T = torch.zeros(2, 3, dtype=torch.uint8)
+L = torch.zeros(2, 3)
+A = torch.zeros(2)
+
+
+def _calls(logits=X, tokens=T, **kw):
+    return (lambda: P.window_logprobs(logits, tokens, **kw), lambda: P.preference_loss(logits, tokens, A, **kw),
+            lambda: P.policy_loss(logits, tokens, L, A, **kw))
+
+
+@pytest.mark.parametrize("kw, what", [
+    ({"logits": X.double()}, "logits"), ({"logits": X[0]}, "logits"), ({"logits": torch.zeros(2, 3, 0)}, "logits"),
+    ({"logits": torch.zeros(2, 4, 3).transpose(1, 2)}, "logits"), ({"logits": [[[0.0]]]}, "logits"), ({"logits": X.int()}, "logits"),
+    ({"logits": torch.zeros(2, 3, 1).expand(2, 3, 4)}, "logits"),
+    ({"tokens": T[:, :2]}, "tokens"), ({"tokens": T.int()}, "tokens"), ({"tokens": T.bool()}, "tokens"), ({"tokens": None}, "tokens"),
+    ({"mask": T[:1]}, "mask"), ({"mask": T.long()}, "mask"), ({"mask": X.half()[..., 0]}, "mask"), ({"mask": True}, "mask"),
+    ({"shift": -1}, "shift"), ({"shift": 1 << 31}, "shift"),
+])
+def test_shared_refusals(kw, what):
+    for call in _calls(**kw):
+        with pytest.raises(ValueError, match=what):
+            call()
+
+
+def test_cpu_tensors_are_refused():
+    for call in _calls():
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+    for call in (lambda: P.grad_norm([A]), lambda: P.clip_grads([A], 1.0), lambda: P.clip_grads(A, 1.0, out=[torch.zeros(2)])):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+def test_refusals_of_numbers_and_names():
+    for bad in (-0.1, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="beta"):
+            P.preference_loss(X, T, A, beta=bad)
+        with pytest.raises(ValueError, match="clip"):
+            P.policy_loss(X, T, L, A, clip=bad)
+        with pytest.raises(ValueError, match="clip"):
+            P.policy_loss(X, T, L, A, clip=(0.2, bad))
+        with pytest.raises(ValueError, match="kl"):
+            P.policy_loss(X, T, L, A, ref_logp=L, kl=bad)
+    for bad in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError, match="label_smoothing"):
+            P.preference_loss(X, T, A, label_smoothing=bad)
+    with pytest.raises(ValueError, match="ref_logp"):
+        P.policy_loss(X, T, L, A, kl=0.1)
+    with pytest.raises(ValueError, match="reduce"):
+        P.policy_loss(X, T, L, A, reduce="sum")
+    with pytest.raises(ValueError, match="reduce"):
+        P.window_logprobs(X, T, reduce="mean")
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            P.clip_grads([A], bad)
+
+
+def test_refusals_of_gradient_lists():
+    for fn in (P.grad_norm, lambda g: P.clip_grads(g, 1.0)):
+        with pytest.raises(ValueError, match="no tensors"):
+            fn([])
+        with pytest.raises(ValueError, match="bf16, fp16 or fp32"):
+            fn([A, A.double()])
+        with pytest.raises(ValueError, match="bf16, fp16 or fp32"):
+            fn([None])
+        with pytest.raises(ValueError, match="dense"):
+            fn([torch.zeros(4, 4)[:, :2]])
+        with pytest.raises(ValueError, match="dense"):
+            fn([torch.zeros(1).expand(4)])
+    with pytest.raises(ValueError, match="out"):
+        P.clip_grads([A], 1.0, out=[A, A])
+    with pytest.raises(ValueError, match="out"):
+        P.clip_grads([A], 1.0, out=[torch.zeros(3)])
+    with pytest.raises(ValueError, match="out"):
+        P.clip_grads([torch.zeros(2, 3)], 1.0, out=[torch.zeros(3, 2).t()])
+    with pytest.raises(ValueError, match="out"):
+        P.clip_grads([A], 1.0, out=[A.half()])
+    with pytest.raises(ValueError, match="not parameters"):
+        P.clip_grads([torch.nn.Parameter(A.clone())], 1.0)
+
+
+def _scored(**kw):
+    b = _C.Scored(64, None, 64, None, 2, 3, 4, 12, 4, 0, 0, 3, 1, 0, 0, 4, 1, 2, 1, 0)
+    for k, v in kw.items():
+        setattr(b, k, v)
+    return ctypes.byref(b)
+
+
+def _message():
+    return (_C._lib.pv_kernels_last_error() or b"").decode()
+
+
+@pytest.mark.parametrize("kw", [{"n": -1}, {"W": -1}, {"W": 1 << 31}, {"V": 0}, {"V": 1 << 31}, {"shift": -1}, {"type": 3}, {"type": -1},
+                                {"token_bytes": 4}, {"mask_bytes": 2}, {"mask_bytes": 1}, {"logits": None}, {"tokens": None},
+                                {"n": 1 << 40, "W": 1 << 30}])
+def test_entry_points_refuse_a_bad_batch(kw):
+    lib, b = _C._lib, _scored(**kw)
+    a = _C.PolicyArgs(64, 64, None, 3, 1, 1, 0, 0, 0, 0.2, 0.2, 0.0, 0)
+    assert lib.pv_score_work_bytes(b) == 0
+    assert lib.pv_logprobs(b, 64, None, None, 0, None) == _C.PV_EARG and _message().startswith("batch")
+    assert lib.pv_logprobs_grad(b, 64, 0, 0, None, 0, None) == _C.PV_EARG
+    assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 40, None) == _C.PV_EARG
+    assert lib.pv_policy(b, ctypes.byref(a), 64, 64, 64, 1 << 40, None) == _C.PV_EARG
+    assert lib.pv_policy_grad(b, ctypes.byref(a), 64, None, 0, None) == _C.PV_EARG
+
+
+def test_entry_points_refuse_missing_arguments():
+    lib, b = _C._lib, _scored()
+    good = dict(old=64, adv=64, ref=None, clip_low=0.2, clip_high=0.2, kl=0.0)
+    assert lib.pv_logprobs(b, None, 64, None, 0, None) == _C.PV_EARG and "scratch" in _message()
+    assert lib.pv_logprobs(b, None, 64, 72, 1 << 30, None) == _C.PV_EARG and "scratch" in _message()      # not 16-byte aligned
+    assert lib.pv_logprobs_grad(b, 64, 0, 0, None, 0, None) == _C.PV_EARG                                  # no gradient to write
+    assert lib.pv_preference(_scored(n=3), 64, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 30, None) == _C.PV_EARG and "odd" in _message()
+    assert lib.pv_preference(b, None, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 30, None) == _C.PV_EARG
+    assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, 64, 1, None) == _C.PV_EARG and "scratch" in _message()
+    for kw in ({"old": None}, {"adv": None}, {"clip_low": -1.0}, {"clip_high": float("nan")}, {"kl": 0.1}):
+        assert lib.pv_policy(b, ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, 64, 64, 1 << 30, None) == _C.PV_EARG
+        assert lib.pv_policy_grad(_scored(grad=64), ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, None, 0, None) == _C.PV_EARG
+    assert lib.pv_policy(b, None, 64, 64, 64, 1 << 30, None) == _C.PV_EARG
+    assert lib.pv_policy(b, ctypes.byref(_C.PolicyArgs(**good)), 64, 64, 64, 8, None) == _C.PV_EARG
+
+
+def _list(ptrs, numels, types):
+    n = len(ptrs)
+    p, k, t = (ctypes.c_uint64 * n)(*ptrs), (ctypes.c_int64 * n)(*numels), (ctypes.c_uint8 * n)(*types)
+    g = _C.Tensors(ctypes.cast(p, ctypes.c_void_p), ctypes.cast(k, ctypes.c_void_p), ctypes.cast(t, ctypes.c_void_p), n)
+    g.kept = (p, k, t)
+    return g
+
+
+def test_entry_points_refuse_bad_lists_and_shared_memory():
+    lib = _C._lib
+
+    def clip(g, out=None, max_norm=1.0, work=64, need=1 << 20):
+        return lib.pv_clip_grads(ctypes.byref(g), ctypes.byref(out) if out is not None else None, max_norm, 64, work, need, None)
+    f = 2                                                                       # float
+    for g in (_list([0], [4], [f]), _list([66], [4], [f]), _list([65], [4], [0]), _list([64], [-1], [f]), _list([64], [4], [3]),
+              _list([64], [1 << 50], [f])):
+        assert clip(g) == _C.PV_EARG and _message().startswith("tensors")
+        assert lib.pv_grad_norm(ctypes.byref(g), 64, 64, 1 << 20, None) == _C.PV_EARG
+    g = _list([256, 512], [4, 8], [f, f])
+    assert clip(g, max_norm=float("nan")) == _C.PV_EARG and clip(g, max_norm=-1.0) == _C.PV_EARG
+    assert clip(g, need=8) == _C.PV_EARG and "scratch" in _message()
+    assert clip(g, work=None) == _C.PV_EARG and clip(g, work=72) == _C.PV_EARG
+    for out in (_list([256], [4], [f]), _list([256, 512], [4, 7], [f, f]), _list([256, 512], [4, 8], [f, 0])):
+        assert clip(g, out) == _C.PV_EARG and _message().startswith("out")
+    shared = "shares memory"
+    for g, out in ((_list([256, 256], [4, 4], [f, f]), None),                    # the same tensor twice, in place
+                   (_list([256, 268], [4, 8], [f, f]), None),                    # one behind the other's start
+                   (_list([268, 256], [8, 4], [f, f]), None),
+                   (_list([256, 512], [4, 8], [f, f]), _list([1024, 1024], [4, 8], [f, f])),     # into the same place
+                   (_list([256, 512], [4, 8], [f, f]), _list([512, 1024], [4, 8], [f, f])),      # over another gradient
+                   (_list([256], [8], [f]), _list([272], [8], [f])),                             # over part of itself
+                   (_list([256], [8], [0]), _list([256], [8], [f]))):                            # wider, over itself
+        assert clip(g, out) == _C.PV_EARG and shared in _message()
