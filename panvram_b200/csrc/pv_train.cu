@@ -47,8 +47,7 @@ enum { LOGP = 0, GRAD = 1, POLICY = 2 };
 
 struct Rows {
     pv_scored b;
-    int64_t tpw;             // tiles per window
-    int32_t rows;            // rows per tile
+    int64_t tpw;             // tiles (of TILE rows, or of one) per window
     // LOGP
     float* logp;             // or NULL
     double* part;            // a partial sum per tile (LOGP: of log-probabilities, POLICY: of loss terms), or NULL
@@ -88,29 +87,38 @@ __device__ __forceinline__ float kl_term(float d, float em1) {
     return em1 - d;
 }
 
-// One thread, per counted row: takes the log-probability, adds the row's term to `sum`, gives the row's derivative by it.
+// What a counted row's end reads, loaded before its logits are waited for.
+struct End { float a, old, ref; double w; };
 template <int MODE>
-__device__ __forceinline__ float row_end(const Rows& k, int64_t i, int64_t t, float lp, float scale, double& sum) {
-    if (MODE == LOGP) {
-        if (k.logp) k.logp[i * k.b.W + t] = lp;
-        sum += lp;
-        return 0.f;
+__device__ __forceinline__ End end_args(const Rows& k, int64_t i, int64_t t) {
+    End e = {0.f, 0.f, 0.f, 0.0};
+    if (MODE == GRAD) e.a = k.up[i * k.up_n + t * k.up_w];
+    if (MODE == POLICY) {
+        e.a = k.a.adv[i * k.a.adv_n + t * k.a.adv_w];
+        e.old = k.a.old[i * k.a.old_n + t * k.a.old_w];
+        if (k.a.ref) e.ref = k.a.ref[i * k.a.ref_n + t * k.a.ref_w];
+        e.w = k.weight[i];
     }
-    if (MODE == GRAD) return k.up[i * k.up_n + t * k.up_w] * scale;
-    const float A = k.a.adv[i * k.a.adv_n + t * k.a.adv_w];
-    const float r = expf(lp - k.a.old[i * k.a.old_n + t * k.a.old_w]);
-    const float one = A == 0.f ? 0.f : r * A;
-    const float two = fminf(fmaxf(r, 1.f - k.a.clip_low), 1.f + k.a.clip_high) * A;
+    return e;
+}
+
+// From a counted row's log-probability its term of the sum and its derivative (the result).
+template <int MODE>
+__device__ __forceinline__ float row_end(const Rows& k, const End& e, float lp, float scale, double& term) {
+    if (MODE == LOGP) { term = lp; return 0.f; }
+    if (MODE == GRAD) { term = 0; return e.a * scale; }
+    const float r = expf(lp - e.old);
+    const float one = e.a == 0.f ? 0.f : r * e.a;
+    const float two = fminf(fmaxf(r, 1.f - k.a.clip_low), 1.f + k.a.clip_high) * e.a;
     const bool free = !(one > two);                          // NaN stays
-    float term = free ? -one : -two, g = free ? -one : 0.f;
+    float v = free ? -one : -two, g = free ? -one : 0.f;
     if (k.a.ref) {
-        const float d = k.a.ref[i * k.a.ref_n + t * k.a.ref_w] - lp, em1 = expm1f(d);
-        term += k.a.kl * kl_term(d, em1);
+        const float d = e.ref - lp, em1 = expm1f(d);
+        v += k.a.kl * kl_term(d, em1);
         g -= k.a.kl * em1;
     }
-    const double w = k.weight[i];
-    sum += (double)term * w;
-    return g * (float)w * scale;
+    term = (double)v * e.w;
+    return g * (float)e.w * scale;
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -125,41 +133,387 @@ __device__ __forceinline__ F warp_sum(F v) {
     return v;
 }
 
-// ---------------------------------------------------------------- a warp per tile of rows, element by element
-// Any type, stride and length: two passes over a row for its maximum and sum, a third for the gradient.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) rows_any_kernel(Rows k) {
-    const int lane = threadIdx.x & 31;
+// ---------------------------------------------------------------- 16 bytes of a row
+template <typename T> struct Traits;
+template <> struct Traits<float> { static constexpr uint32_t LOW = 0xFF800000u; };             // -inf, as a word of elements
+template <> struct Traits<__half> { static constexpr uint32_t LOW = 0xFC00FC00u; };
+template <> struct Traits<__nv_bfloat16> { static constexpr uint32_t LOW = 0xFF80FF80u; };
+template <typename T> constexpr int K_OF = 16 / (int)sizeof(T);
+
+template <typename T> __device__ __forceinline__ void unpack(const uint4& r, float (&x)[K_OF<T>]);
+template <> __device__ __forceinline__ void unpack<float>(const uint4& r, float (&x)[4]) {
+    x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int q = 0; q < 4; q++) { x[2 * q] = __uint_as_float(w[q] << 16); x[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u); }
+}
+template <> __device__ __forceinline__ void unpack<__half>(const uint4& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const float2 f = __half22float2(*(const __half2*)&w[q]);
+        x[2 * q] = f.x; x[2 * q + 1] = f.y;
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&x)[K_OF<T>]);
+template <> __device__ __forceinline__ uint4 pack<float>(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) { const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * q], x[2 * q + 1]); w[q] = *(const uint32_t*)&v; }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <> __device__ __forceinline__ uint4 pack<__half>(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) { const __half2 v = __floats2half2_rn(x[2 * q], x[2 * q + 1]); w[q] = *(const uint32_t*)&v; }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A row of V elements seen as aligned 16-byte pieces: piece v holds elements v K - off ... + K, off = how far into its
+// first piece the row starts. The pieces at the row's ends are moved by element, so nothing outside the row is touched.
+template <typename T>
+__device__ __forceinline__ int row_off(const T* x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+template <typename T>
+__device__ __forceinline__ uint4 edge_piece(const T* x, int e0, int V) {       // -inf outside the row
+    constexpr int K = K_OF<T>;
+    alignas(16) T v[K];
+#pragma unroll
+    for (int q = 0; q < K; q++) v[q] = e0 + q >= 0 && e0 + q < V ? x[e0 + q] : from32<T>(-INFINITY);
+    return *(const uint4*)v;
+}
+template <typename T>
+__device__ __forceinline__ bool whole(int e0, int V) { return e0 >= 0 && e0 + K_OF<T> <= V; }
+template <typename T>
+__device__ __forceinline__ void store_piece(T* d, int e0, int V, bool aligned, const float (&x)[K_OF<T>]) {
+    constexpr int K = K_OF<T>;
+    if (aligned && whole<T>(e0, V)) { *(uint4*)(d + e0) = pack<T>(x); return; }
+#pragma unroll
+    for (int q = 0; q < K; q++)
+        if (e0 + q >= 0 && e0 + q < V) d[e0 + q] = from32<T>(x[q]);
+}
+// the pieces of x and d fall alike
+template <typename T>
+__device__ __forceinline__ bool alike(const T* x, const T* d) { return (((uintptr_t)x ^ (uintptr_t)d) & 15) == 0; }
+
+// ---------------------------------------------------------------- rows of up to 256 pieces: G lanes a row, NV pieces a lane
+// The row stays in registers from its load to its gradient, so it is read once. A warp takes a tile of 32 rows, 32 / G at
+// a time; each lane loads one row's target and arguments for the whole tile first.
+constexpr int TILE = 32;
+
+template <typename T, int G, int NV, int MODE>
+__global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
+    constexpr int K = K_OF<T>, RP = 32 / G;
+    const int lane = threadIdx.x & 31, sub = lane % G, grp = lane / G, V = (int)k.b.V;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     const int64_t tiles = k.b.n * k.tpw, step = (int64_t)gridDim.x * (blockDim.x >> 5);
     for (int64_t tile = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); tile < tiles; tile += step) {
-        const int64_t i = tile / k.tpw, t0 = (tile - i * k.tpw) * k.rows, t1 = min(t0 + k.rows, k.b.W);
+        const int64_t i = tile / k.tpw, t0 = (tile - i * k.tpw) * TILE;
+        const int rows = (int)min((int64_t)TILE, k.b.W - t0);
+        const int y_l = lane < rows ? target(k.b, i, t0 + lane) : -1;
         double sum = 0;
-        for (int64_t t = t0; t < t1; t++) {
+        for (int s0 = 0; s0 < rows; s0 += RP) {
+            const int row = s0 + grp;
+            const int64_t t = t0 + row;
+            const int y = __shfl_sync(~0u, y_l, row);
             const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
-            T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
-            const int y = target(k.b, i, t), V = (int)k.b.V;
-            if (y < 0) {
-                if (MODE == LOGP && k.logp && lane == 0) k.logp[i * k.b.W + t] = 0.f;
-                if (MODE != LOGP && d)
-                    for (int j = lane; j < V; j += 32) d[j] = from32<T>(0.f);
-                continue;
+            const int off = row_off(x);
+            uint4 raw[NV];
+            End end = {0.f, 0.f, 0.f, 0.0};
+            float xt = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; j++) raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+            if (y >= 0) {
+                end = end_args<MODE>(k, i, t);
+                xt = f32(x[y]);
+#pragma unroll
+                for (int j = 0; j < NV; j++) {
+                    const int e0 = (sub + j * G) * K - off;
+                    if (whole<T>(e0, V)) raw[j] = *(const uint4*)(x + e0);
+                    else if (e0 < V) raw[j] = edge_piece(x, e0, V);
+                }
             }
-            float m = -INFINITY, o = 0.f;
-            for (int j = lane; j < V; j += 32) m = fmaxf(m, f32(x[j]));
-            m = warp_max(m);
-            for (int j = lane; j < V; j += 32) o += j == y ? 0.f : numerator(f32(x[j]), m);
-            o = warp_sum(o);
-            float e, g = 0.f;
-            const float lp = row_logp(m, o, f32(x[y]), &e);
-            if (lane == 0) g = row_end<MODE>(k, i, t, lp, scale, sum);
-            if (MODE == LOGP || !d) continue;
-            g = __shfl_sync(~0u, g, 0);
-            const float inv = 1.f / (o + e), f = -g * inv;
-            for (int j = lane; j < V; j += 32) d[j] = from32<T>(j == y ? g * (o * inv) : f * numerator(f32(x[j]), m));
+            float m = -INFINITY, o = 0.f, e[NV][K];
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                unpack<T>(raw[j], e[j]);
+#pragma unroll
+                for (int q = 0; q < K; q++) m = fmaxf(m, e[j][q]);
+            }
+#pragma unroll
+            for (int s = G / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, s));
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int at = y - ((sub + j * G) * K - off);
+                float part = 0.f;
+#pragma unroll
+                for (int q = 0; q < K; q++) {
+                    e[j][q] = numerator(e[j][q], m);
+                    part += q == at ? 0.f : e[j][q];
+                }
+                o += part;
+            }
+#pragma unroll
+            for (int s = G / 2; s; s >>= 1) o += __shfl_xor_sync(~0u, o, s);
+            float et, lp = 0.f, g = 0.f;
+            double term = 0;
+            if (y >= 0) {
+                lp = row_logp(m, o, xt, &et);
+                g = row_end<MODE>(k, end, lp, scale, term);
+                if (sub == 0) sum += term;
+            }
+            if (MODE == LOGP) {
+                if (k.logp && sub == 0 && row < rows) k.logp[i * k.b.W + t] = lp;
+            } else if (k.b.grad && row < rows) {
+                T* d = (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w;
+                const bool same = alike(x, d);
+                const float inv = 1.f / (o + et), f = -g * inv, ft = g * (o * inv);
+#pragma unroll
+                for (int j = 0; j < NV; j++) {
+                    const int e0 = (sub + j * G) * K - off;
+                    float v[K];
+#pragma unroll
+                    for (int q = 0; q < K; q++) v[q] = y < 0 ? 0.f : q == y - e0 ? ft : e[j][q] * f;
+                    if (e0 < V) store_piece(d, e0, V, same, v);
+                }
+            }
         }
-        if (k.part && lane == 0) k.part[tile] = sum;
+        if (k.part) {
+            sum = warp_sum(sum);
+            if (lane == 0) k.part[tile] = sum;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- longer rows: a block a row
+// the running maximum and sum of a thread; `base`: the maximum, or 0 where there is none yet
+struct Run { float m = -INFINITY, o = 0.f; };
+template <int K>
+__device__ __forceinline__ void take(Run& r, const float (&x)[K], int at) {       // at: the target's place among them, if any
+    float m = x[0];
+#pragma unroll
+    for (int q = 1; q < K; q++) m = fmaxf(m, x[q]);
+    if (m > r.m) { r.o *= numerator(r.m, m); r.m = m; }
+    const float base = r.m == -INFINITY ? 0.f : r.m;
+    float part = 0.f;
+    if (at >= 0 && at < K) {
+#pragma unroll
+        for (int q = 0; q < K; q++) part += q == at ? 0.f : numerator(x[q], base);
+    } else {
+#pragma unroll
+        for (int q = 0; q < K; q++) part += numerator(x[q], base);
+    }
+    r.o += part;
+}
+__device__ __forceinline__ void warp_join(Run& r) {
+    const float m = warp_max(r.m);
+    r.o = warp_sum(r.m == m ? r.o : r.o * numerator(r.m, m));
+    r.m = m;
+}
+// The block's: one barrier a row, two buffers in turn (a buffer is written again only after the next row's barrier, which
+// every thread reaches after its reads here).
+template <int THREADS>
+__device__ __forceinline__ void block_join(Run& r, float2 (&red)[2][THREADS / 32], int turn) {
+    constexpr int NW = THREADS / 32;
+    warp_join(r);
+    if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = make_float2(r.m, r.o);
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    r = Run();
+    if (lane < NW) { const float2 v = red[turn][lane]; r.m = v.x; r.o = v.y; }
+    warp_join(r);
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_row(T* d, int V, int threads) {
+    constexpr int K = K_OF<T>;
+    const int off = row_off(d);
+    float z[K];
+#pragma unroll
+    for (int q = 0; q < K; q++) z[q] = 0.f;
+    for (int e0 = (int)threadIdx.x * K - off; e0 < V; e0 += threads * K) store_piece(d, e0, V, true, z);
+}
+
+template <typename T>
+__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, int y, float m, float f, float ft) {
+    constexpr int K = K_OF<T>;
+    float x[K];
+    unpack<T>(raw, x);
+#pragma unroll
+    for (int q = 0; q < K; q++) x[q] = f * numerator(x[q], m);
+    if (y >= e0 && y < e0 + K) {
+#pragma unroll
+        for (int q = 0; q < K; q++) x[q] = q == y - e0 ? ft : x[q];
+    }
+    store_piece(d, e0, V, same, x);
+}
+
+// Rows that fit a ring of S pieces a thread in shared memory. Every thread copies its own pieces in asynchronously and
+// reads only those, so the copies need no barrier: the ring runs ahead into the next rows while this row is reduced, and
+// a piece leaves it when the row's gradient has been formed from it. One copy group is committed for every step of either
+// pass (an empty one where nothing is copied), so at least S - 1 groups lie behind the one that a step needs.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, int THREADS, int S, int MODE>
+__global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
+    constexpr int K = K_OF<T>;
+    extern __shared__ uint4 ring[];                          // [S][THREADS]
+    __shared__ float2 red[2][THREADS / 32];
+    const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
+    if (MODE != LOGP && k.skip_one && scale == 1.f) return;
+    const int tid = threadIdx.x, V = (int)k.b.V;
+    const int64_t rows = k.b.n * k.b.W, stride = gridDim.x;
+    const auto target_of = [&](int64_t r) { return r < rows ? target(k.b, r / k.b.W, r % k.b.W) : -1; };
+    const auto row_at = [&](int64_t r) { return (const T*)k.b.logits + (r / k.b.W) * k.b.logits_n + (r % k.b.W) * k.b.logits_w; };
+
+    // what is copied next: piece in_j of row in_row (a counted one), into slot in_slot
+    int64_t in_row = blockIdx.x;
+    int in_j = 0, in_slot = 0;
+    while (in_row < rows && target_of(in_row) < 0) in_row += stride;
+    const T* in_x = in_row < rows ? row_at(in_row) : nullptr;
+    const auto copy_next = [&]() {
+        if (in_row < rows) {
+            const int e0 = (tid + in_j * THREADS) * K - row_off(in_x);
+            uint4* to = &ring[in_slot * THREADS + tid];
+            if (whole<T>(e0, V)) copy16(to, in_x + e0);
+            else if (e0 < V) *to = edge_piece(in_x, e0, V);
+            if (++in_j == steps) {
+                in_j = 0;
+                do in_row += stride; while (in_row < rows && target_of(in_row) < 0);
+                if (in_row < rows) in_x = row_at(in_row);
+            }
+        }
+        if (++in_slot == S) in_slot = 0;
+        copies_commit();
+    };
+#pragma unroll 1
+    for (int s = 0; s < S; s++) copy_next();
+
+    int slot = 0, turn = 0, y = target_of(blockIdx.x);
+    for (int64_t r = blockIdx.x; r < rows; r += stride) {
+        const int64_t i = r / k.b.W, t = r - i * k.b.W;
+        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
+        const int y_next = target_of(r + stride);
+        if (y < 0) {
+            if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
+            if (MODE != LOGP && d) zero_row(d, V, THREADS);
+            if (k.part && tid == 0) k.part[r] = 0;
+            y = y_next;
+            continue;
+        }
+        const T* x = row_at(r);
+        const int off = row_off(x);
+        const End end = end_args<MODE>(k, i, t);
+        const float xt = f32(x[y]);
+        Run run;
+        int at = slot;
+        for (int j = 0; j < steps; j++) {
+            const int e0 = (tid + j * THREADS) * K - off;
+            copies_wait<S - 1>();
+            if (e0 < V) {
+                float v[K];
+                unpack<T>(ring[at * THREADS + tid], v);
+                take(run, v, y - e0);
+            }
+            if (++at == S) at = 0;
+            if (MODE == LOGP || !d) copy_next(); else copies_commit();
+        }
+        block_join<THREADS>(run, red, turn);
+        turn ^= 1;
+        float e;
+        double term;
+        const float lp = row_logp(run.m, run.o, xt, &e), g = row_end<MODE>(k, end, lp, scale, term);
+        if (tid == 0) {
+            if (MODE == LOGP && k.logp) k.logp[r] = lp;
+            if (k.part) k.part[r] = term;
+        }
+        if (MODE != LOGP && d) {
+            const bool same = alike(x, d);
+            const float inv = 1.f / (run.o + e), f = -g * inv, ft = g * (run.o * inv);
+            at = slot;
+            for (int j = 0; j < steps; j++) {
+                const int e0 = (tid + j * THREADS) * K - off;
+                if (e0 < V) grad_piece(ring[at * THREADS + tid], d, e0, V, same, y, run.m, f, ft);
+                if (++at == S) at = 0;
+                copy_next();
+            }
+        }
+        slot = at;
+        y = y_next;
+    }
+    copies_wait<0>();
+}
+
+// Rows of any length: read twice, the second time for the gradient.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
+    constexpr int K = K_OF<T>, THREADS = 512, U = 4;
+    __shared__ float2 red[2][THREADS / 32];
+    const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
+    if (MODE != LOGP && k.skip_one && scale == 1.f) return;
+    const int tid = threadIdx.x, V = (int)k.b.V;
+    const int64_t rows = k.b.n * k.b.W;
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const int64_t i = r / k.b.W, t = r - i * k.b.W;
+        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
+        const int y = target(k.b, i, t);
+        if (y < 0) {
+            if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
+            if (MODE != LOGP && d) zero_row(d, V, THREADS);
+            if (k.part && tid == 0) k.part[r] = 0;
+            continue;
+        }
+        const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
+        const int off = row_off(x);
+        const End end = end_args<MODE>(k, i, t);
+        const float xt = f32(x[y]);
+        // pieces of the row, U at a time in flight; 64-bit places, as the last step may pass 2^31
+        const auto pieces = [&](auto&& f) {
+            for (int64_t p0 = tid; p0 * K - off < V; p0 += THREADS * U) {
+                uint4 raw[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int64_t e0 = (p0 + u * THREADS) * K - off;
+                    if (e0 >= V) continue;
+                    raw[u] = whole<T>((int)e0, V) ? *(const uint4*)(x + e0) : edge_piece(x, (int)e0, V);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int64_t e0 = (p0 + u * THREADS) * K - off;
+                    if (e0 < V) f(raw[u], (int)e0);
+                }
+            }
+        };
+        Run run;
+        pieces([&](const uint4& raw, int e0) {
+            float v[K];
+            unpack<T>(raw, v);
+            take(run, v, y - e0);
+        });
+        block_join<THREADS>(run, red, turn);
+        turn ^= 1;
+        float e;
+        double term;
+        const float lp = row_logp(run.m, run.o, xt, &e), g = row_end<MODE>(k, end, lp, scale, term);
+        if (tid == 0) {
+            if (MODE == LOGP && k.logp) k.logp[r] = lp;
+            if (k.part) k.part[r] = term;
+        }
+        if (MODE != LOGP && d) {
+            const bool same = alike(x, d);
+            const float inv = 1.f / (run.o + e), f = -g * inv, ft = g * (run.o * inv);
+            pieces([&](const uint4& raw, int e0) { grad_piece(raw, d, e0, V, same, y, run.m, f, ft); });
+        }
     }
 }
 
@@ -260,7 +614,7 @@ int launched() {
 
 const char* bad_batch(const pv_scored* b) {
     if (!b) return "batch: NULL";
-    if (b->n < 0 || b->W < 0 || b->W >= (1ll << 31) || b->V < 1 || b->V >= (1ll << 31)) return "batch: n, W or V out of range";
+    if (b->n < 0 || b->W < 0 || b->W >= (1ll << 31) || b->V < 1 || b->V >= (1ll << 30)) return "batch: n, W or V out of range";
     if (b->shift < 0) return "batch: shift is negative";
     if (b->type < PV_T_BF16 || b->type > PV_T_FP32) return "batch: logits are bf16, fp16 or fp32";
     if (b->token_bytes != 1 && b->token_bytes != 8) return "batch: tokens are uint8 or int64";
@@ -270,11 +624,20 @@ const char* bad_batch(const pv_scored* b) {
     return nullptr;
 }
 
-struct Plan { int32_t rows; int64_t tpw, tiles, spans; };
+// How a batch is run, by its rows' 16-byte pieces (one more than their bytes say where a row may start inside one):
+// up to 256 in registers, G lanes a row; up to RING_MOST in a ring in shared memory, a block a row; else read twice.
+enum { GROUP, RING, LONG };
+struct Plan { int form, pieces; int64_t tpw, tiles, spans; };
+constexpr int RING_MOST = 26 * 512;
+int size_of(int type) { return type == PV_T_FP32 ? 4 : 2; }
 Plan plan_of(const pv_scored& b) {
     Plan p;
-    p.rows = b.V >= 512 ? 1 : 16;
-    p.tpw = (b.W + p.rows - 1) / p.rows;
+    const int64_t size = size_of(b.type), k = 16 / size;
+    const bool aligned = (((uintptr_t)b.logits | (uint64_t)(b.logits_n * size) | (uint64_t)(b.logits_w * size)) & 15) == 0;
+    const int64_t pieces = (b.V + k - 1 + (aligned ? 0 : k - 1)) / k;
+    p.pieces = (int)std::min<int64_t>(pieces, 1 << 30);
+    p.form = pieces <= 256 ? GROUP : pieces <= RING_MOST ? RING : LONG;
+    p.tpw = p.form == GROUP ? (b.W + TILE - 1) / TILE : b.W;
     p.tiles = b.n * p.tpw;
     p.spans = (b.W + COUNT_SPAN - 1) / COUNT_SPAN;
     return p;
@@ -291,15 +654,66 @@ Scratch scratch_of(const pv_scored& b, const Plan& p, void* work) {
     return s;
 }
 
-template <int MODE>
-int launch_rows(const Rows& k, cudaStream_t st) {
+// a persistent grid: as many blocks as are resident, at most one per `per_block` of the work
+template <typename F>
+unsigned grid_of(F* f, int threads, size_t smem, int64_t blocks) {
+    int per_sm = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, f, threads, smem) != cudaSuccess || per_sm < 1) per_sm = 1;
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)SMS * per_sm));
+}
+
+template <typename T, int G, int NV, int MODE>
+void group_rows(const Rows& k, cudaStream_t st) {
+    const auto f = rows_group_kernel<T, G, NV, MODE>;
     const int64_t tiles = k.b.n * k.tpw;
-    if (tiles == 0) return PV_OK;
-    const unsigned grid = (unsigned)std::min<int64_t>((tiles + 7) / 8, SMS * 8);
+    static const unsigned most = grid_of(f, 256, 0, 1 << 20);
+    f<<<(unsigned)std::min<int64_t>((tiles + 7) / 8, most), 256, 0, st>>>(k);
+}
+
+template <typename T, int THREADS, int S, int MODE>
+void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
+    constexpr int SMEM = S * THREADS * 16;
+    const auto f = rows_ring_kernel<T, THREADS, S, MODE>;
+    static thread_local uint64_t set = 0;                    // devices whose attribute is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(set >> dev & 1)) {
+        cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (dev < 64) set |= 1ull << dev;
+    }
+    static const unsigned most = grid_of(f, THREADS, SMEM, 1 << 20);
+    f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), THREADS, SMEM, st>>>(k, (pieces + THREADS - 1) / THREADS);
+}
+
+template <typename T, int MODE>
+void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
+    if (p.form == LONG) {
+        const auto f = rows_long_kernel<T, MODE>;
+        static const unsigned most = grid_of(f, 512, 0, 1 << 20);
+        f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
+    } else if (p.form == RING) {
+        if (p.pieces <= 128 * 8) ring_rows<T, 128, 12, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 256 * 16) ring_rows<T, 256, 24, MODE>(k, p.pieces, st);
+        else ring_rows<T, 512, 26, MODE>(k, p.pieces, st);
+    } else {
+        if (p.pieces <= 1) group_rows<T, 1, 1, MODE>(k, st);
+        else if (p.pieces <= 2) group_rows<T, 1, 2, MODE>(k, st);
+        else if (p.pieces <= 4) group_rows<T, 1, 4, MODE>(k, st);
+        else if (p.pieces <= 16) group_rows<T, 4, 4, MODE>(k, st);
+        else if (p.pieces <= 32) group_rows<T, 8, 4, MODE>(k, st);
+        else if (p.pieces <= 64) group_rows<T, 16, 4, MODE>(k, st);
+        else if (p.pieces <= 128) group_rows<T, 32, 4, MODE>(k, st);
+        else group_rows<T, 32, 8, MODE>(k, st);
+    }
+}
+
+template <int MODE>
+int launch_rows(const Rows& k, const Plan& p, cudaStream_t st) {
+    if (k.b.n == 0 || k.b.W == 0) return PV_OK;
     switch (k.b.type) {
-        case PV_T_BF16: rows_any_kernel<__nv_bfloat16, MODE><<<grid, 256, 0, st>>>(k); break;
-        case PV_T_FP16: rows_any_kernel<__half, MODE><<<grid, 256, 0, st>>>(k); break;
-        default: rows_any_kernel<float, MODE><<<grid, 256, 0, st>>>(k);
+        case PV_T_BF16: typed_rows<__nv_bfloat16, MODE>(k, p, st); break;
+        case PV_T_FP16: typed_rows<__half, MODE>(k, p, st); break;
+        default: typed_rows<float, MODE>(k, p, st);
     }
     return launched();
 }
@@ -308,7 +722,6 @@ Rows rows_of(const pv_scored& b, const Plan& p) {
     Rows k = {};
     k.b = b;
     k.tpw = p.tpw;
-    k.rows = p.rows;
     return k;
 }
 
@@ -349,7 +762,7 @@ int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* work, size_t
     k.logp = logp;
     k.part = sums ? s.part : nullptr;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (const int e = launch_rows<LOGP>(k, st)) return e;
+    if (const int e = launch_rows<LOGP>(k, p, st)) return e;
     return sums ? window_sums(p, b->n, s.part, sums, nullptr, st) : PV_OK;
 }
 
@@ -357,10 +770,11 @@ int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t 
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !up) return fail(PV_EARG, "pv_logprobs_grad: NULL gradient");
-    Rows k = rows_of(*b, plan_of(*b));
+    const Plan p = plan_of(*b);
+    Rows k = rows_of(*b, p);
     k.up = up; k.up_n = up_n; k.up_w = up_w;
     k.scale = scale; k.skip_one = scale && skip_one;
-    return launch_rows<GRAD>(k, (cudaStream_t)stream);
+    return launch_rows<GRAD>(k, p, (cudaStream_t)stream);
 }
 
 int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float beta, float smoothing, float* loss, float* margins, float* coef,
@@ -376,7 +790,7 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
         Rows k = rows_of(*b, p);
         k.b.grad = nullptr;
         k.part = s.part;
-        if (const int e = launch_rows<LOGP>(k, st)) return e;
+        if (const int e = launch_rows<LOGP>(k, p, st)) return e;
         if (const int e = window_sums(p, b->n, s.part, nullptr, s.win, st)) return e;
     }
     pairs_kernel<<<1, 1024, 0, st>>>(s.win, b->n, ref, ref_n, beta, smoothing, loss, margins, coef);
@@ -400,7 +814,7 @@ int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* 
         k.part = s.part;
         k.a = *a;
         k.weight = weight;
-        if (const int e = launch_rows<POLICY>(k, st)) return e;
+        if (const int e = launch_rows<POLICY>(k, p, st)) return e;
     }
     total_kernel<<<1, 1024, 0, st>>>(s.part, p.tiles, loss);
     return launched();
@@ -411,11 +825,12 @@ int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* we
     if (const int e = bad_policy(b, a)) return e;
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !weight || !a->old || !a->adv) return fail(PV_EARG, "pv_policy_grad: NULL argument");
-    Rows k = rows_of(*b, plan_of(*b));
+    const Plan p = plan_of(*b);
+    Rows k = rows_of(*b, p);
     k.a = *a;
     k.weight = weight;
     k.scale = scale; k.skip_one = scale && skip_one;
-    return launch_rows<POLICY>(k, (cudaStream_t)stream);
+    return launch_rows<POLICY>(k, p, (cudaStream_t)stream);
 }
 
 }  // extern "C"

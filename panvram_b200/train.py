@@ -48,8 +48,8 @@ def _batch(logits, tokens, mask, shift, ignore):
     sn, sw, sv = logits.stride()
     if V < 1 or (V > 1 and sv != 1):
         raise ValueError("logits: at least one word, and a position's words contiguous")
-    if W >= 1 << 31 or V >= 1 << 31:
-        raise ValueError("logits: W and V below 2^31")
+    if W >= 1 << 31 or V >= 1 << 30:
+        raise ValueError("logits: W below 2^31 and V below 2^30")
     if not isinstance(tokens, torch.Tensor) or tokens.shape != (n, W) or tokens.dtype not in (torch.uint8, torch.int64):
         raise ValueError("tokens: a uint8 or int64 tensor [n, W]")
     ids = tokens.dtype == torch.int64
