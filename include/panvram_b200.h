@@ -468,7 +468,7 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
 typedef struct pv_policy_args {
     const float *old, *adv, *ref;
     int64_t old_n, old_w, adv_n, adv_w, ref_n, ref_w;
-    float clip_low, clip_high, kl;
+    float clip_low, clip_high, kl, scale;
     int32_t by_window;
 } pv_policy_args;
 int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* weight, void* work, size_t work_bytes, void* stream);

@@ -78,7 +78,7 @@ class Scored(ctypes.Structure):
 class PolicyArgs(ctypes.Structure):
     _fields_ = ([(k, ctypes.c_void_p) for k in ("old", "adv", "ref")]
                 + [(k, ctypes.c_int64) for k in ("old_n", "old_w", "adv_n", "adv_w", "ref_n", "ref_w")]
-                + [(k, ctypes.c_float) for k in ("clip_low", "clip_high", "kl")] + [("by_window", ctypes.c_int32)])
+                + [(k, ctypes.c_float) for k in ("clip_low", "clip_high", "kl", "scale")] + [("by_window", ctypes.c_int32)])
 
 
 class Tensors(ctypes.Structure):

@@ -1,11 +1,13 @@
 // pv_train.cu - log-probabilities of windows' tokens under a model's logits, the preference loss over pairs of windows
 // and the clipped policy loss with a KL term, forward and backward (include/panvram_b200.h pv_logprobs ... pv_policy_grad).
 //
-// The mathematics, per row (a position's V logits x, its target y): m = max x, numerators e_j = 2^((x_j - m) log2 e),
-// their sum s, p_j = e_j / s, log p_y = x_y - m - log s, and d log p_y / d x_j = [j = y] - p_j.
-// The difference comes before the product (not one FMA with m log2 e): logits at their type's lowest or highest value
-// would overflow there. The sum o over the other words is kept apart from the target's numerator e: 1 - p_y = o / (o + e)
-// and, where e >= o, log p_y = -log1p(o / e), so neither loses its digits where the model is nearly sure.
+// The mathematics, per row (a position's V logits x, its target y): with L = log2(e), a reference c and e_j = 2^(x_j L - c),
+// s = sum e_j, p_j = e_j / s, log p_y = ln2 (x_y L - c) - log s, and d log p_y / d x_j = [j = y] - p_j.
+// c is the rounded product of the maximum and L. Its rounding is the same for every numerator and for log p_y, so it
+// cancels, and x_j L - c is one FMA. Where the maximum is beyond 2^29 (that rounding would then be too large; the product
+// overflows at the lowest or highest value of bf16 and fp32) the difference comes first: e_j = 2^((x_j - max) L).
+// The sum o over the other words is kept apart from the target's numerator e: 1 - p_y = o / (o + e) and, where e >= o,
+// log p_y = -log1p(o / e), so neither loses its digits where the model is nearly sure.
 // All statistics are in 32 bits; sums over rows are in 64 bits and in a fixed order (a partial sum per tile of rows, then
 // over the tiles), so results do not change from call to call.
 #include <cuda_bf16.h>
@@ -24,7 +26,7 @@ namespace {
 
 using pvb::g_cuda_err;
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int SMS = 148;
 
 // ---------------------------------------------------------------- elements
@@ -71,13 +73,63 @@ __device__ __forceinline__ int target(const pv_scored& b, int64_t i, int64_t t) 
     return y < 0 || y >= b.V || y == b.ignore ? -1 : (int)y;
 }
 
-__device__ __forceinline__ float numerator(float x, float m) { return ex2((x - m) * LOG2E); }
+// a row's (or a thread's part of a row's) reference
+__device__ __forceinline__ bool far(float m) { return !(fabsf(m) < 536870912.f); }     // infinities too
+__device__ __forceinline__ float ref_of(float m) { return far(m) ? 0.f : m * LOG2E; }
+__device__ __forceinline__ float exponent(float x, float m, float c) { return far(m) ? (x - m) * LOG2E : fmaf(x, LOG2E, -c); }
+// what a sum of numerators with the maximum m is multiplied by, to be one with the maximum M >= m
+__device__ __forceinline__ float rescale(float m, float M) { return ex2(far(m) || far(M) ? (m - M) * LOG2E : ref_of(m) - ref_of(M)); }
 
-// log p of the target with logit xt: m the maximum, o the sum of the other words' numerators; *e receives the target's
-__device__ __forceinline__ float row_logp(float m, float o, float xt, float* e) {
-    *e = numerator(xt, m);
-    if (m == -INFINITY) return NAN;                         // nothing to normalise by
-    return *e >= o ? -log1pf(o / *e) : (xt - m) - logf(o + *e);
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void halves(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+// x becomes its numerators, two to an FMA
+template <int K>
+__device__ __forceinline__ void numerators(float (&x)[K], float m, float c) {
+    if (far(m)) {
+#pragma unroll
+        for (int q = 0; q < K; q++) x[q] -= m;
+    }
+    const uint64_t l = pair(LOG2E, LOG2E), nc = pair(-c, -c);
+#pragma unroll
+    for (int q = 0; q < K; q += 2) {
+        uint64_t v;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pair(x[q], x[q + 1])), "l"(l), "l"(nc));
+        float a, b;
+        halves(v, a, b);
+        x[q] = ex2(a);
+        x[q + 1] = ex2(b);
+    }
+}
+template <int K>
+__device__ __forceinline__ float sum_of(const float (&x)[K]) {
+    uint64_t v = pair(x[0], x[1]);
+#pragma unroll
+    for (int q = 2; q < K; q += 2) asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(v), "l"(pair(x[q], x[q + 1])));
+    float a, b;
+    halves(v, a, b);
+    return a + b;
+}
+template <int K>
+__device__ __forceinline__ void times(float (&x)[K], float f) {
+    const uint64_t ff = pair(f, f);
+#pragma unroll
+    for (int q = 0; q < K; q += 2) {
+        uint64_t v;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pair(x[q], x[q + 1])), "l"(ff));
+        halves(v, x[q], x[q + 1]);
+    }
+}
+
+// log p of the target: t its exponent, e its numerator, o the sum of the others', m the maximum. Where the target does not
+// outweigh the others the sum is about 1 or more, and log1p of what it is above 1 is its logarithm.
+__device__ __forceinline__ float row_logp(float m, float o, float t, float e) {
+    const bool sure = e >= o;
+    const float l = log1pf(sure ? o / e : (o + e) - 1.f);
+    return m == -INFINITY ? NAN : (sure ? 0.f : t * LN2) - l;            // -inf: nothing to normalise by
 }
 
 // exp(d) - d - 1: by its series near 0, where the difference would lose its digits
@@ -88,38 +140,40 @@ __device__ __forceinline__ float kl_term(float d, float em1) {
 }
 
 // What a counted row's end reads, loaded before its logits are waited for.
-struct End { float a, old, ref; double w; };
+struct End { float a, old, ref; };
 template <int MODE>
 __device__ __forceinline__ End end_args(const Rows& k, int64_t i, int64_t t) {
-    End e = {0.f, 0.f, 0.f, 0.0};
+    End e = {0.f, 0.f, 0.f};
     if (MODE == GRAD) e.a = k.up[i * k.up_n + t * k.up_w];
     if (MODE == POLICY) {
         e.a = k.a.adv[i * k.a.adv_n + t * k.a.adv_w];
         e.old = k.a.old[i * k.a.old_n + t * k.a.old_w];
         if (k.a.ref) e.ref = k.a.ref[i * k.a.ref_n + t * k.a.ref_w];
-        e.w = k.weight[i];
     }
     return e;
 }
 
-// From a counted row's log-probability its term of the sum and its derivative (the result).
+// From a counted row's log-probability its term of the sum (before the window's weight w) and its derivative, times w and
+// the upstream scale (the result).
 template <int MODE>
-__device__ __forceinline__ float row_end(const Rows& k, const End& e, float lp, float scale, double& term) {
+__device__ __forceinline__ float row_end(const Rows& k, const End& e, float lp, float w, float scale, float& term) {
     if (MODE == LOGP) { term = lp; return 0.f; }
-    if (MODE == GRAD) { term = 0; return e.a * scale; }
+    if (MODE == GRAD) { term = 0.f; return e.a * scale; }
     const float r = expf(lp - e.old);
     const float one = e.a == 0.f ? 0.f : r * e.a;
     const float two = fminf(fmaxf(r, 1.f - k.a.clip_low), 1.f + k.a.clip_high) * e.a;
     const bool free = !(one > two);                          // NaN stays
-    float v = free ? -one : -two, g = free ? -one : 0.f;
+    float g = free ? -one : 0.f;
+    term = free ? -one : -two;
     if (k.a.ref) {
         const float d = e.ref - lp, em1 = expm1f(d);
-        v += k.a.kl * kl_term(d, em1);
+        term += k.a.kl * kl_term(d, em1);
         g -= k.a.kl * em1;
     }
-    term = (double)v * e.w;
-    return g * (float)e.w * scale;
+    return g * w * scale;
 }
+template <int MODE>
+__device__ __forceinline__ double weight_of(const Rows& k, int64_t i) { return MODE == POLICY ? k.weight[i] : 1.0; }
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -174,6 +228,21 @@ template <> __device__ __forceinline__ uint4 pack<__half>(const float (&x)[8]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+template <typename T> __device__ __forceinline__ float piece_max(const uint4& r);
+template <> __device__ __forceinline__ float piece_max<float>(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+}
+template <> __device__ __forceinline__ float piece_max<__nv_bfloat16>(const uint4& r) {
+    const __nv_bfloat162* w = (const __nv_bfloat162*)&r;
+    const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+template <> __device__ __forceinline__ float piece_max<__half>(const uint4& r) {
+    const __half2* w = (const __half2*)&r;
+    const __half2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
 // A row of V elements seen as aligned 16-byte pieces: piece v holds elements v K - off ... + K, off = how far into its
 // first piece the row starts. The pieces at the row's ends are moved by element, so nothing outside the row is touched.
 template <typename T>
@@ -216,103 +285,112 @@ __global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
         const int64_t i = tile / k.tpw, t0 = (tile - i * k.tpw) * TILE;
         const int rows = (int)min((int64_t)TILE, k.b.W - t0);
         const int y_l = lane < rows ? target(k.b, i, t0 + lane) : -1;
+        End end_l = {0.f, 0.f, 0.f};
+        if (y_l >= 0) end_l = end_args<MODE>(k, i, t0 + lane);
+        const double w = weight_of<MODE>(k, i);
+        const T* const x0 = (const T*)k.b.logits + i * k.b.logits_n + t0 * k.b.logits_w;
+        T* const d0 = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t0 * k.b.grad_w : nullptr;
         double sum = 0;
         for (int s0 = 0; s0 < rows; s0 += RP) {
-            const int row = s0 + grp;
-            const int64_t t = t0 + row;
-            const int y = __shfl_sync(~0u, y_l, row);
-            const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
+            const int row = s0 + grp, y = __shfl_sync(~0u, y_l, row);
+            const T* x = x0 + row * k.b.logits_w;
             const int off = row_off(x);
             uint4 raw[NV];
-            End end = {0.f, 0.f, 0.f, 0.0};
             float xt = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; j++) raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
             if (y >= 0) {
-                end = end_args<MODE>(k, i, t);
-                xt = f32(x[y]);
 #pragma unroll
                 for (int j = 0; j < NV; j++) {
                     const int e0 = (sub + j * G) * K - off;
                     if (whole<T>(e0, V)) raw[j] = *(const uint4*)(x + e0);
                     else if (e0 < V) raw[j] = edge_piece(x, e0, V);
                 }
+                xt = f32(x[y]);
             }
-            float m = -INFINITY, o = 0.f, e[NV][K];
+            float m = piece_max<T>(raw[0]);
+#pragma unroll
+            for (int j = 1; j < NV; j++) m = fmaxf(m, piece_max<T>(raw[j]));
+#pragma unroll
+            for (int s = G / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, s));
+            const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
+            float e[NV][K], o = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 unpack<T>(raw[j], e[j]);
-#pragma unroll
-                for (int q = 0; q < K; q++) m = fmaxf(m, e[j][q]);
-            }
-#pragma unroll
-            for (int s = G / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, s));
-#pragma unroll
-            for (int j = 0; j < NV; j++) {
-                const int at = y - ((sub + j * G) * K - off);
-                float part = 0.f;
-#pragma unroll
-                for (int q = 0; q < K; q++) {
-                    e[j][q] = numerator(e[j][q], m);
-                    part += q == at ? 0.f : e[j][q];
-                }
-                o += part;
+                numerators(e[j], m, c);
+                o += sum_of(e[j]);
             }
 #pragma unroll
             for (int s = G / 2; s; s >>= 1) o += __shfl_xor_sync(~0u, o, s);
-            float et, lp = 0.f, g = 0.f;
-            double term = 0;
+            o -= et;
+            // where the target outweighs the others that difference has lost their digits: they are summed by themselves
+            if (__any_sync(~0u, y >= 0 && !(et < o))) {
+                float p = 0.f;
+#pragma unroll
+                for (int j = 0; j < NV; j++) {
+                    const int at = y - ((sub + j * G) * K - off);
+#pragma unroll
+                    for (int q = 0; q < K; q++) p += q == at ? 0.f : e[j][q];
+                }
+#pragma unroll
+                for (int s = G / 2; s; s >>= 1) p += __shfl_xor_sync(~0u, p, s);
+                if (!(et < o)) o = p;
+            }
+            const End end = {MODE != LOGP ? __shfl_sync(~0u, end_l.a, row) : 0.f, MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
+                             MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
+            float lp = 0.f, g = 0.f, term = 0.f;
             if (y >= 0) {
-                lp = row_logp(m, o, xt, &et);
-                g = row_end<MODE>(k, end, lp, scale, term);
-                if (sub == 0) sum += term;
+                if (MODE != GRAD) lp = row_logp(m, o, t, et);
+                g = row_end<MODE>(k, end, lp, (float)w, scale, term);
+                if (sub == 0) sum += (double)term;
             }
             if (MODE == LOGP) {
-                if (k.logp && sub == 0 && row < rows) k.logp[i * k.b.W + t] = lp;
-            } else if (k.b.grad && row < rows) {
-                T* d = (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w;
+                if (k.logp && sub == 0 && row < rows) k.logp[i * k.b.W + t0 + row] = lp;
+            } else if (d0 && row < rows) {
+                T* d = d0 + row * k.b.grad_w;
                 const bool same = alike(x, d);
-                const float inv = 1.f / (o + et), f = -g * inv, ft = g * (o * inv);
+                const float inv = 1.f / (o + et), f = y < 0 ? 0.f : -g * inv;
 #pragma unroll
                 for (int j = 0; j < NV; j++) {
                     const int e0 = (sub + j * G) * K - off;
-                    float v[K];
+                    if (y < 0) {
 #pragma unroll
-                    for (int q = 0; q < K; q++) v[q] = y < 0 ? 0.f : q == y - e0 ? ft : e[j][q] * f;
-                    if (e0 < V) store_piece(d, e0, V, same, v);
+                        for (int q = 0; q < K; q++) e[j][q] = 0.f;
+                    }
+                    times(e[j], f);
+                    if (e0 < V) store_piece(d, e0, V, same, e[j]);
+                    if (y >= e0 && y < e0 + K && y >= 0) d[y] = from32<T>(g * (o * inv));
                 }
             }
         }
         if (k.part) {
             sum = warp_sum(sum);
-            if (lane == 0) k.part[tile] = sum;
+            if (lane == 0) k.part[tile] = sum * w;
         }
     }
 }
 
 // ---------------------------------------------------------------- longer rows: a block a row
-// the running maximum and sum of a thread; `base`: the maximum, or 0 where there is none yet
-struct Run { float m = -INFINITY, o = 0.f; };
-template <int K>
-__device__ __forceinline__ void take(Run& r, const float (&x)[K], int at) {       // at: the target's place among them, if any
-    float m = x[0];
-#pragma unroll
-    for (int q = 1; q < K; q++) m = fmaxf(m, x[q]);
-    if (m > r.m) { r.o *= numerator(r.m, m); r.m = m; }
-    const float base = r.m == -INFINITY ? 0.f : r.m;
-    float part = 0.f;
+// the running maximum and sum of a thread
+struct Run { float m = -INFINITY, c = 0.f, o = 0.f; };
+template <typename T>
+__device__ __forceinline__ void take(Run& r, const uint4& raw, int at) {          // at: the target's place in the piece, if any
+    constexpr int K = K_OF<T>;
+    const float m = piece_max<T>(raw);
+    if (m > r.m) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }            // from nothing: 0 times 0
+    float x[K];
+    unpack<T>(raw, x);
+    numerators(x, r.m == -INFINITY ? 0.f : r.m, r.c);                             // nothing but -inf so far: numerators of 0
     if (at >= 0 && at < K) {
 #pragma unroll
-        for (int q = 0; q < K; q++) part += q == at ? 0.f : numerator(x[q], base);
-    } else {
-#pragma unroll
-        for (int q = 0; q < K; q++) part += numerator(x[q], base);
+        for (int q = 0; q < K; q++) x[q] = q == at ? 0.f : x[q];
     }
-    r.o += part;
+    r.o += sum_of(x);
 }
 __device__ __forceinline__ void warp_join(Run& r) {
     const float m = warp_max(r.m);
-    r.o = warp_sum(r.m == m ? r.o : r.o * numerator(r.m, m));
+    r.o = warp_sum(r.m == m ? r.o : r.o * rescale(r.m, m));
     r.m = m;
 }
 // The block's: one barrier a row, two buffers in turn (a buffer is written again only after the next row's barrier, which
@@ -327,6 +405,7 @@ __device__ __forceinline__ void block_join(Run& r, float2 (&red)[2][THREADS / 32
     r = Run();
     if (lane < NW) { const float2 v = red[turn][lane]; r.m = v.x; r.o = v.y; }
     warp_join(r);
+    r.c = ref_of(r.m);
 }
 
 template <typename T>
@@ -340,17 +419,14 @@ __device__ __forceinline__ void zero_row(T* d, int V, int threads) {
 }
 
 template <typename T>
-__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, int y, float m, float f, float ft) {
+__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, int y, const Run& r, float f, float ft) {
     constexpr int K = K_OF<T>;
     float x[K];
     unpack<T>(raw, x);
-#pragma unroll
-    for (int q = 0; q < K; q++) x[q] = f * numerator(x[q], m);
-    if (y >= e0 && y < e0 + K) {
-#pragma unroll
-        for (int q = 0; q < K; q++) x[q] = q == y - e0 ? ft : x[q];
-    }
+    numerators(x, r.m, r.c);
+    times(x, f);
     store_piece(d, e0, V, same, x);
+    if (y >= e0 && y < e0 + K) d[y] = from32<T>(ft);
 }
 
 // Rows that fit a ring of S pieces a thread in shared memory. Every thread copies its own pieces in asynchronously and
@@ -413,6 +489,7 @@ __global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
         const T* x = row_at(r);
         const int off = row_off(x);
         const End end = end_args<MODE>(k, i, t);
+        const double w = weight_of<MODE>(k, i);
         const float xt = f32(x[y]);
         Run run;
         int at = slot;
@@ -420,21 +497,19 @@ __global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
             const int e0 = (tid + j * THREADS) * K - off;
             copies_wait<S - 1>();
             if (e0 < V) {
-                float v[K];
-                unpack<T>(ring[at * THREADS + tid], v);
-                take(run, v, y - e0);
+                take<T>(run, ring[at * THREADS + tid], y - e0);
             }
             if (++at == S) at = 0;
             if (MODE == LOGP || !d) copy_next(); else copies_commit();
         }
         block_join<THREADS>(run, red, turn);
         turn ^= 1;
-        float e;
-        double term;
-        const float lp = row_logp(run.m, run.o, xt, &e), g = row_end<MODE>(k, end, lp, scale, term);
+        const float ex = exponent(xt, run.m, run.c), e = ex2(ex), lp = row_logp(run.m, run.o, ex, e);
+        float term;
+        const float g = row_end<MODE>(k, end, lp, (float)w, scale, term);
         if (tid == 0) {
             if (MODE == LOGP && k.logp) k.logp[r] = lp;
-            if (k.part) k.part[r] = term;
+            if (k.part) k.part[r] = (double)term * w;
         }
         if (MODE != LOGP && d) {
             const bool same = alike(x, d);
@@ -442,7 +517,7 @@ __global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
             at = slot;
             for (int j = 0; j < steps; j++) {
                 const int e0 = (tid + j * THREADS) * K - off;
-                if (e0 < V) grad_piece(ring[at * THREADS + tid], d, e0, V, same, y, run.m, f, ft);
+                if (e0 < V) grad_piece(ring[at * THREADS + tid], d, e0, V, same, y, run, f, ft);
                 if (++at == S) at = 0;
                 copy_next();
             }
@@ -476,6 +551,7 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
         const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
         const int off = row_off(x);
         const End end = end_args<MODE>(k, i, t);
+        const double w = weight_of<MODE>(k, i);
         const float xt = f32(x[y]);
         // pieces of the row, U at a time in flight; 64-bit places, as the last step may pass 2^31
         const auto pieces = [&](auto&& f) {
@@ -496,23 +572,21 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
         };
         Run run;
         pieces([&](const uint4& raw, int e0) {
-            float v[K];
-            unpack<T>(raw, v);
-            take(run, v, y - e0);
+            take<T>(run, raw, y - e0);
         });
         block_join<THREADS>(run, red, turn);
         turn ^= 1;
-        float e;
-        double term;
-        const float lp = row_logp(run.m, run.o, xt, &e), g = row_end<MODE>(k, end, lp, scale, term);
+        const float ex = exponent(xt, run.m, run.c), e = ex2(ex), lp = row_logp(run.m, run.o, ex, e);
+        float term;
+        const float g = row_end<MODE>(k, end, lp, (float)w, scale, term);
         if (tid == 0) {
             if (MODE == LOGP && k.logp) k.logp[r] = lp;
-            if (k.part) k.part[r] = term;
+            if (k.part) k.part[r] = (double)term * w;
         }
         if (MODE != LOGP && d) {
             const bool same = alike(x, d);
             const float inv = 1.f / (run.o + e), f = -g * inv, ft = g * (run.o * inv);
-            pieces([&](const uint4& raw, int e0) { grad_piece(raw, d, e0, V, same, y, run.m, f, ft); });
+            pieces([&](const uint4& raw, int e0) { grad_piece(raw, d, e0, V, same, y, run, f, ft); });
         }
     }
 }
@@ -575,7 +649,7 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const double* sums, int64_t
 }
 
 // counted positions of each window: a block per (window, part of it), then one block turns them into weights
-constexpr int COUNT_SPAN = 16384;
+constexpr int COUNT_SPAN = 2048;
 __global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, int32_t* counts) {
     for (int64_t q = blockIdx.x; q < b.n * spans; q += gridDim.x) {
         const int64_t i = q / spans, t0 = (q - i * spans) * COUNT_SPAN, t1 = min(t0 + (int64_t)COUNT_SPAN, b.W);
@@ -585,7 +659,7 @@ __global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, 
         if (threadIdx.x == 0) counts[q] = v;
     }
 }
-__global__ void __launch_bounds__(1024) weights_kernel(const int32_t* counts, int64_t n, int64_t spans, int by_window, double* weight) {
+__global__ void __launch_bounds__(1024) weights_kernel(const int32_t* counts, int64_t n, int64_t spans, int by_window, double scale, double* weight) {
     double all = 0, some = 0;
     for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
         int64_t c = 0;
@@ -598,7 +672,7 @@ __global__ void __launch_bounds__(1024) weights_kernel(const int32_t* counts, in
     some = block_sum(some);
     for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
         const double c = weight[i];
-        weight[i] = by_window ? (c > 0 ? 1.0 / (c * some) : 0.0) : (all > 0 ? 1.0 / all : 0.0);
+        weight[i] = by_window ? (c > 0 ? scale / (c * some) : 0.0) : (all > 0 ? scale / all : 0.0);
     }
 }
 
@@ -737,6 +811,7 @@ int window_sums(const Plan& p, int64_t n, const double* part, float* sums, doubl
 
 int bad_policy(const pv_scored* b, const pv_policy_args* a) {
     if (!a) return fail(PV_EARG, "pv_policy: NULL arguments");
+    if (!(a->scale >= 0.f)) return fail(PV_EARG, "pv_policy: scale is negative");
     if (!(a->clip_low >= 0.f) || !(a->clip_high >= 0.f)) return fail(PV_EARG, "pv_policy: clip is negative");
     if (!(a->kl == 0.f) && !a->ref && b->n && b->W) return fail(PV_EARG, "pv_policy: a KL term without reference log-probabilities");
     return PV_OK;
@@ -808,7 +883,7 @@ int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* 
     const cudaStream_t st = (cudaStream_t)stream;
     if (b->n) {
         count_kernel<<<(unsigned)std::min<int64_t>(b->n * std::max<int64_t>(p.spans, 1), SMS * 8), 256, 0, st>>>(*b, p.spans, s.counts);
-        weights_kernel<<<1, 1024, 0, st>>>(s.counts, b->n, p.spans, a->by_window, weight);
+        weights_kernel<<<1, 1024, 0, st>>>(s.counts, b->n, p.spans, a->by_window, (double)a->scale, weight);
         if (const int e = launched()) return e;
         Rows k = rows_of(*b, p);
         k.part = s.part;

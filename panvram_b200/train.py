@@ -17,6 +17,8 @@ gradient has their type. Arguments other than the logits are constants. A loss k
 backward pass: with Cohort.sampler, run it before the sampler's next call overwrites its windows."""
 import ctypes
 import math
+from array import array
+from contextlib import nullcontext
 
 import torch
 
@@ -24,6 +26,7 @@ from . import _C
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ready = set()
+_here = nullcontext()
 
 
 def _failed(what):
@@ -88,70 +91,63 @@ def _number(v, name, low, high=math.inf):
     return v
 
 
-def _work(b, dev):
-    need = _C._lib.pv_score_work_bytes(ctypes.byref(b))
-    return torch.empty(need, dtype=torch.uint8, device=dev), need
+def _on(dev):
+    """the device made current for a launch (nothing to do where it is)"""
+    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _stream(dev):
     return torch.cuda.current_stream(dev).cuda_stream
 
 
-def _grad_into(b, logits):
-    """a new gradient of the logits, entered in b"""
-    g = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    b.grad, b.grad_n, b.grad_w = g.data_ptr(), g.stride(0), g.stride(1)
-    return g
+def _work(b, dev, more=0):
+    """scratch for b, and `more` bytes in front of it (rounded up to 16) -> (tensor, address of the scratch, its bytes)"""
+    need, more = _C._lib.pv_score_work_bytes(ctypes.byref(b)), (more + 15) // 16 * 16
+    t = torch.empty(more + need, dtype=torch.uint8, device=dev)
+    return t, t.data_ptr() + more, need
 
 
-def _scale(g):
-    """a loss's upstream gradient as a device float"""
-    return g if g.dtype == torch.float32 else g.float()
+def _with_grad(b, logits, g=None):
+    """b with a gradient of the logits to be written, a new one if none is given -> (b, gradient)"""
+    if g is None:
+        g = logits.new_empty(logits.shape)
+    b = _C.Scored.from_buffer_copy(b)
+    b.grad, (b.grad_n, b.grad_w, _) = g.data_ptr(), g.stride()
+    return b, g
 
 
-class _Saved:
-    """what a backward pass reads again: the batch's tensors go through autograd's saved tensors (which refuse one that
-    was changed in place meanwhile), the rest stays here"""
-
-    def __init__(self, ctx, logits, tokens, mask, shift, ignore):
-        ctx.save_for_backward(logits, tokens, mask)
-        self.shift, self.ignore = shift, ignore
-
-    def batch(self, ctx):
-        logits, tokens, mask = ctx.saved_tensors
-        return logits, _batch(logits, tokens, mask, self.shift, self.ignore)
+def _wants_grad(logits):
+    return isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()
 
 
 # ---------------------------------------------------------------------- log-probabilities
-def _logprobs(logits, tokens, mask, shift, ignore, window):
-    b = _batch(logits, tokens, mask, shift, ignore)
-    dev = logits.device
-    with torch.cuda.device(dev):
+def _logprobs(b, dev, window):
+    with _on(dev):
         out = torch.empty((b.n,) if window else (b.n, b.W), dtype=torch.float32, device=dev)
-        work, need = _work(b, dev) if window else (None, 0)
-        if _C._lib.pv_logprobs(ctypes.byref(b), None if window else out.data_ptr(), out.data_ptr() if window else None,
-                               work.data_ptr() if window else None, need, _stream(dev)):
+        kept, work, need = _work(b, dev) if window else (None, None, 0)
+        if _C._lib.pv_logprobs(ctypes.byref(b), None if window else out.data_ptr(), out.data_ptr() if window else None, work, need, _stream(dev)):
             raise _failed("log-probabilities")
     return out
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, mask, shift, ignore, window):
-        out = _logprobs(logits, tokens, mask, shift, ignore, window)
-        ctx.saved = _Saved(ctx, logits, tokens, mask, shift, ignore)
-        return out
+    def forward(ctx, logits, tokens, mask, b, window):
+        # autograd's saved tensors refuse one that is changed in place before the backward pass; b points into them
+        ctx.save_for_backward(logits, tokens, mask)
+        ctx.b = b
+        return _logprobs(b, logits.device, window)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        logits, b = ctx.saved.batch(ctx)
+        logits = ctx.saved_tensors[0]
         up_n, up_w = (up.stride(0), 0) if up.dim() == 1 else up.stride()
-        with torch.cuda.device(logits.device):
-            g = _grad_into(b, logits)
+        with _on(logits.device):
+            b, g = _with_grad(ctx.b, logits)
             if _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), up_n, up_w, None, 0, _stream(logits.device)):
                 raise _failed("log-probabilities' gradient")
-        return g, None, None, None, None, None
+        return g, None, None, None, None
 
 
 def window_logprobs(logits, tokens, mask=None, shift=1, ignore=None, reduce="token"):
@@ -160,47 +156,41 @@ def window_logprobs(logits, tokens, mask=None, shift=1, ignore=None, reduce="tok
     Differentiable by the logits."""
     if reduce not in ("token", "window"):
         raise ValueError('reduce: "token" or "window"')
-    f = _LogProbs.apply if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad else _logprobs
-    return f(logits, tokens, mask, shift, ignore, reduce == "window")
+    b = _batch(logits, tokens, mask, shift, ignore)
+    if _wants_grad(logits):
+        return _LogProbs.apply(logits, tokens, mask, b, reduce == "window")
+    return _logprobs(b, logits.device, reduce == "window")
 
 
 # ---------------------------------------------------------------------- preference
-def _preference(logits, tokens, mask, shift, ignore, ref, beta, smoothing):
-    """-> (loss, margins, each window's derivative)"""
-    b = _batch(logits, tokens, mask, shift, ignore)
-    dev = logits.device
-    if b.n % 2:
-        raise ValueError("logits: an even number of windows, the preferred ones first")
-    ref = _floats(ref, "ref_logp", ((b.n,),), dev)
-    with torch.cuda.device(dev):
+def _preference(b, dev, ref, beta, smoothing, margins):
+    """-> (loss, a buffer that starts with each window's derivative)"""
+    with _on(dev):
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        margins = torch.empty(b.n // 2, dtype=torch.float32, device=dev)
-        coef = torch.empty(b.n, dtype=torch.float32, device=dev)
-        work, need = _work(b, dev)
-        if _C._lib.pv_preference(ctypes.byref(b), ref.data_ptr(), ref.stride(0), beta, smoothing, loss.data_ptr(), margins.data_ptr(),
-                                 coef.data_ptr(), work.data_ptr(), need, _stream(dev)):
+        coef, work, need = _work(b, dev, 4 * b.n)
+        if _C._lib.pv_preference(ctypes.byref(b), ref.data_ptr(), ref.stride(0), beta, smoothing, loss.data_ptr(),
+                                 margins.data_ptr() if margins is not None else None, coef.data_ptr(), work, need, _stream(dev)):
             raise _failed("preference loss")
-    return loss, margins, coef
+    return loss, coef
 
 
 class _Preference(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, mask, shift, ignore, ref, beta, smoothing):
-        loss, margins, ctx.coef = _preference(logits, tokens, mask, shift, ignore, ref, beta, smoothing)
-        ctx.saved = _Saved(ctx, logits, tokens, mask, shift, ignore)
-        ctx.mark_non_differentiable(margins)
-        return loss, margins
+    def forward(ctx, logits, tokens, mask, b, ref, beta, smoothing, margins):
+        ctx.save_for_backward(logits, tokens, mask)
+        ctx.b = b
+        loss, ctx.coef = _preference(b, logits.device, ref, beta, smoothing, margins)
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, up, _):
-        logits, b = ctx.saved.batch(ctx)
-        with torch.cuda.device(logits.device):
-            up = _scale(up)
-            g = _grad_into(b, logits)
+    def backward(ctx, up):
+        logits = ctx.saved_tensors[0]
+        with _on(logits.device):
+            b, g = _with_grad(ctx.b, logits)
             if _C._lib.pv_logprobs_grad(ctypes.byref(b), ctx.coef.data_ptr(), 1, 0, up.data_ptr(), 0, _stream(logits.device)):
                 raise _failed("preference loss's gradient")
-        return (g,) + (None,) * 7
+        return g, None, None, None, None, None, None, None
 
 
 def preference_loss(logits, tokens, ref_logp, beta=0.1, label_smoothing=0.0, mask=None, shift=1, ignore=None, return_margins=False):
@@ -210,13 +200,21 @@ def preference_loss(logits, tokens, ref_logp, beta=0.1, label_smoothing=0.0, mas
     and its loss -(1 - label_smoothing) log sigmoid(beta margin) - label_smoothing log sigmoid(-beta margin); the mean over
     pairs (0 without any). return_margins: also the margins, float32 [n/2], which carry no gradient."""
     beta, smoothing = _number(beta, "beta", 0.0), _number(label_smoothing, "label_smoothing", 0.0, 1.0)
-    f = _Preference.apply if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad else _preference
-    r = f(logits, tokens, mask, shift, ignore, ref_logp, beta, smoothing)
-    return (r[0], r[1]) if return_margins else r[0]
+    b = _batch(logits, tokens, mask, shift, ignore)
+    dev = logits.device
+    if b.n % 2:
+        raise ValueError("logits: an even number of windows, the preferred ones first")
+    ref = _floats(ref_logp, "ref_logp", ((b.n,),), dev)
+    margins = torch.empty(b.n // 2, dtype=torch.float32, device=dev) if return_margins else None
+    if _wants_grad(logits):
+        loss = _Preference.apply(logits, tokens, mask, b, ref, beta, smoothing, margins)
+    else:
+        loss = _preference(b, dev, ref, beta, smoothing, margins)[0]
+    return (loss, margins) if return_margins else loss
 
 
 # ---------------------------------------------------------------------- policy
-def _policy_args(b, old, adv, ref, clip, kl, by_window, dev):
+def _policy_args(b, old, adv, ref, clip, kl, by_window, scale, dev):
     """-> (pv_policy_args, the tensors it points to)"""
     each = ((b.n, b.W),)
     old = _floats(old, "old_logp", each, dev)
@@ -225,61 +223,68 @@ def _policy_args(b, old, adv, ref, clip, kl, by_window, dev):
     av = adv.stride() if adv.dim() == 2 else (adv.stride(0), 0)
     rv = ref.stride() if ref is not None else (0, 0)
     return _C.PolicyArgs(old.data_ptr(), adv.data_ptr(), ref.data_ptr() if ref is not None else None, *old.stride(), *av, *rv, clip[0], clip[1], kl,
-                         by_window), (old, adv, ref)
+                         scale, by_window), (old, adv, ref)
 
 
-def _policy(logits, tokens, mask, shift, ignore, old, adv, ref, clip, kl, by_window):
-    """-> (loss, the arguments and weights that the gradient takes)"""
-    b = _batch(logits, tokens, mask, shift, ignore)
-    dev = logits.device
-    a, kept = _policy_args(b, old, adv, ref, clip, kl, by_window, dev)
-    with torch.cuda.device(dev):
+def _policy(b, dev, a):
+    """-> (loss, a buffer that starts with the windows' weights); b's gradient too, if it names one"""
+    with _on(dev):
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        weight = torch.empty(b.n, dtype=torch.float64, device=dev)
-        work, need = _work(b, dev)
-        if _C._lib.pv_policy(ctypes.byref(b), ctypes.byref(a), loss.data_ptr(), weight.data_ptr(), work.data_ptr(), need, _stream(dev)):
+        weight, work, need = _work(b, dev, 8 * b.n)
+        if _C._lib.pv_policy(ctypes.byref(b), ctypes.byref(a), loss.data_ptr(), weight.data_ptr(), work, need, _stream(dev)):
             raise _failed("policy loss")
-    return loss, (a, kept, weight)
+    return loss, weight
 
 
 class _Policy(torch.autograd.Function):
+    # A position's weight is known from the tokens alone, so the loss's pass over the logits forms their gradient too and
+    # the logits are read once: backward finds it made where its upstream gradient is 1, and forms it again where it is not
+    # (found out on the device, without a wait). Half-precision logits come with a loss scale that keeps their gradient in
+    # range, so theirs is left to backward.
     @staticmethod
-    def forward(ctx, logits, tokens, mask, shift, ignore, old, adv, ref, clip, kl, by_window):
-        loss, ctx.rest = _policy(logits, tokens, mask, shift, ignore, old, adv, ref, clip, kl, by_window)
-        ctx.saved = _Saved(ctx, logits, tokens, mask, shift, ignore)
+    def forward(ctx, logits, tokens, mask, b, a, kept):
+        ctx.save_for_backward(logits, tokens, mask, *kept)
+        ctx.b, ctx.a, ctx.grad = b, a, None
+        if logits.dtype != torch.float16:
+            b, ctx.grad = _with_grad(b, logits)
+        loss, ctx.weight = _policy(b, logits.device, a)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        logits, b = ctx.saved.batch(ctx)
-        a, _, weight = ctx.rest
-        with torch.cuda.device(logits.device):
-            up = _scale(up)
-            g = _grad_into(b, logits)
-            if _C._lib.pv_policy_grad(ctypes.byref(b), ctypes.byref(a), weight.data_ptr(), up.data_ptr(), 0, _stream(logits.device)):
+        logits = ctx.saved_tensors[0]
+        made, ctx.grad = ctx.grad, None
+        with _on(logits.device):
+            b, g = _with_grad(ctx.b, logits, made)
+            if _C._lib.pv_policy_grad(ctypes.byref(b), ctypes.byref(ctx.a), ctx.weight.data_ptr(), up.data_ptr(), made is not None,
+                                      _stream(logits.device)):
                 raise _failed("policy loss's gradient")
-        return (g,) + (None,) * 10
+        return g, None, None, None, None, None
 
 
-def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, kl=0.0, mask=None, shift=1, ignore=None, reduce="token"):
+def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, kl=0.0, mask=None, shift=1, ignore=None, reduce="token", scale=1.0):
     """The clipped policy loss with a KL term, a float32 scalar. With logp the log-probabilities of window_logprobs, and
     old_logp (of the policy that drew the tokens) and ref_logp (of the reference model) laid out the same, float32 [n, W]:
     r = exp(logp - old_logp), and per counted position
         -min(r A, clamp(r, 1 - clip, 1 + clip) A) + kl (exp(d) - d - 1),    d = ref_logp - logp.
     advantages A: float32 [n], or [n, W] at the logits' positions. clip: a number, or (below, above). kl > 0 needs ref_logp.
     reduce: "token", the mean over all counted positions; "window", the mean over the windows that have any of their own
-    means. 0 where nothing is counted."""
+    means. 0 where nothing is counted. The result is multiplied by `scale`: with 1 / (batches a step) there, and not on the
+    loss, the gradient is made in the loss's own pass over bf16 or fp32 logits (whose memory it takes from then on); an
+    upstream gradient other than 1 makes it once more."""
     if reduce not in ("token", "window"):
         raise ValueError('reduce: "token" or "window"')
     lo, hi = clip if isinstance(clip, (tuple, list)) else (clip, clip)
-    clip, kl = (_number(lo, "clip", 0.0), _number(hi, "clip", 0.0)), _number(kl, "kl", 0.0)
+    clip, kl, scale = (_number(lo, "clip", 0.0), _number(hi, "clip", 0.0)), _number(kl, "kl", 0.0), _number(scale, "scale", 0.0)
     if kl and ref_logp is None:
         raise ValueError("kl: a KL term needs ref_logp")
-    args = (logits, tokens, mask, shift, ignore, old_logp, advantages, ref_logp if kl else None, clip, kl, reduce == "window")
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
-        return _Policy.apply(*args)
-    return _policy(*args)[0]
+    b = _batch(logits, tokens, mask, shift, ignore)
+    dev = logits.device
+    a, kept = _policy_args(b, old_logp, advantages, ref_logp if kl else None, clip, kl, reduce == "window", scale, dev)
+    if _wants_grad(logits):
+        return _Policy.apply(logits, tokens, mask, b, a, kept)
+    return _policy(b, dev, a)[0]
 
 
 # ---------------------------------------------------------------------- gradients
@@ -296,40 +301,36 @@ def _dense(t):
 
 
 def _tensors(ts, name):
-    """-> (pv_tensors, what it points to, the tensors as a list)"""
-    if isinstance(ts, torch.Tensor):
-        ts = [ts]
-    ts = list(ts)
+    """-> (pv_tensors, the arrays it points to, the tensors as a list, their types, whether all are contiguous)"""
+    ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
     try:
-        types = bytes([_TYPES[t.dtype] for t in ts])
+        types = array("B", [_TYPES[t.dtype] for t in ts])
     except (KeyError, AttributeError):
         raise ValueError(f"{name}: bf16, fp16 or fp32 tensors") from None
-    dense = [t.is_contiguous() for t in ts]
-    if not all(dense) and not all(_dense(t) for t in ts):
+    plain = all([t.is_contiguous() for t in ts])
+    if not plain and not all(_dense(t) for t in ts):
         raise ValueError(f"{name}: tensors that are dense in memory (no gaps, no expanded dimensions)")
-    if len({t.device for t in ts}) > 1:
+    if len(set([t.get_device() for t in ts])) > 1:
         raise ValueError(f"{name}: on one device")
-    n = len(ts)
-    ptr, numel = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in ts]), (ctypes.c_int64 * n)(*[t.numel() for t in ts])
-    kept = (ptr, numel, ctypes.c_char_p(types))
-    return _C.Tensors(ctypes.cast(ptr, ctypes.c_void_p), ctypes.cast(numel, ctypes.c_void_p), ctypes.cast(kept[2], ctypes.c_void_p), n), kept, ts
+    if not ts:
+        raise ValueError(f"{name}: no tensors")
+    kept = array("Q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts]), types
+    return _C.Tensors(*(a.buffer_info()[0] for a in kept), len(ts)), kept, ts, types, plain
 
 
-def _norm_buffers(g, ts):
-    dev = _device(ts[0], "gradients")
+def _norm_buffers(g, dev):
     need = _C._lib.pv_grads_work_bytes(ctypes.byref(g))
-    return dev, torch.empty((), dtype=torch.float32, device=dev), torch.empty(need, dtype=torch.uint8, device=dev), need
+    return torch.empty((), dtype=torch.float32, device=dev), torch.empty(need, dtype=torch.uint8, device=dev), need
 
 
 def grad_norm(grads):
     """The 2-norm over all elements of all tensors (a tensor, or bf16 / fp16 / fp32 tensors of any shapes on one device,
     each dense in memory) -> float32 scalar on their device, summed in 64 bits. An empty list is refused: it has no
     device."""
-    g, kept, ts = _tensors(grads, "grads")
-    if not ts:
-        raise ValueError("grads: no tensors")
-    with torch.cuda.device(_device(ts[0], "gradients")):
-        dev, norm, work, need = _norm_buffers(g, ts)
+    g, kept, ts, _, _ = _tensors(grads, "grads")
+    dev = _device(ts[0], "gradients")
+    with _on(dev):
+        norm, work, need = _norm_buffers(g, dev)
         if _C._lib.pv_grad_norm(ctypes.byref(g), norm.data_ptr(), work.data_ptr(), need, _stream(dev)):
             raise _failed("gradient norm")
     return norm
@@ -343,23 +344,21 @@ def clip_grads(grads, max_norm, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm: 0 or more")
-    g, kept, ts = _tensors(grads, "grads")
-    if not ts:
-        raise ValueError("grads: no tensors")
-    o = okept = None
+    g, kept, ts, types, plain = _tensors(grads, "grads")
+    o, written = None, ts
     if out is not None:
-        o, okept, outs = _tensors(out, "out")
-        if len(outs) != len(ts) or any(a.shape != b.shape or a.stride() != b.stride() for a, b in zip(ts, outs)):
+        o, okept, written, otypes, oplain = _tensors(out, "out")
+        if [t.shape for t in ts] != [t.shape for t in written] or not (plain and oplain) and any(a.stride() != b.stride() for a, b in zip(ts, written)):
             raise ValueError("out: one tensor per gradient, of its shape and strides")
-        if any(b.dtype != a.dtype and b.dtype != torch.float32 for a, b in zip(ts, outs)):
+        if any([b != 2 and a != b for a, b in zip(types, otypes)]):
             raise ValueError("out: of the gradient's type, or float32")
-        if outs[0].device != ts[0].device:
+        if written[0].device != ts[0].device:
             raise ValueError("out: on the gradients' device")
-    written = ts if out is None else outs
-    if any(t.requires_grad and t.is_leaf and torch.is_grad_enabled() for t in written):
+    if True in [t.requires_grad for t in written] and any(t.requires_grad and t.is_leaf for t in written) and torch.is_grad_enabled():
         raise ValueError("clip_grads: pass the gradients (p.grad), not parameters")
-    with torch.cuda.device(_device(ts[0], "gradients")):
-        dev, norm, work, need = _norm_buffers(g, ts)
+    dev = _device(ts[0], "gradients")
+    with _on(dev):
+        norm, work, need = _norm_buffers(g, dev)
         code = _C._lib.pv_clip_grads(ctypes.byref(g), ctypes.byref(o) if o is not None else None, max_norm, norm.data_ptr(), work.data_ptr(), need,
                                      _stream(dev))
     if code == _C.PV_EARG:

@@ -341,6 +341,8 @@ def test_policy(P, cuda, n, W, V, shift, kind):
         close(d2, *grad_of(x, p, y, ok, -2.5 * g, 2.5 * g_err), "scaled")
         (again,) = torch.autograd.grad(got, x)
         assert torch.equal(again, d)
+        half = P.policy_loss(x, t, old, adv, ref, clip, kl, m, shift, reduce=reduce, scale=0.5)           # exact in every step
+        assert torch.equal(half, 0.5 * got) and (kind == "fp16" or torch.equal(torch.autograd.grad(half, x)[0], 0.5 * d))
         with torch.no_grad():
             assert torch.equal(P.policy_loss(x, t, old, adv, ref, clip, kl, m, shift, reduce=reduce), got)
 

@@ -50,6 +50,8 @@ def test_refusals_of_numbers_and_names():
             P.policy_loss(X, T, L, A, clip=bad)
         with pytest.raises(ValueError, match="clip"):
             P.policy_loss(X, T, L, A, clip=(0.2, bad))
+        with pytest.raises(ValueError, match="scale"):
+            P.policy_loss(X, T, L, A, scale=bad)
         with pytest.raises(ValueError, match="kl"):
             P.policy_loss(X, T, L, A, ref_logp=L, kl=bad)
     for bad in (-0.1, 1.1, float("nan")):
@@ -106,7 +108,7 @@ def _message():
                                 {"n": 1 << 40, "W": 1 << 30}])
 def test_entry_points_refuse_a_bad_batch(kw):
     lib, b = _C._lib, _scored(**kw)
-    a = _C.PolicyArgs(64, 64, None, 3, 1, 1, 0, 0, 0, 0.2, 0.2, 0.0, 0)
+    a = _C.PolicyArgs(64, 64, None, 3, 1, 1, 0, 0, 0, 0.2, 0.2, 0.0, 1.0, 0)
     assert lib.pv_score_work_bytes(b) == 0
     assert lib.pv_logprobs(b, 64, None, None, 0, None) == _C.PV_EARG and _message().startswith("batch")
     assert lib.pv_logprobs_grad(b, 64, 0, 0, None, 0, None) == _C.PV_EARG
@@ -117,14 +119,14 @@ def test_entry_points_refuse_a_bad_batch(kw):
 
 def test_entry_points_refuse_missing_arguments():
     lib, b = _C._lib, _scored()
-    good = dict(old=64, adv=64, ref=None, clip_low=0.2, clip_high=0.2, kl=0.0)
+    good = dict(old=64, adv=64, ref=None, clip_low=0.2, clip_high=0.2, kl=0.0, scale=1.0)
     assert lib.pv_logprobs(b, None, 64, None, 0, None) == _C.PV_EARG and "scratch" in _message()
     assert lib.pv_logprobs(b, None, 64, 72, 1 << 30, None) == _C.PV_EARG and "scratch" in _message()      # not 16-byte aligned
     assert lib.pv_logprobs_grad(b, 64, 0, 0, None, 0, None) == _C.PV_EARG                                  # no gradient to write
     assert lib.pv_preference(_scored(n=3), 64, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 30, None) == _C.PV_EARG and "odd" in _message()
     assert lib.pv_preference(b, None, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 30, None) == _C.PV_EARG
     assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, 64, 1, None) == _C.PV_EARG and "scratch" in _message()
-    for kw in ({"old": None}, {"adv": None}, {"clip_low": -1.0}, {"clip_high": float("nan")}, {"kl": 0.1}):
+    for kw in ({"old": None}, {"adv": None}, {"clip_low": -1.0}, {"clip_high": float("nan")}, {"kl": 0.1}, {"scale": -1.0}):
         assert lib.pv_policy(b, ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, 64, 64, 1 << 30, None) == _C.PV_EARG
         assert lib.pv_policy_grad(_scored(grad=64), ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, None, 0, None) == _C.PV_EARG
     assert lib.pv_policy(b, None, 64, 64, 64, 1 << 30, None) == _C.PV_EARG
