@@ -62,15 +62,16 @@ struct Rows {
     const float* scale; int32_t skip_one;
 };
 
-// the target of row (i, t), or -1
+// the target of row (i, t), or -1 (token and mask are loaded side by side)
 __device__ __forceinline__ int target(const pv_scored& b, int64_t i, int64_t t) {
     const int64_t at = t + b.shift;
     if (at >= b.W) return -1;
-    if (b.mask_bytes == 1 && ((const uint8_t*)b.mask)[i * b.mask_n + at * b.mask_w] == 0) return -1;
-    if (b.mask_bytes == 4 && ((const float*)b.mask)[i * b.mask_n + at * b.mask_w] == 0.f) return -1;
     const int64_t y = b.token_bytes == 1 ? ((const uint8_t*)b.tokens)[i * b.tokens_n + at * b.tokens_w]
                                          : ((const int64_t*)b.tokens)[i * b.tokens_n + at * b.tokens_w];
-    return y < 0 || y >= b.V || y == b.ignore ? -1 : (int)y;
+    bool on = true;
+    if (b.mask_bytes == 1) on = ((const uint8_t*)b.mask)[i * b.mask_n + at * b.mask_w] != 0;
+    else if (b.mask_bytes == 4) on = ((const float*)b.mask)[i * b.mask_n + at * b.mask_w] != 0.f;
+    return !on || y < 0 || y >= b.V || y == b.ignore ? -1 : (int)y;
 }
 
 // a row's (or a thread's part of a row's) reference
@@ -86,13 +87,14 @@ __device__ __forceinline__ uint64_t pair(float a, float b) {
     return r;
 }
 __device__ __forceinline__ void halves(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-// x becomes its numerators, two to an FMA
+// x becomes its numerators, two to an FMA (where the maximum is far, x less the maximum comes in and c is 0)
 template <int K>
-__device__ __forceinline__ void numerators(float (&x)[K], float m, float c) {
-    if (far(m)) {
+__device__ __forceinline__ void less(float (&x)[K], float m) {
 #pragma unroll
-        for (int q = 0; q < K; q++) x[q] -= m;
-    }
+    for (int q = 0; q < K; q++) x[q] -= m;
+}
+template <int K>
+__device__ __forceinline__ void numerators(float (&x)[K], float c) {
     const uint64_t l = pair(LOG2E, LOG2E), nc = pair(-c, -c);
 #pragma unroll
     for (int q = 0; q < K; q += 2) {
@@ -274,9 +276,11 @@ __device__ __forceinline__ bool alike(const T* x, const T* d) { return (((uintpt
 // a time; each lane loads one row's target and arguments for the whole tile first.
 constexpr int TILE = 32;
 
-template <typename T, int G, int NV, int MODE>
-__global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
+// A: rows of whole pieces, logits' and gradient's alike. Then the next rows' loads are under way while these are worked on.
+template <typename T, int G, int NV, int MODE, bool A>
+__global__ void __launch_bounds__(256, NV <= 4 && MODE != POLICY ? 3 : 2) rows_group_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G;
+    constexpr bool AHEAD = A && NV <= 4;
     const int lane = threadIdx.x & 31, sub = lane % G, grp = lane / G, V = (int)k.b.V;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
@@ -291,23 +295,32 @@ __global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
         const T* const x0 = (const T*)k.b.logits + i * k.b.logits_n + t0 * k.b.logits_w;
         T* const d0 = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t0 * k.b.grad_w : nullptr;
         double sum = 0;
-        for (int s0 = 0; s0 < rows; s0 += RP) {
+        // rows s0 ... + RP; a group without a counted row loads nothing
+        const auto load = [&](int s0, uint4 (&raw)[NV], float& xt) {
             const int row = s0 + grp, y = __shfl_sync(~0u, y_l, row);
             const T* x = x0 + row * k.b.logits_w;
-            const int off = row_off(x);
-            uint4 raw[NV];
-            float xt = 0.f;
+            const int off = A ? 0 : row_off(x);
 #pragma unroll
-            for (int j = 0; j < NV; j++) raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
-            if (y >= 0) {
-#pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    const int e0 = (sub + j * G) * K - off;
-                    if (whole<T>(e0, V)) raw[j] = *(const uint4*)(x + e0);
-                    else if (e0 < V) raw[j] = edge_piece(x, e0, V);
+            for (int j = 0; j < NV; j++) {
+                raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+                const int e0 = (sub + j * G) * K - off;
+                if (y >= 0 && e0 < V) {
+                    if (A || whole<T>(e0, V)) raw[j] = *(const uint4*)(x + e0);
+                    else raw[j] = edge_piece(x, e0, V);
                 }
-                xt = f32(x[y]);
             }
+            xt = y >= 0 ? f32(x[y]) : 0.f;
+        };
+        uint4 raw[NV], next[AHEAD ? NV : 1];
+        float xt, xt_next = 0.f;
+        if (AHEAD) load(0, raw, xt);
+        for (int s0 = 0; s0 < rows; s0 += RP) {
+            if constexpr (AHEAD) {
+                if (s0 + RP < rows) load(s0 + RP, next, xt_next);
+            } else {
+                load(s0, raw, xt);
+            }
+            const int row = s0 + grp, y = __shfl_sync(~0u, y_l, row);
             float m = piece_max<T>(raw[0]);
 #pragma unroll
             for (int j = 1; j < NV; j++) m = fmaxf(m, piece_max<T>(raw[j]));
@@ -316,14 +329,20 @@ __global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
             const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
             float e[NV][K], o = 0.f;
 #pragma unroll
+            for (int j = 0; j < NV; j++) unpack<T>(raw[j], e[j]);
+            if (far(m)) {
+#pragma unroll
+                for (int j = 0; j < NV; j++) less(e[j], m);
+            }
+#pragma unroll
             for (int j = 0; j < NV; j++) {
-                unpack<T>(raw[j], e[j]);
-                numerators(e[j], m, c);
+                numerators(e[j], c);
                 o += sum_of(e[j]);
             }
 #pragma unroll
             for (int s = G / 2; s; s >>= 1) o += __shfl_xor_sync(~0u, o, s);
             o -= et;
+            const int off = A ? 0 : row_off(x0 + row * k.b.logits_w);
             // where the target outweighs the others that difference has lost their digits: they are summed by themselves
             if (__any_sync(~0u, y >= 0 && !(et < o))) {
                 float p = 0.f;
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
                 if (k.logp && sub == 0 && row < rows) k.logp[i * k.b.W + t0 + row] = lp;
             } else if (d0 && row < rows) {
                 T* d = d0 + row * k.b.grad_w;
-                const bool same = alike(x, d);
+                const bool same = A || alike(x0 + row * k.b.logits_w, d);
                 const float inv = 1.f / (o + et), f = y < 0 ? 0.f : -g * inv;
 #pragma unroll
                 for (int j = 0; j < NV; j++) {
@@ -359,9 +378,17 @@ __global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
                         for (int q = 0; q < K; q++) e[j][q] = 0.f;
                     }
                     times(e[j], f);
-                    if (e0 < V) store_piece(d, e0, V, same, e[j]);
-                    if (y >= e0 && y < e0 + K && y >= 0) d[y] = from32<T>(g * (o * inv));
+                    if (e0 < V) {
+                        if (A) *(uint4*)(d + e0) = pack<T>(e[j]);
+                        else store_piece(d, e0, V, same, e[j]);
+                    }
+                    if (y >= 0 && y >= e0 && y < e0 + K) d[y] = from32<T>(g * (o * inv));
                 }
+            }
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int j = 0; j < NV; j++) raw[j] = next[j];
+                xt = xt_next;
             }
         }
         if (k.part) {
@@ -374,38 +401,75 @@ __global__ void __launch_bounds__(256) rows_group_kernel(Rows k) {
 // ---------------------------------------------------------------- longer rows: a block a row
 // the running maximum and sum of a thread
 struct Run { float m = -INFINITY, c = 0.f, o = 0.f; };
+__device__ __forceinline__ void raise(Run& r, float m) {                            // from nothing: 0 times 0
+    if (m > r.m) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }
+}
+// adds a piece; at: the target's place in it, if any, whose logit goes to *xt
 template <typename T>
-__device__ __forceinline__ void take(Run& r, const uint4& raw, int at) {          // at: the target's place in the piece, if any
+__device__ __forceinline__ void add(Run& r, const uint4& raw, int at, float* xt) {
     constexpr int K = K_OF<T>;
-    const float m = piece_max<T>(raw);
-    if (m > r.m) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }            // from nothing: 0 times 0
     float x[K];
     unpack<T>(raw, x);
-    numerators(x, r.m == -INFINITY ? 0.f : r.m, r.c);                             // nothing but -inf so far: numerators of 0
+    float own = 0.f;
+    if (at >= 0 && at < K) {
+#pragma unroll
+        for (int q = 0; q < K; q++) own = q == at ? x[q] : own;
+        *xt = own;
+    }
+    if (far(r.m) && r.m != -INFINITY) less(x, r.m);                                 // nothing but -inf so far: numerators of 0
+    numerators(x, r.c);
     if (at >= 0 && at < K) {
 #pragma unroll
         for (int q = 0; q < K; q++) x[q] = q == at ? 0.f : x[q];
     }
     r.o += sum_of(x);
 }
+template <typename T>
+__device__ __forceinline__ void take(Run& r, const uint4& raw, int at, float* xt) {
+    raise(r, piece_max<T>(raw));
+    add<T>(r, raw, at, xt);
+}
 __device__ __forceinline__ void warp_join(Run& r) {
     const float m = warp_max(r.m);
     r.o = warp_sum(r.m == m ? r.o : r.o * rescale(r.m, m));
     r.m = m;
 }
-// The block's: one barrier a row, two buffers in turn (a buffer is written again only after the next row's barrier, which
-// every thread reaches after its reads here).
+// What the warps leave for warp 0 at a row's end, and it for them: two of each in turn, so that a row's is written again
+// only behind the barrier of the row between, which warp 0 reaches after reading it.
 template <int THREADS>
-__device__ __forceinline__ void block_join(Run& r, float2 (&red)[2][THREADS / 32], int turn) {
+struct Meeting {
+    float2 run[2][THREADS / 32];
+    float xt[2];
+    float4 grad[2];          // the maximum, the reference, the factor of a numerator and the target's derivative
+};
+// Ends a counted row: the threads' sums join, warp 0 takes them to the row's log-probability, term and derivative.
+template <int MODE, int THREADS>
+__device__ __forceinline__ float4 block_end(const Rows& k, Meeting<THREADS>& at, int turn, Run& run, const End& end, double w, float scale, int64_t r,
+                                            bool grad) {
     constexpr int NW = THREADS / 32;
-    warp_join(r);
-    if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = make_float2(r.m, r.o);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    warp_join(run);
+    if (lane == 0) at.run[turn][warp] = make_float2(run.m, run.o);
     __syncthreads();
-    const int lane = threadIdx.x & 31;
-    r = Run();
-    if (lane < NW) { const float2 v = red[turn][lane]; r.m = v.x; r.o = v.y; }
-    warp_join(r);
-    r.c = ref_of(r.m);
+    if (warp == 0) {
+        Run all;
+        if (lane < NW) { const float2 v = at.run[turn][lane]; all.m = v.x; all.o = v.y; }
+        warp_join(all);
+        const float c = ref_of(all.m), t = exponent(at.xt[turn], all.m, c), e = ex2(t);
+        float term;
+        const float lp = MODE == GRAD ? 0.f : row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
+        if (lane == 0) {
+            if (MODE == LOGP && k.logp) k.logp[r] = lp;
+            if (k.part) k.part[r] = (double)term * w;
+            if (grad) {
+                const float inv = 1.f / (all.o + e);
+                at.grad[turn] = make_float4(all.m, c, -g * inv, g * (all.o * inv));
+            }
+        }
+    }
+    if (!grad) return make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+    return at.grad[turn];
 }
 
 template <typename T>
@@ -419,54 +483,82 @@ __device__ __forceinline__ void zero_row(T* d, int V, int threads) {
 }
 
 template <typename T>
-__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, int y, const Run& r, float f, float ft) {
+__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, int y, const float4& g) {
     constexpr int K = K_OF<T>;
     float x[K];
     unpack<T>(raw, x);
-    numerators(x, r.m, r.c);
-    times(x, f);
+    if (far(g.x)) less(x, g.x);
+    numerators(x, g.y);
+    times(x, g.z);
     store_piece(d, e0, V, same, x);
-    if (y >= e0 && y < e0 + K) d[y] = from32<T>(ft);
+    if (y >= e0 && y < e0 + K) d[y] = from32<T>(g.w);
 }
 
-// Rows that fit a ring of S pieces a thread in shared memory. Every thread copies its own pieces in asynchronously and
-// reads only those, so the copies need no barrier: the ring runs ahead into the next rows while this row is reduced, and
-// a piece leaves it when the row's gradient has been formed from it. One copy group is committed for every step of either
-// pass (an empty one where nothing is copied), so at least S - 1 groups lie behind the one that a step needs.
+// rows r, r + stride, ... of a batch, with their windows and positions
+struct Pos {
+    int64_t r, i, t;
+    __device__ __forceinline__ Pos(int64_t r, int64_t W) : r(r), i(r / W), t(r % W) {}
+    __device__ __forceinline__ void next(int64_t stride, int64_t si, int64_t st, int64_t W) {
+        r += stride; i += si; t += st;
+        if (t >= W) { t -= W; i++; }
+    }
+};
+
+// Rows that fit a ring of S steps in shared memory, U pieces a thread each. Every thread copies its own pieces in
+// asynchronously and reads only those, so the copies need no barrier: the ring runs ahead into the next rows while this row
+// is reduced, and a step's pieces leave it when the row's gradient has been formed from them. One copy group is committed
+// for every step of either pass (an empty one where nothing is copied), so at least S - 1 groups lie behind the one that a
+// step needs: between a step's copy and its use lie the S - 1 steps that were copied after it, or a whole pass more.
 __device__ __forceinline__ void copy16(void* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int THREADS, int S, int MODE>
-__global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
-    constexpr int K = K_OF<T>;
-    extern __shared__ uint4 ring[];                          // [S][THREADS]
-    __shared__ float2 red[2][THREADS / 32];
+template <typename T, int THREADS, int U, int S, int MODE>
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) rows_ring_kernel(Rows k, int steps) {
+    constexpr int K = K_OF<T>, SPAN = THREADS * K;           // elements from a thread's piece to its next
+    extern __shared__ uint4 ring[];                          // [S][U][THREADS]
+    __shared__ Meeting<THREADS> meet;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     const int tid = threadIdx.x, V = (int)k.b.V;
-    const int64_t rows = k.b.n * k.b.W, stride = gridDim.x;
-    const auto target_of = [&](int64_t r) { return r < rows ? target(k.b, r / k.b.W, r % k.b.W) : -1; };
-    const auto row_at = [&](int64_t r) { return (const T*)k.b.logits + (r / k.b.W) * k.b.logits_n + (r % k.b.W) * k.b.logits_w; };
+    const int64_t W = k.b.W, rows = k.b.n * W, stride = gridDim.x, si = stride / W, st = stride - si * W;
+    const auto target_of = [&](const Pos& p) { return p.r < rows ? target(k.b, p.i, p.t) : -1; };
+    // all U pieces from e0 on lie inside the row
+    const auto inside = [&](int e0) { return e0 >= 0 && e0 + (U - 1) * SPAN + K <= V; };
 
-    // what is copied next: piece in_j of row in_row (a counted one), into slot in_slot
-    int64_t in_row = blockIdx.x;
-    int in_j = 0, in_slot = 0;
-    while (in_row < rows && target_of(in_row) < 0) in_row += stride;
-    const T* in_x = in_row < rows ? row_at(in_row) : nullptr;
+    // what is copied next: step in_j of row `in` (a counted one), into slot in_slot; the row after it is looked up ahead
+    Pos in(blockIdx.x, W), ahead = in;
+    ahead.next(stride, si, st, W);
+    int in_y = target_of(in), ahead_y = target_of(ahead), in_j = 0, in_slot = 0, in_off = 0;
+    const T* in_x = nullptr;
+    const auto find = [&]() {                                // from `in` on to a counted row
+        while (in.r < rows && in_y < 0) {
+            in = ahead;
+            in_y = ahead_y;
+            ahead.next(stride, si, st, W);
+            ahead_y = target_of(ahead);
+        }
+        if (in.r < rows) { in_x = (const T*)k.b.logits + in.i * k.b.logits_n + in.t * k.b.logits_w; in_off = row_off(in_x); }
+    };
+    find();
     const auto copy_next = [&]() {
-        if (in_row < rows) {
-            const int e0 = (tid + in_j * THREADS) * K - row_off(in_x);
-            uint4* to = &ring[in_slot * THREADS + tid];
-            if (whole<T>(e0, V)) copy16(to, in_x + e0);
-            else if (e0 < V) *to = edge_piece(in_x, e0, V);
-            if (++in_j == steps) {
-                in_j = 0;
-                do in_row += stride; while (in_row < rows && target_of(in_row) < 0);
-                if (in_row < rows) in_x = row_at(in_row);
+        if (in.r < rows) {
+            const int e0 = (tid + in_j * U * THREADS) * K - in_off;
+            uint4* to = &ring[in_slot * U * THREADS + tid];
+            if (inside(e0)) {
+#pragma unroll
+                for (int u = 0; u < U; u++) copy16(to + u * THREADS, in_x + e0 + u * SPAN);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < U; u++) {
+                    const int e = e0 + u * SPAN;
+                    if (whole<T>(e, V)) copy16(to + u * THREADS, in_x + e);
+                    else if (e < V) to[u * THREADS] = edge_piece(in_x, e, V);
+                }
             }
+            if (++in_j == steps) { in_j = 0; in_y = -1; find(); }
         }
         if (++in_slot == S) in_slot = 0;
         copies_commit();
@@ -474,11 +566,14 @@ __global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
 #pragma unroll 1
     for (int s = 0; s < S; s++) copy_next();
 
-    int slot = 0, turn = 0, y = target_of(blockIdx.x);
-    for (int64_t r = blockIdx.x; r < rows; r += stride) {
-        const int64_t i = r / k.b.W, t = r - i * k.b.W;
+    int slot = 0, turn = 0;
+    Pos p(blockIdx.x, W);
+    int y = target_of(p);
+    while (p.r < rows) {
+        const int64_t r = p.r, i = p.i, t = p.t;
+        p.next(stride, si, st, W);
+        const int y_next = target_of(p);
         T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
-        const int y_next = target_of(r + stride);
         if (y < 0) {
             if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
             if (MODE != LOGP && d) zero_row(d, V, THREADS);
@@ -486,38 +581,58 @@ __global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
             y = y_next;
             continue;
         }
-        const T* x = row_at(r);
+        const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
         const int off = row_off(x);
-        const End end = end_args<MODE>(k, i, t);
-        const double w = weight_of<MODE>(k, i);
-        const float xt = f32(x[y]);
+        const bool grad = MODE != LOGP && d;
+        End end = {0.f, 0.f, 0.f};
+        double w = 1.0;
+        if (tid < 32) { end = end_args<MODE>(k, i, t); w = weight_of<MODE>(k, i); }
         Run run;
         int at = slot;
         for (int j = 0; j < steps; j++) {
-            const int e0 = (tid + j * THREADS) * K - off;
+            const int e0 = (tid + j * U * THREADS) * K - off;
+            const uint4* from = &ring[at * U * THREADS + tid];
             copies_wait<S - 1>();
-            if (e0 < V) {
-                take<T>(run, ring[at * THREADS + tid], y - e0);
+            if (inside(e0)) {
+                uint4 raw[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
+                float m = piece_max<T>(raw[0]);
+#pragma unroll
+                for (int u = 1; u < U; u++) m = fmaxf(m, piece_max<T>(raw[u]));
+                raise(run, m);
+#pragma unroll
+                for (int u = 0; u < U; u++) add<T>(run, raw[u], y - e0 - u * SPAN, &meet.xt[turn]);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < U && e0 + u * SPAN < V; u++) take<T>(run, from[u * THREADS], y - e0 - u * SPAN, &meet.xt[turn]);
             }
             if (++at == S) at = 0;
-            if (MODE == LOGP || !d) copy_next(); else copies_commit();
+            if (grad) copies_commit(); else copy_next();
         }
-        block_join<THREADS>(run, red, turn);
+        const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
         turn ^= 1;
-        const float ex = exponent(xt, run.m, run.c), e = ex2(ex), lp = row_logp(run.m, run.o, ex, e);
-        float term;
-        const float g = row_end<MODE>(k, end, lp, (float)w, scale, term);
-        if (tid == 0) {
-            if (MODE == LOGP && k.logp) k.logp[r] = lp;
-            if (k.part) k.part[r] = (double)term * w;
-        }
-        if (MODE != LOGP && d) {
+        if (grad) {
             const bool same = alike(x, d);
-            const float inv = 1.f / (run.o + e), f = -g * inv, ft = g * (run.o * inv);
             at = slot;
             for (int j = 0; j < steps; j++) {
-                const int e0 = (tid + j * THREADS) * K - off;
-                if (e0 < V) grad_piece(ring[at * THREADS + tid], d, e0, V, same, y, run, f, ft);
+                const int e0 = (tid + j * U * THREADS) * K - off;
+                const uint4* from = &ring[at * U * THREADS + tid];
+                if (same && inside(e0)) {
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        float v[K];
+                        unpack<T>(from[u * THREADS], v);
+                        if (far(g.x)) less(v, g.x);
+                        numerators(v, g.y);
+                        times(v, g.z);
+                        *(uint4*)(d + e0 + u * SPAN) = pack<T>(v);
+                    }
+                    if (((y + off) / K) % THREADS == tid && y >= e0 && y < e0 + (U - 1) * SPAN + K) d[y] = from32<T>(g.w);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) grad_piece(from[u * THREADS], d, e0 + u * SPAN, V, same, y, g);
+                }
                 if (++at == S) at = 0;
                 copy_next();
             }
@@ -532,7 +647,7 @@ __global__ void __launch_bounds__(THREADS) rows_ring_kernel(Rows k, int steps) {
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
     constexpr int K = K_OF<T>, THREADS = 512, U = 4;
-    __shared__ float2 red[2][THREADS / 32];
+    __shared__ Meeting<THREADS> meet;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     const int tid = threadIdx.x, V = (int)k.b.V;
@@ -550,9 +665,9 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
         }
         const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
         const int off = row_off(x);
-        const End end = end_args<MODE>(k, i, t);
-        const double w = weight_of<MODE>(k, i);
-        const float xt = f32(x[y]);
+        End end = {0.f, 0.f, 0.f};
+        double w = 1.0;
+        if (tid < 32) { end = end_args<MODE>(k, i, t); w = weight_of<MODE>(k, i); }
         // pieces of the row, U at a time in flight; 64-bit places, as the last step may pass 2^31
         const auto pieces = [&](auto&& f) {
             for (int64_t p0 = tid; p0 * K - off < V; p0 += THREADS * U) {
@@ -571,22 +686,13 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
             }
         };
         Run run;
-        pieces([&](const uint4& raw, int e0) {
-            take<T>(run, raw, y - e0);
-        });
-        block_join<THREADS>(run, red, turn);
+        pieces([&](const uint4& raw, int e0) { take<T>(run, raw, y - e0, &meet.xt[turn]); });
+        const bool grad = MODE != LOGP && d;
+        const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
         turn ^= 1;
-        const float ex = exponent(xt, run.m, run.c), e = ex2(ex), lp = row_logp(run.m, run.o, ex, e);
-        float term;
-        const float g = row_end<MODE>(k, end, lp, (float)w, scale, term);
-        if (tid == 0) {
-            if (MODE == LOGP && k.logp) k.logp[r] = lp;
-            if (k.part) k.part[r] = (double)term * w;
-        }
-        if (MODE != LOGP && d) {
+        if (grad) {
             const bool same = alike(x, d);
-            const float inv = 1.f / (run.o + e), f = -g * inv, ft = g * (run.o * inv);
-            pieces([&](const uint4& raw, int e0) { grad_piece(raw, d, e0, V, same, y, run, f, ft); });
+            pieces([&](const uint4& raw, int e0) { grad_piece(raw, d, e0, V, same, y, g); });
         }
     }
 }
@@ -623,18 +729,31 @@ __global__ void __launch_bounds__(256) window_sums_kernel(const double* part, in
 // one block: the sum of `count` partial sums
 __global__ void __launch_bounds__(1024) total_kernel(const double* part, int64_t count, float* out) {
     double v = 0;
-    for (int64_t j = threadIdx.x; j < count; j += blockDim.x) v += part[j];
+#pragma unroll 8
+    for (int64_t j = threadIdx.x; j < count; j += 1024) v += part[j];
     v = block_sum(v);
     if (threadIdx.x == 0) *out = (float)v;
 }
 
-// one block: the pairs' margins, loss and derivatives from the windows' sums
-__global__ void __launch_bounds__(1024) pairs_kernel(const double* sums, int64_t n, const float* ref, int64_t ref_n, float beta, float eps,
-                                                     float* loss, float* margins, float* coef) {
+// one block: the pairs' margins, loss and derivatives from the windows' sums, which lie in `tpw` parts each (summed into
+// `sums` first, a warp a window, where tpw is not 1)
+__global__ void __launch_bounds__(1024) pairs_kernel(const double* part, int64_t tpw, double* sums, int64_t n, const float* ref, int64_t ref_n,
+                                                     float beta, float eps, float* loss, float* margins, float* coef) {
     const int64_t m = n / 2;
+    if (tpw != 1) {
+        for (int64_t i = threadIdx.x >> 5; i < n; i += 32) {
+            double v = 0;
+#pragma unroll 8
+            for (int64_t j = threadIdx.x & 31; j < tpw; j += 32) v += part[i * tpw + j];
+            v = warp_sum(v);
+            if ((threadIdx.x & 31) == 0) sums[i] = v;
+        }
+        __syncthreads();
+        part = sums;
+    }
     double all = 0;
     for (int64_t j = threadIdx.x; j < m; j += blockDim.x) {
-        const double gap = (sums[j] - (double)ref[j * ref_n]) - (sums[j + m] - (double)ref[(j + m) * ref_n]);
+        const double gap = (part[j] - (double)ref[j * ref_n]) - (part[j + m] - (double)ref[(j + m) * ref_n]);
         const double h = (double)beta * gap;
         // log sigmoid(h) = min(h, 0) - log1p(exp(-|h|))
         const double l = log1p(exp(-fabs(h))), up = fmin(h, 0.0) - l, down = fmin(-h, 0.0) - l;
@@ -648,25 +767,37 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const double* sums, int64_t
     if (threadIdx.x == 0) *loss = m ? (float)(all / (double)m) : 0.f;
 }
 
-// counted positions of each window: a block per (window, part of it), then one block turns them into weights
-constexpr int COUNT_SPAN = 2048;
+// Counted positions of each window, turned into weights: up to COUNT_ONE positions by one block, a warp a window; more by a
+// block per (window, span of it) first.
+constexpr int COUNT_SPAN = 2048, COUNT_ONE = 32768;
 __global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, int32_t* counts) {
     for (int64_t q = blockIdx.x; q < b.n * spans; q += gridDim.x) {
-        const int64_t i = q / spans, t0 = (q - i * spans) * COUNT_SPAN, t1 = min(t0 + (int64_t)COUNT_SPAN, b.W);
+        const int64_t i = q / spans, t0 = (q - i * spans) * COUNT_SPAN;
         int v = 0;
-        for (int64_t t = t0 + threadIdx.x; t < t1; t += blockDim.x) v += target(b, i, t) >= 0;
+#pragma unroll
+        for (int u = 0; u < COUNT_SPAN / 256; u++) {
+            const int64_t t = t0 + threadIdx.x + u * 256;
+            v += t < b.W && target(b, i, t) >= 0;
+        }
         v = (int)block_sum((double)v);
         if (threadIdx.x == 0) counts[q] = v;
     }
 }
-__global__ void __launch_bounds__(1024) weights_kernel(const int32_t* counts, int64_t n, int64_t spans, int by_window, double scale, double* weight) {
+__global__ void __launch_bounds__(1024) weights_kernel(pv_scored b, const int32_t* counts, int64_t spans, int by_window, double scale,
+                                                       double* weight) {
     double all = 0, some = 0;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        int64_t c = 0;
-        for (int64_t j = 0; j < spans; j++) c += counts[i * spans + j];
-        all += (double)c;
-        some += c > 0;
-        weight[i] = (double)c;
+    const int64_t n = b.n;
+    const int lane = threadIdx.x & 31;
+    for (int64_t i = threadIdx.x >> 5; i < n; i += 32) {
+        int c = 0;
+        if (counts) {
+            for (int64_t j = lane; j < spans; j += 32) c += counts[i * spans + j];
+        } else {
+#pragma unroll 4
+            for (int64_t t = lane; t < b.W; t += 32) c += target(b, i, t) >= 0;
+        }
+        c = (int)__reduce_add_sync(~0u, (unsigned)c);
+        if (lane == 0) { weight[i] = (double)c; all += (double)c; some += c > 0; }
     }
     all = block_sum(all);
     some = block_sum(some);
@@ -701,14 +832,18 @@ const char* bad_batch(const pv_scored* b) {
 // How a batch is run, by its rows' 16-byte pieces (one more than their bytes say where a row may start inside one):
 // up to 256 in registers, G lanes a row; up to RING_MOST in a ring in shared memory, a block a row; else read twice.
 enum { GROUP, RING, LONG };
-struct Plan { int form, pieces; int64_t tpw, tiles, spans; };
-constexpr int RING_MOST = 26 * 512;
+struct Plan { int form, pieces; bool aligned; int64_t tpw, tiles, spans; };
+constexpr int RING_MOST = 14 * 2 * 512;
 int size_of(int type) { return type == PV_T_FP32 ? 4 : 2; }
+// every row starts at a 16-byte boundary
+bool whole_pieces(const void* p, int64_t n, int64_t w, int64_t size) {
+    return (((uintptr_t)p | (uint64_t)(n * size) | (uint64_t)(w * size)) & 15) == 0;
+}
 Plan plan_of(const pv_scored& b) {
     Plan p;
     const int64_t size = size_of(b.type), k = 16 / size;
-    const bool aligned = (((uintptr_t)b.logits | (uint64_t)(b.logits_n * size) | (uint64_t)(b.logits_w * size)) & 15) == 0;
-    const int64_t pieces = (b.V + k - 1 + (aligned ? 0 : k - 1)) / k;
+    p.aligned = whole_pieces(b.logits, b.logits_n, b.logits_w, size);
+    const int64_t pieces = (b.V + k - 1 + (p.aligned ? 0 : k - 1)) / k;
     p.pieces = (int)std::min<int64_t>(pieces, 1 << 30);
     p.form = pieces <= 256 ? GROUP : pieces <= RING_MOST ? RING : LONG;
     p.tpw = p.form == GROUP ? (b.W + TILE - 1) / TILE : b.W;
@@ -736,18 +871,18 @@ unsigned grid_of(F* f, int threads, size_t smem, int64_t blocks) {
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)SMS * per_sm));
 }
 
-template <typename T, int G, int NV, int MODE>
+template <typename T, int G, int NV, int MODE, bool A>
 void group_rows(const Rows& k, cudaStream_t st) {
-    const auto f = rows_group_kernel<T, G, NV, MODE>;
+    const auto f = rows_group_kernel<T, G, NV, MODE, A>;
     const int64_t tiles = k.b.n * k.tpw;
     static const unsigned most = grid_of(f, 256, 0, 1 << 20);
     f<<<(unsigned)std::min<int64_t>((tiles + 7) / 8, most), 256, 0, st>>>(k);
 }
 
-template <typename T, int THREADS, int S, int MODE>
+template <typename T, int THREADS, int U, int S, int MODE>
 void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
-    constexpr int SMEM = S * THREADS * 16;
-    const auto f = rows_ring_kernel<T, THREADS, S, MODE>;
+    constexpr int SMEM = S * U * THREADS * 16;
+    const auto f = rows_ring_kernel<T, THREADS, U, S, MODE>;
     static thread_local uint64_t set = 0;                    // devices whose attribute is set
     int dev = 0;
     cudaGetDevice(&dev);
@@ -756,7 +891,19 @@ void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
         if (dev < 64) set |= 1ull << dev;
     }
     static const unsigned most = grid_of(f, THREADS, SMEM, 1 << 20);
-    f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), THREADS, SMEM, st>>>(k, (pieces + THREADS - 1) / THREADS);
+    f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), THREADS, SMEM, st>>>(k, (pieces + U * THREADS - 1) / (U * THREADS));
+}
+
+template <typename T, int MODE, bool A>
+void group_rows_of(const Rows& k, const Plan& p, cudaStream_t st) {
+    if (p.pieces <= 1) group_rows<T, 1, 1, MODE, A>(k, st);
+    else if (p.pieces <= 2) group_rows<T, 1, 2, MODE, A>(k, st);
+    else if (p.pieces <= 4) group_rows<T, 1, 4, MODE, A>(k, st);
+    else if (p.pieces <= 16) group_rows<T, 4, 4, MODE, A>(k, st);
+    else if (p.pieces <= 32) group_rows<T, 8, 4, MODE, A>(k, st);
+    else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, A>(k, st);
+    else if (p.pieces <= 128) group_rows<T, 32, 4, MODE, A>(k, st);
+    else group_rows<T, 32, 8, MODE, A>(k, st);
 }
 
 template <typename T, int MODE>
@@ -766,18 +913,13 @@ void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
         static const unsigned most = grid_of(f, 512, 0, 1 << 20);
         f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
     } else if (p.form == RING) {
-        if (p.pieces <= 128 * 8) ring_rows<T, 128, 12, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 256 * 16) ring_rows<T, 256, 24, MODE>(k, p.pieces, st);
-        else ring_rows<T, 512, 26, MODE>(k, p.pieces, st);
+        if (p.pieces <= 1024) ring_rows<T, 128, 2, 6, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 4096) ring_rows<T, 256, 4, 6, MODE>(k, p.pieces, st);
+        else ring_rows<T, 512, 2, 14, MODE>(k, p.pieces, st);
+    } else if (p.aligned && k.b.V % K_OF<T> == 0 && (MODE == LOGP || !k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T)))) {
+        group_rows_of<T, MODE, true>(k, p, st);
     } else {
-        if (p.pieces <= 1) group_rows<T, 1, 1, MODE>(k, st);
-        else if (p.pieces <= 2) group_rows<T, 1, 2, MODE>(k, st);
-        else if (p.pieces <= 4) group_rows<T, 1, 4, MODE>(k, st);
-        else if (p.pieces <= 16) group_rows<T, 4, 4, MODE>(k, st);
-        else if (p.pieces <= 32) group_rows<T, 8, 4, MODE>(k, st);
-        else if (p.pieces <= 64) group_rows<T, 16, 4, MODE>(k, st);
-        else if (p.pieces <= 128) group_rows<T, 32, 4, MODE>(k, st);
-        else group_rows<T, 32, 8, MODE>(k, st);
+        group_rows_of<T, MODE, false>(k, p, st);
     }
 }
 
@@ -866,9 +1008,16 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
         k.b.grad = nullptr;
         k.part = s.part;
         if (const int e = launch_rows<LOGP>(k, p, st)) return e;
-        if (const int e = window_sums(p, b->n, s.part, nullptr, s.win, st)) return e;
     }
-    pairs_kernel<<<1, 1024, 0, st>>>(s.win, b->n, ref, ref_n, beta, smoothing, loss, margins, coef);
+    // up to 32,768 parts the one block adds itself (32 a lane), more a block a window before it
+    int64_t parts = p.tpw;
+    const double* from = s.part;
+    if (p.tiles > 32768) {
+        if (const int e = window_sums(p, b->n, s.part, nullptr, s.win, st)) return e;
+        parts = 1;
+        from = s.win;
+    }
+    pairs_kernel<<<1, 1024, 0, st>>>(from, parts, s.win, b->n, ref, ref_n, beta, smoothing, loss, margins, coef);
     if (const int e = launched()) return e;
     return b->grad ? pv_logprobs_grad(b, coef, 1, 0, nullptr, 0, stream) : PV_OK;
 }
@@ -882,8 +1031,9 @@ int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* 
     if (check_work(s, work, work_bytes)) return PV_EARG;
     const cudaStream_t st = (cudaStream_t)stream;
     if (b->n) {
-        count_kernel<<<(unsigned)std::min<int64_t>(b->n * std::max<int64_t>(p.spans, 1), SMS * 8), 256, 0, st>>>(*b, p.spans, s.counts);
-        weights_kernel<<<1, 1024, 0, st>>>(s.counts, b->n, p.spans, a->by_window, (double)a->scale, weight);
+        const bool one = b->n * b->W <= COUNT_ONE;
+        if (!one) count_kernel<<<(unsigned)std::min<int64_t>(b->n * p.spans, SMS * 8), 256, 0, st>>>(*b, p.spans, s.counts);
+        weights_kernel<<<1, 1024, 0, st>>>(*b, one ? nullptr : s.counts, p.spans, a->by_window, (double)a->scale, weight);
         if (const int e = launched()) return e;
         Rows k = rows_of(*b, p);
         k.part = s.part;

@@ -97,7 +97,7 @@ def _on(dev):
 
 
 def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _work(b, dev, more=0):
@@ -114,6 +114,12 @@ def _with_grad(b, logits, g=None):
     b = _C.Scored.from_buffer_copy(b)
     b.grad, (b.grad_n, b.grad_w, _) = g.data_ptr(), g.stride()
     return b, g
+
+
+def _once(backward):
+    """no second derivative: refused where one is asked for (torch's own wrapper, entered only where a graph is being made)"""
+    refusing = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, up: refusing(ctx, up) if torch.is_grad_enabled() else backward(ctx, up)
 
 
 def _wants_grad(logits):
@@ -139,7 +145,7 @@ class _LogProbs(torch.autograd.Function):
         return _logprobs(b, logits.device, window)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, up):
         logits = ctx.saved_tensors[0]
         up_n, up_w = (up.stride(0), 0) if up.dim() == 1 else up.stride()
@@ -183,7 +189,7 @@ class _Preference(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, up):
         logits = ctx.saved_tensors[0]
         with _on(logits.device):
@@ -251,7 +257,7 @@ class _Policy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, up):
         logits = ctx.saved_tensors[0]
         made, ctx.grad = ctx.grad, None
