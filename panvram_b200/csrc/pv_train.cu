@@ -194,6 +194,7 @@ template <typename T> struct Traits;
 template <> struct Traits<float> { static constexpr uint32_t LOW = 0xFF800000u; };             // -inf, as a word of elements
 template <> struct Traits<__half> { static constexpr uint32_t LOW = 0xFC00FC00u; };
 template <> struct Traits<__nv_bfloat16> { static constexpr uint32_t LOW = 0xFF80FF80u; };
+template <typename T> __device__ __forceinline__ T lowest() { return from32<T>(-INFINITY); }
 template <typename T> constexpr int K_OF = 16 / (int)sizeof(T);
 
 template <typename T> __device__ __forceinline__ void unpack(const uint4& r, float (&x)[K_OF<T>]);
@@ -271,68 +272,131 @@ __device__ __forceinline__ void store_piece(T* d, int e0, int V, bool aligned, c
 template <typename T>
 __device__ __forceinline__ bool alike(const T* x, const T* d) { return (((uintptr_t)x ^ (uintptr_t)d) & 15) == 0; }
 
-// ---------------------------------------------------------------- rows of up to 256 pieces: G lanes a row, NV pieces a lane
-// The row stays in registers from its load to its gradient, so it is read once. A warp takes a tile of 32 rows, 32 / G at
-// a time; each lane loads one row's target and arguments for the whole tile first.
-constexpr int TILE = 32;
+// ---------------------------------------------------------------- asynchronous copies into shared memory
+// places r, r + stride, ... of n windows of W, with their windows and positions
+struct Pos {
+    int64_t r, i, t;
+    __device__ __forceinline__ Pos(int64_t r, int64_t W) : r(r), i(r / W), t(r % W) {}
+    __device__ __forceinline__ void next(int64_t stride, int64_t si, int64_t st, int64_t W) {
+        r += stride; i += si; t += st;
+        if (t >= W) { t -= W; i++; }
+    }
+};
 
-// A: rows of whole pieces, logits' and gradient's alike. Then the next rows' loads are under way while these are worked on.
-template <typename T, int G, int NV, int MODE, bool A>
-__global__ void __launch_bounds__(256, NV <= 4 && MODE != POLICY ? 3 : 2) rows_group_kernel(Rows k) {
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// ---------------------------------------------------------------- rows of up to 256 pieces: G lanes a row, NV pieces a lane
+// A warp takes tiles of 32 rows, 32 / G at a step. Its rows come through a ring of S steps of its own in shared memory: every
+// lane copies its own pieces in and reads them once, into registers, where the row stays until its gradient is out. A step's
+// copy follows S - 1 groups behind its use. The targets of the tile being copied are loaded a tile ahead of it, those and the
+// arguments of the tile being worked on a tile ahead of that, so neither is waited for. The target's logit is read out of
+// the ring and -inf put in its place: the sum of the others and their maximum follow without a comparison an element.
+constexpr int TILE = 32, WARPS = 8;
+
+// A: rows of whole pieces, logits' and gradient's alike
+template <typename T, int G, int NV, int S, int MODE, bool A>
+__global__ void __launch_bounds__(WARPS * 32) rows_group_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G;
-    constexpr bool AHEAD = A && NV <= 4;
+    extern __shared__ uint4 rings[];                         // [WARPS][S][NV][32]
     const int lane = threadIdx.x & 31, sub = lane % G, grp = lane / G, V = (int)k.b.V;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
-    const int64_t tiles = k.b.n * k.tpw, step = (int64_t)gridDim.x * (blockDim.x >> 5);
-    for (int64_t tile = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); tile < tiles; tile += step) {
-        const int64_t i = tile / k.tpw, t0 = (tile - i * k.tpw) * TILE;
-        const int rows = (int)min((int64_t)TILE, k.b.W - t0);
-        const int y_l = lane < rows ? target(k.b, i, t0 + lane) : -1;
-        End end_l = {0.f, 0.f, 0.f};
-        if (y_l >= 0) end_l = end_args<MODE>(k, i, t0 + lane);
+    uint4* const ring = rings + (threadIdx.x >> 5) * (S * NV * 32);
+    // pieces beyond a row's end are never copied: -inf from here on
+#pragma unroll
+    for (int s = 0; s < S * NV; s++) ring[s * 32 + lane] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+
+    const int64_t W = k.b.W, tiles = k.b.n * k.tpw, stride = (int64_t)gridDim.x * WARPS, si = stride / k.tpw, st = stride - si * k.tpw;
+    const int64_t first = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    const auto target_of = [&](const Pos& p) { return p.r < tiles && p.t * TILE + lane < W ? target(k.b, p.i, p.t * TILE + lane) : -1; };
+    const auto end_of = [&](const Pos& p, int y) {
+        const End none = {0.f, 0.f, 0.f};
+        return y >= 0 ? end_args<MODE>(k, p.i, p.t * TILE + lane) : none;
+    };
+
+    // the tile being copied, its targets, and those of the one after it
+    Pos in(first, k.tpw), in_next = in;
+    in_next.next(stride, si, st, k.tpw);
+    int in_y = target_of(in), in_y_next = target_of(in_next), in_s = 0, in_slot = 0;
+    const T* in_x = (const T*)k.b.logits + in.i * k.b.logits_n + in.t * TILE * k.b.logits_w;
+    const auto copy_next = [&]() {
+        if (in.r < tiles) {
+            const int row = in_s * RP + grp, y = __shfl_sync(~0u, in_y, row);
+            if (y >= 0) {
+                const T* x = in_x + row * k.b.logits_w;
+                const int off = A ? 0 : row_off(x);
+#pragma unroll
+                for (int j = 0; j < NV; j++) {
+                    const int e0 = (sub + j * G) * K - off;
+                    uint4* to = ring + (in_slot * NV + j) * 32 + lane;
+                    if (A ? e0 < V : whole<T>(e0, V)) copy16(to, x + e0);
+                    else if (!A) *to = edge_piece(x, e0, V);
+                }
+            }
+            if (++in_s == G) {
+                in_s = 0;
+                in = in_next;
+                in_y = in_y_next;
+                in_next.next(stride, si, st, k.tpw);
+                in_y_next = target_of(in_next);
+                in_x = (const T*)k.b.logits + in.i * k.b.logits_n + in.t * TILE * k.b.logits_w;
+            }
+        }
+        if (++in_slot == S) in_slot = 0;
+        copies_commit();
+    };
+#pragma unroll 1
+    for (int s = 0; s < S; s++) copy_next();
+
+    int slot = 0;
+    Pos p(first, k.tpw);
+    int y_l = target_of(p);
+    End end_l = end_of(p, y_l);
+    while (p.r < tiles) {
+        const int64_t tile = p.r, i = p.i, t0 = p.t * TILE;
+        p.next(stride, si, st, k.tpw);
+        const int y_next = target_of(p);
+        const End end_next = end_of(p, y_next);
+        const int rows = (int)min((int64_t)TILE, W - t0);
         const double w = weight_of<MODE>(k, i);
         const T* const x0 = (const T*)k.b.logits + i * k.b.logits_n + t0 * k.b.logits_w;
         T* const d0 = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t0 * k.b.grad_w : nullptr;
+        float* const lp0 = MODE == LOGP && k.logp ? k.logp + i * W + t0 : nullptr;
         double sum = 0;
-        // rows s0 ... + RP; a group without a counted row loads nothing
-        const auto load = [&](int s0, uint4 (&raw)[NV], float& xt) {
-            const int row = s0 + grp, y = __shfl_sync(~0u, y_l, row);
-            const T* x = x0 + row * k.b.logits_w;
-            const int off = A ? 0 : row_off(x);
+#pragma unroll 1
+        for (int s = 0; s < G; s++) {
+            const int row = s * RP + grp, y = __shfl_sync(~0u, y_l, row), off = A ? 0 : row_off(x0 + row * k.b.logits_w);
+            uint4* const own = ring + slot * NV * 32 + lane;
+            copies_wait<S - 1>();
+            __syncwarp();
+            const int piece = (max(y, 0) + off) / K;
+            T* const at = (T*)(ring + (slot * NV + piece / G) * 32 + grp * G + piece % G) + (max(y, 0) + off) % K;
+            const float xt = f32(*at);
+            __syncwarp();
+            if (piece % G == sub) *at = lowest<T>();
+            uint4 raw[NV];
 #pragma unroll
-            for (int j = 0; j < NV; j++) {
-                raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
-                const int e0 = (sub + j * G) * K - off;
-                if (y >= 0 && e0 < V) {
-                    if (A || whole<T>(e0, V)) raw[j] = *(const uint4*)(x + e0);
-                    else raw[j] = edge_piece(x, e0, V);
-                }
-            }
-            xt = y >= 0 ? f32(x[y]) : 0.f;
-        };
-        uint4 raw[NV], next[AHEAD ? NV : 1];
-        float xt, xt_next = 0.f;
-        if (AHEAD) load(0, raw, xt);
-        for (int s0 = 0; s0 < rows; s0 += RP) {
-            if constexpr (AHEAD) {
-                if (s0 + RP < rows) load(s0 + RP, next, xt_next);
-            } else {
-                load(s0, raw, xt);
-            }
-            const int row = s0 + grp, y = __shfl_sync(~0u, y_l, row);
+            for (int j = 0; j < NV; j++) raw[j] = own[j * 32];
+            copy_next();
+            if (++slot == S) slot = 0;
             float m = piece_max<T>(raw[0]);
 #pragma unroll
             for (int j = 1; j < NV; j++) m = fmaxf(m, piece_max<T>(raw[j]));
 #pragma unroll
-            for (int s = G / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, s));
+            for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
+            m = fmaxf(m, xt);
             const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
             float e[NV][K], o = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; j++) unpack<T>(raw[j], e[j]);
-            if (far(m)) {
+            if (__any_sync(~0u, far(m))) {
+                const float by = far(m) ? m : 0.f;
 #pragma unroll
-                for (int j = 0; j < NV; j++) less(e[j], m);
+                for (int j = 0; j < NV; j++) less(e[j], by);
             }
 #pragma unroll
             for (int j = 0; j < NV; j++) {
@@ -340,22 +404,7 @@ __global__ void __launch_bounds__(256, NV <= 4 && MODE != POLICY ? 3 : 2) rows_g
                 o += sum_of(e[j]);
             }
 #pragma unroll
-            for (int s = G / 2; s; s >>= 1) o += __shfl_xor_sync(~0u, o, s);
-            o -= et;
-            const int off = A ? 0 : row_off(x0 + row * k.b.logits_w);
-            // where the target outweighs the others that difference has lost their digits: they are summed by themselves
-            if (__any_sync(~0u, y >= 0 && !(et < o))) {
-                float p = 0.f;
-#pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    const int at = y - ((sub + j * G) * K - off);
-#pragma unroll
-                    for (int q = 0; q < K; q++) p += q == at ? 0.f : e[j][q];
-                }
-#pragma unroll
-                for (int s = G / 2; s; s >>= 1) p += __shfl_xor_sync(~0u, p, s);
-                if (!(et < o)) o = p;
-            }
+            for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
             const End end = {MODE != LOGP ? __shfl_sync(~0u, end_l.a, row) : 0.f, MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
                              MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
             float lp = 0.f, g = 0.f, term = 0.f;
@@ -365,37 +414,35 @@ __global__ void __launch_bounds__(256, NV <= 4 && MODE != POLICY ? 3 : 2) rows_g
                 if (sub == 0) sum += (double)term;
             }
             if (MODE == LOGP) {
-                if (k.logp && sub == 0 && row < rows) k.logp[i * k.b.W + t0 + row] = lp;
+                if (lp0 && sub == 0 && row < rows) lp0[row] = lp;
             } else if (d0 && row < rows) {
                 T* d = d0 + row * k.b.grad_w;
                 const bool same = A || alike(x0 + row * k.b.logits_w, d);
-                const float inv = 1.f / (o + et), f = y < 0 ? 0.f : -g * inv;
+                const float inv = 1.f / (o + et), f = -g * inv;
 #pragma unroll
                 for (int j = 0; j < NV; j++) {
                     const int e0 = (sub + j * G) * K - off;
+                    times(e[j], f);
                     if (y < 0) {
 #pragma unroll
                         for (int q = 0; q < K; q++) e[j][q] = 0.f;
                     }
-                    times(e[j], f);
                     if (e0 < V) {
                         if (A) *(uint4*)(d + e0) = pack<T>(e[j]);
                         else store_piece(d, e0, V, same, e[j]);
                     }
-                    if (y >= 0 && y >= e0 && y < e0 + K) d[y] = from32<T>(g * (o * inv));
                 }
-            }
-            if constexpr (AHEAD) {
-#pragma unroll
-                for (int j = 0; j < NV; j++) raw[j] = next[j];
-                xt = xt_next;
+                if (y >= 0 && piece % G == sub) d[y] = from32<T>(g * (o * inv));
             }
         }
         if (k.part) {
             sum = warp_sum(sum);
             if (lane == 0) k.part[tile] = sum * w;
         }
+        y_l = y_next;
+        end_l = end_next;
     }
+    copies_wait<0>();
 }
 
 // ---------------------------------------------------------------- longer rows: a block a row
@@ -404,30 +451,13 @@ struct Run { float m = -INFINITY, c = 0.f, o = 0.f; };
 __device__ __forceinline__ void raise(Run& r, float m) {                            // from nothing: 0 times 0
     if (m > r.m) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }
 }
-// adds a piece; at: the target's place in it, if any, whose logit goes to *xt
-template <typename T>
-__device__ __forceinline__ void add(Run& r, const uint4& raw, int at, float* xt) {
-    constexpr int K = K_OF<T>;
-    float x[K];
+template <typename T, bool FAR>
+__device__ __forceinline__ void add(Run& r, const uint4& raw) {
+    float x[K_OF<T>];
     unpack<T>(raw, x);
-    float own = 0.f;
-    if (at >= 0 && at < K) {
-#pragma unroll
-        for (int q = 0; q < K; q++) own = q == at ? x[q] : own;
-        *xt = own;
-    }
-    if (far(r.m) && r.m != -INFINITY) less(x, r.m);                                 // nothing but -inf so far: numerators of 0
+    if (FAR) less(x, far(r.m) && r.m != -INFINITY ? r.m : 0.f);                     // nothing but -inf so far: numerators of 0
     numerators(x, r.c);
-    if (at >= 0 && at < K) {
-#pragma unroll
-        for (int q = 0; q < K; q++) x[q] = q == at ? 0.f : x[q];
-    }
     r.o += sum_of(x);
-}
-template <typename T>
-__device__ __forceinline__ void take(Run& r, const uint4& raw, int at, float* xt) {
-    raise(r, piece_max<T>(raw));
-    add<T>(r, raw, at, xt);
 }
 __device__ __forceinline__ void warp_join(Run& r) {
     const float m = warp_max(r.m);
@@ -455,6 +485,7 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<THREADS>& at,
         Run all;
         if (lane < NW) { const float2 v = at.run[turn][lane]; all.m = v.x; all.o = v.y; }
         warp_join(all);
+        raise(all, at.xt[turn]);                             // the sums leave the target out
         const float c = ref_of(all.m), t = exponent(at.xt[turn], all.m, c), e = ex2(t);
         float term;
         const float lp = MODE == GRAD ? 0.f : row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
@@ -483,38 +514,20 @@ __device__ __forceinline__ void zero_row(T* d, int V, int threads) {
 }
 
 template <typename T>
-__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, int y, const float4& g) {
-    constexpr int K = K_OF<T>;
-    float x[K];
+__device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V, bool same, const float4& g) {
+    float x[K_OF<T>];
     unpack<T>(raw, x);
-    if (far(g.x)) less(x, g.x);
+    less(x, far(g.x) ? g.x : 0.f);
     numerators(x, g.y);
     times(x, g.z);
     store_piece(d, e0, V, same, x);
-    if (y >= e0 && y < e0 + K) d[y] = from32<T>(g.w);
 }
-
-// rows r, r + stride, ... of a batch, with their windows and positions
-struct Pos {
-    int64_t r, i, t;
-    __device__ __forceinline__ Pos(int64_t r, int64_t W) : r(r), i(r / W), t(r % W) {}
-    __device__ __forceinline__ void next(int64_t stride, int64_t si, int64_t st, int64_t W) {
-        r += stride; i += si; t += st;
-        if (t >= W) { t -= W; i++; }
-    }
-};
 
 // Rows that fit a ring of S steps in shared memory, U pieces a thread each. Every thread copies its own pieces in
 // asynchronously and reads only those, so the copies need no barrier: the ring runs ahead into the next rows while this row
 // is reduced, and a step's pieces leave it when the row's gradient has been formed from them. One copy group is committed
 // for every step of either pass (an empty one where nothing is copied), so at least S - 1 groups lie behind the one that a
 // step needs: between a step's copy and its use lie the S - 1 steps that were copied after it, or a whole pass more.
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <typename T, int THREADS, int U, int S, int MODE>
 __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) rows_ring_kernel(Rows k, int steps) {
     constexpr int K = K_OF<T>, SPAN = THREADS * K;           // elements from a thread's piece to its next
@@ -587,25 +600,35 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) r
         End end = {0.f, 0.f, 0.f};
         double w = 1.0;
         if (tid < 32) { end = end_args<MODE>(k, i, t); w = weight_of<MODE>(k, i); }
+        // the target's piece: which thread's, and where in the row it starts
+        const int own_p = (y + off) / K, own_e0 = own_p * K - off, own_u = own_p / THREADS % U;
+        const bool owner = own_p % THREADS == tid;
         Run run;
         int at = slot;
         for (int j = 0; j < steps; j++) {
             const int e0 = (tid + j * U * THREADS) * K - off;
             const uint4* from = &ring[at * U * THREADS + tid];
             copies_wait<S - 1>();
+            if (owner && e0 + own_u * SPAN == own_e0) {       // the target's logit out of the ring, -inf in its place
+                T* own = (T*)&ring[(at * U + own_u) * THREADS + tid] + (y - own_e0);
+                meet.xt[turn] = f32(*own);
+                *own = lowest<T>();
+            }
+            float m = -INFINITY;
             if (inside(e0)) {
-                uint4 raw[U];
 #pragma unroll
-                for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
-                float m = piece_max<T>(raw[0]);
-#pragma unroll
-                for (int u = 1; u < U; u++) m = fmaxf(m, piece_max<T>(raw[u]));
-                raise(run, m);
-#pragma unroll
-                for (int u = 0; u < U; u++) add<T>(run, raw[u], y - e0 - u * SPAN, &meet.xt[turn]);
+                for (int u = 0; u < U; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
             } else {
 #pragma unroll 1
-                for (int u = 0; u < U && e0 + u * SPAN < V; u++) take<T>(run, from[u * THREADS], y - e0 - u * SPAN, &meet.xt[turn]);
+                for (int u = 0; u < U && e0 + u * SPAN < V; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
+            }
+            raise(run, m);
+            if (inside(e0) && !far(run.m)) {
+#pragma unroll
+                for (int u = 0; u < U; u++) add<T, false>(run, from[u * THREADS]);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < U && e0 + u * SPAN < V; u++) add<T, true>(run, from[u * THREADS]);
             }
             if (++at == S) at = 0;
             if (grad) copies_commit(); else copy_next();
@@ -618,21 +641,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) r
             for (int j = 0; j < steps; j++) {
                 const int e0 = (tid + j * U * THREADS) * K - off;
                 const uint4* from = &ring[at * U * THREADS + tid];
-                if (same && inside(e0)) {
+                if (same && inside(e0) && !far(g.x)) {
 #pragma unroll
                     for (int u = 0; u < U; u++) {
                         float v[K];
                         unpack<T>(from[u * THREADS], v);
-                        if (far(g.x)) less(v, g.x);
                         numerators(v, g.y);
                         times(v, g.z);
                         *(uint4*)(d + e0 + u * SPAN) = pack<T>(v);
                     }
-                    if (((y + off) / K) % THREADS == tid && y >= e0 && y < e0 + (U - 1) * SPAN + K) d[y] = from32<T>(g.w);
                 } else {
 #pragma unroll 1
-                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) grad_piece(from[u * THREADS], d, e0 + u * SPAN, V, same, y, g);
+                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) grad_piece(from[u * THREADS], d, e0 + u * SPAN, V, same, g);
                 }
+                if (owner && e0 + own_u * SPAN == own_e0) d[y] = from32<T>(g.w);
                 if (++at == S) at = 0;
                 copy_next();
             }
@@ -686,13 +708,27 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
             }
         };
         Run run;
-        pieces([&](const uint4& raw, int e0) { take<T>(run, raw, y - e0, &meet.xt[turn]); });
+        pieces([&](const uint4& raw, int e0) {
+            alignas(16) T v[K];
+            *(uint4*)v = raw;
+            if (y >= e0 && y < e0 + K) {                     // the target's logit, and -inf in its place
+#pragma unroll
+                for (int q = 0; q < K; q++)
+                    if (q == y - e0) { meet.xt[turn] = f32(v[q]); v[q] = lowest<T>(); }
+            }
+            const uint4 others = *(const uint4*)v;
+            raise(run, piece_max<T>(others));
+            add<T, true>(run, others);
+        });
         const bool grad = MODE != LOGP && d;
         const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
         turn ^= 1;
         if (grad) {
             const bool same = alike(x, d);
-            pieces([&](const uint4& raw, int e0) { grad_piece(raw, d, e0, V, same, y, g); });
+            pieces([&](const uint4& raw, int e0) {
+                grad_piece(raw, d, e0, V, same, g);
+                if (y >= e0 && y < e0 + K) d[y] = from32<T>(g.w);
+            });
         }
     }
 }
@@ -769,7 +805,7 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const double* part, int64_t
 
 // Counted positions of each window, turned into weights: up to COUNT_ONE positions by one block, a warp a window; more by a
 // block per (window, span of it) first.
-constexpr int COUNT_SPAN = 2048, COUNT_ONE = 32768;
+constexpr int COUNT_SPAN = 2048, COUNT_ONE = 4096;
 __global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, int32_t* counts) {
     for (int64_t q = blockIdx.x; q < b.n * spans; q += gridDim.x) {
         const int64_t i = q / spans, t0 = (q - i * spans) * COUNT_SPAN;
@@ -871,25 +907,32 @@ unsigned grid_of(F* f, int threads, size_t smem, int64_t blocks) {
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)SMS * per_sm));
 }
 
+// a kernel's dynamic shared memory, set once per thread and device
+int allow_smem(const void* f, int bytes, uint64_t& set) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !(set >> dev & 1)) {
+        cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (dev < 64) set |= 1ull << dev;
+    }
+    return bytes;
+}
+
 template <typename T, int G, int NV, int MODE, bool A>
 void group_rows(const Rows& k, cudaStream_t st) {
-    const auto f = rows_group_kernel<T, G, NV, MODE, A>;
-    const int64_t tiles = k.b.n * k.tpw;
-    static const unsigned most = grid_of(f, 256, 0, 1 << 20);
-    f<<<(unsigned)std::min<int64_t>((tiles + 7) / 8, most), 256, 0, st>>>(k);
+    constexpr int S = NV <= 4 ? 4 : 3, SMEM = WARPS * S * NV * 512;
+    const auto f = rows_group_kernel<T, G, NV, S, MODE, A>;
+    static thread_local uint64_t set = 0;
+    allow_smem((const void*)f, SMEM, set);
+    static const unsigned most = grid_of(f, WARPS * 32, SMEM, 1 << 20);
+    f<<<(unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most), WARPS * 32, SMEM, st>>>(k);
 }
 
 template <typename T, int THREADS, int U, int S, int MODE>
 void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
     constexpr int SMEM = S * U * THREADS * 16;
     const auto f = rows_ring_kernel<T, THREADS, U, S, MODE>;
-    static thread_local uint64_t set = 0;                    // devices whose attribute is set
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 64 || !(set >> dev & 1)) {
-        cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-        if (dev < 64) set |= 1ull << dev;
-    }
+    static thread_local uint64_t set = 0;
+    allow_smem((const void*)f, SMEM, set);
     static const unsigned most = grid_of(f, THREADS, SMEM, 1 << 20);
     f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), THREADS, SMEM, st>>>(k, (pieces + U * THREADS - 1) / (U * THREADS));
 }
@@ -899,6 +942,7 @@ void group_rows_of(const Rows& k, const Plan& p, cudaStream_t st) {
     if (p.pieces <= 1) group_rows<T, 1, 1, MODE, A>(k, st);
     else if (p.pieces <= 2) group_rows<T, 1, 2, MODE, A>(k, st);
     else if (p.pieces <= 4) group_rows<T, 1, 4, MODE, A>(k, st);
+    else if (p.pieces <= 8) group_rows<T, 2, 4, MODE, A>(k, st);
     else if (p.pieces <= 16) group_rows<T, 4, 4, MODE, A>(k, st);
     else if (p.pieces <= 32) group_rows<T, 8, 4, MODE, A>(k, st);
     else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, A>(k, st);
@@ -1009,10 +1053,10 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
         k.part = s.part;
         if (const int e = launch_rows<LOGP>(k, p, st)) return e;
     }
-    // up to 32,768 parts the one block adds itself (32 a lane), more a block a window before it
+    // up to 4,096 parts the one block adds itself (4 a lane), more a block a window before it
     int64_t parts = p.tpw;
     const double* from = s.part;
-    if (p.tiles > 32768) {
+    if (p.tiles > 4096) {
         if (const int e = window_sums(p, b->n, s.part, nullptr, s.win, st)) return e;
         parts = 1;
         from = s.win;
