@@ -528,36 +528,50 @@ __device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V
 // is reduced, and a step's pieces leave it when the row's gradient has been formed from them. One copy group is committed
 // for every step of either pass (an empty one where nothing is copied), so at least S - 1 groups lie behind the one that a
 // step needs: between a step's copy and its use lie the S - 1 steps that were copied after it, or a whole pass more.
+//
+// A row's target and place take tens of instructions, and every warp needs them: a warp works them out for 32 of its block's
+// rows at once, a lane each, and hands them round by shuffles.
 template <typename T, int THREADS, int U, int S, int MODE>
-__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) rows_ring_kernel(Rows k, int steps) {
+__global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 / (THREADS / 32)) rows_ring_kernel(Rows k, int steps) {
     constexpr int K = K_OF<T>, SPAN = THREADS * K;           // elements from a thread's piece to its next
     extern __shared__ uint4 ring[];                          // [S][U][THREADS]
     __shared__ Meeting<THREADS> meet;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
-    const int tid = threadIdx.x, V = (int)k.b.V;
-    const int64_t W = k.b.W, rows = k.b.n * W, stride = gridDim.x, si = stride / W, st = stride - si * W;
-    const auto target_of = [&](const Pos& p) { return p.r < rows ? target(k.b, p.i, p.t) : -1; };
+    const int tid = threadIdx.x, lane = tid & 31, V = (int)k.b.V;
+    const int64_t W = k.b.W, rows = k.b.n * W, stride = gridDim.x;
     // all U pieces from e0 on lie inside the row
     const auto inside = [&](int e0) { return e0 >= 0 && e0 + (U - 1) * SPAN + K <= V; };
 
-    // what is copied next: step in_j of row `in` (a counted one), into slot in_slot; the row after it is looked up ahead
-    Pos in(blockIdx.x, W), ahead = in;
-    ahead.next(stride, si, st, W);
-    int in_y = target_of(in), ahead_y = target_of(ahead), in_j = 0, in_slot = 0, in_off = 0;
+    // 32 rows from `first` on, a lane each: window, position, target (-1 beyond the last row)
+    struct Lot { int64_t i, t; int y; };
+    const auto lot_of = [&](int64_t first) {
+        const int64_t r = first + lane * stride;
+        Lot q = {r / W, r % W, -1};
+        if (r < rows) q.y = target(k.b, q.i, q.t);
+        return q;
+    };
+
+    // what is copied next: step in_j of the lowest row in in_left, the counted ones of a lot, into slot in_slot
+    int64_t in_first = blockIdx.x, in_at = 0;                // in_at: a lane's row in the logits
+    unsigned in_left = 0;
     const T* in_x = nullptr;
-    const auto find = [&]() {                                // from `in` on to a counted row
-        while (in.r < rows && in_y < 0) {
-            in = ahead;
-            in_y = ahead_y;
-            ahead.next(stride, si, st, W);
-            ahead_y = target_of(ahead);
+    int in_j = 0, in_slot = 0, in_off = 0;
+    const auto find = [&]() {
+        while (!in_left && in_first < rows) {
+            const Lot q = lot_of(in_first);
+            in_left = __ballot_sync(~0u, q.y >= 0);
+            in_at = q.i * k.b.logits_n + q.t * k.b.logits_w;
+            in_first += 32 * stride;
         }
-        if (in.r < rows) { in_x = (const T*)k.b.logits + in.i * k.b.logits_n + in.t * k.b.logits_w; in_off = row_off(in_x); }
+        if (in_left) {
+            in_x = (const T*)k.b.logits + __shfl_sync(~0u, in_at, __ffs(in_left) - 1);
+            in_off = row_off(in_x);
+        }
     };
     find();
     const auto copy_next = [&]() {
-        if (in.r < rows) {
+        if (in_left) {
             const int e0 = (tid + in_j * U * THREADS) * K - in_off;
             uint4* to = &ring[in_slot * U * THREADS + tid];
             if (inside(e0)) {
@@ -571,7 +585,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) r
                     else if (e < V) to[u * THREADS] = edge_piece(in_x, e, V);
                 }
             }
-            if (++in_j == steps) { in_j = 0; in_y = -1; find(); }
+            if (++in_j == steps) {
+                in_j = 0;
+                in_left &= in_left - 1;
+                find();
+            }
         }
         if (++in_slot == S) in_slot = 0;
         copies_commit();
@@ -580,87 +598,98 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 512 / THREADS) r
     for (int s = 0; s < S; s++) copy_next();
 
     int slot = 0, turn = 0;
-    Pos p(blockIdx.x, W);
-    int y = target_of(p);
-    while (p.r < rows) {
-        const int64_t r = p.r, i = p.i, t = p.t;
-        p.next(stride, si, st, W);
-        const int y_next = target_of(p);
-        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
-        if (y < 0) {
-            if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
-            if (MODE != LOGP && d) zero_row(d, V, THREADS);
-            if (k.part && tid == 0) k.part[r] = 0;
-            y = y_next;
-            continue;
-        }
-        const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
-        const int off = row_off(x);
-        const bool grad = MODE != LOGP && d;
-        End end = {0.f, 0.f, 0.f};
-        double w = 1.0;
-        if (tid < 32) { end = end_args<MODE>(k, i, t); w = weight_of<MODE>(k, i); }
-        // the target's piece: which thread's, and where in the row it starts
-        const int own_p = (y + off) / K, own_e0 = own_p * K - off, own_u = own_p / THREADS % U;
-        const bool owner = own_p % THREADS == tid;
-        Run run;
-        int at = slot;
-        for (int j = 0; j < steps; j++) {
-            const int e0 = (tid + j * U * THREADS) * K - off;
-            const uint4* from = &ring[at * U * THREADS + tid];
-            copies_wait<S - 1>();
-            if (owner && e0 + own_u * SPAN == own_e0) {       // the target's logit out of the ring, -inf in its place
-                T* own = (T*)&ring[(at * U + own_u) * THREADS + tid] + (y - own_e0);
-                meet.xt[turn] = f32(*own);
-                *own = lowest<T>();
+    for (int64_t first = blockIdx.x; first < rows; first += 32 * stride) {
+        const Lot lot = lot_of(first);
+        const int64_t x_at = lot.i * k.b.logits_n + lot.t * k.b.logits_w, d_at = lot.i * k.b.grad_n + lot.t * k.b.grad_w;
+        End ends = {0.f, 0.f, 0.f};
+        double ws = 1.0;
+        if (tid < 32 && lot.y >= 0) { ends = end_args<MODE>(k, lot.i, lot.t); ws = weight_of<MODE>(k, lot.i); }
+        for (int l = 0; l < 32; l++) {
+            const int64_t r = first + l * stride;
+            if (r >= rows) break;
+            const int y = __shfl_sync(~0u, lot.y, l);
+            T* const d = MODE != LOGP && k.b.grad ? (T*)k.b.grad + __shfl_sync(~0u, d_at, l) : nullptr;
+            if (y < 0) {
+                if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
+                if (MODE != LOGP && d) zero_row(d, V, THREADS);
+                if (k.part && tid == 0) k.part[r] = 0;
+                continue;
             }
-            float m = -INFINITY;
-            if (inside(e0)) {
-#pragma unroll
-                for (int u = 0; u < U; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
-            } else {
-#pragma unroll 1
-                for (int u = 0; u < U && e0 + u * SPAN < V; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
-            }
-            raise(run, m);
-            if (inside(e0) && !far(run.m)) {
-#pragma unroll
-                for (int u = 0; u < U; u++) add<T, false>(run, from[u * THREADS]);
-            } else {
-#pragma unroll 1
-                for (int u = 0; u < U && e0 + u * SPAN < V; u++) add<T, true>(run, from[u * THREADS]);
-            }
-            if (++at == S) at = 0;
-            if (grad) copies_commit(); else copy_next();
-        }
-        const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
-        turn ^= 1;
-        if (grad) {
-            const bool same = alike(x, d);
-            at = slot;
+            const T* const x = (const T*)k.b.logits + __shfl_sync(~0u, x_at, l);
+            const int off = row_off(x);
+            const bool grad = MODE != LOGP && d;
+            // the target's piece: which thread's, and where in the row it starts
+            const int own_p = (y + off) / K, own_e0 = own_p * K - off, own_u = own_p / THREADS % U;
+            const int own_j = own_p % THREADS == tid ? own_p / (THREADS * U) : -1;
+            Run run;
+            int at = slot;
             for (int j = 0; j < steps; j++) {
                 const int e0 = (tid + j * U * THREADS) * K - off;
-                const uint4* from = &ring[at * U * THREADS + tid];
-                if (same && inside(e0) && !far(g.x)) {
+                uint4* const from = &ring[at * U * THREADS + tid];
+                copies_wait<S - 1>();
+                if (j == own_j) {                            // the target's logit out of the ring, -inf in its place
+                    T* own = (T*)(from + own_u * THREADS) + (y - own_e0);
+                    meet.xt[turn] = f32(*own);
+                    *own = lowest<T>();
+                }
+                const bool in = inside(e0);
+                float m = -INFINITY;
+                if (in) {
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        float v[K];
-                        unpack<T>(from[u * THREADS], v);
-                        numerators(v, g.y);
-                        times(v, g.z);
-                        *(uint4*)(d + e0 + u * SPAN) = pack<T>(v);
-                    }
+                    for (int u = 0; u < U; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
                 } else {
 #pragma unroll 1
-                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) grad_piece(from[u * THREADS], d, e0 + u * SPAN, V, same, g);
+                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
                 }
-                if (owner && e0 + own_u * SPAN == own_e0) d[y] = from32<T>(g.w);
+                raise(run, m);
+                if (in && !far(run.m)) {
+#pragma unroll
+                    for (int u = 0; u < U; u++) add<T, false>(run, from[u * THREADS]);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) add<T, true>(run, from[u * THREADS]);
+                }
                 if (++at == S) at = 0;
-                copy_next();
+                if (grad) copies_commit(); else copy_next();
             }
+            End end = {0.f, 0.f, 0.f};
+            double w = 1.0;
+            if (tid < 32) {
+                if (MODE != LOGP) end.a = __shfl_sync(~0u, ends.a, l);
+                if (MODE == POLICY) {
+                    end.old = __shfl_sync(~0u, ends.old, l);
+                    end.ref = __shfl_sync(~0u, ends.ref, l);
+                    w = __shfl_sync(~0u, ws, l);
+                }
+            }
+            const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
+            turn ^= 1;
+            if (grad) {
+                const bool same = alike(x, d);
+                at = slot;
+                for (int j = 0; j < steps; j++) {
+                    const int e0 = (tid + j * U * THREADS) * K - off;
+                    const uint4* const from = &ring[at * U * THREADS + tid];
+                    if (same && inside(e0) && !far(g.x)) {
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
+                            float v[K];
+                            unpack<T>(from[u * THREADS], v);
+                            numerators(v, g.y);
+                            times(v, g.z);
+                            *(uint4*)(d + e0 + u * SPAN) = pack<T>(v);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int u = 0; u < U && e0 + u * SPAN < V; u++) grad_piece(from[u * THREADS], d, e0 + u * SPAN, V, same, g);
+                    }
+                    if (j == own_j) d[y] = from32<T>(g.w);
+                    if (++at == S) at = 0;
+                    copy_next();
+                }
+            }
+            slot = at;
         }
-        slot = at;
-        y = y_next;
     }
     copies_wait<0>();
 }
@@ -957,8 +986,10 @@ void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
         static const unsigned most = grid_of(f, 512, 0, 1 << 20);
         f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
     } else if (p.form == RING) {
-        if (p.pieces <= 1024) ring_rows<T, 128, 2, 6, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 4096) ring_rows<T, 256, 4, 6, MODE>(k, p.pieces, st);
+        if (p.pieces <= 640) ring_rows<T, 32, 4, 6, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 1280) ring_rows<T, 64, 4, 6, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 2560) ring_rows<T, 128, 4, 6, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 5120) ring_rows<T, 256, 4, 6, MODE>(k, p.pieces, st);
         else ring_rows<T, 512, 2, 14, MODE>(k, p.pieces, st);
     } else if (p.aligned && k.b.V % K_OF<T> == 0 && (MODE == LOGP || !k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T)))) {
         group_rows_of<T, MODE, true>(k, p, st);
