@@ -448,8 +448,12 @@ __global__ void __launch_bounds__(WARPS * 32) rows_group_kernel(Rows k) {
 // ---------------------------------------------------------------- longer rows: a block a row
 // the running maximum and sum of a thread
 struct Run { float m = -INFINITY, c = 0.f, o = 0.f; };
+// The reference is raised only by more than HEADROOM, so that it seldom is: numerators go up to e^8, and the largest is 1 or more.
+constexpr float HEADROOM = 8.f;
 __device__ __forceinline__ void raise(Run& r, float m) {                            // from nothing: 0 times 0
-    if (m > r.m) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }
+    if (__any_sync(~0u, m > r.m + HEADROOM)) {
+        if (m > r.m + HEADROOM) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }
+    }
 }
 template <typename T, bool FAR>
 __device__ __forceinline__ void add(Run& r, const uint4& raw) {
@@ -459,39 +463,85 @@ __device__ __forceinline__ void add(Run& r, const uint4& raw) {
     numerators(x, r.c);
     r.o += sum_of(x);
 }
+template <typename T, int U>
+__device__ __forceinline__ void add_all(Run& r, const uint4 (&raw)[U]) {
+    uint64_t v = pair(r.o, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float x[K_OF<T>];
+        unpack<T>(raw[u], x);
+        numerators(x, r.c);
+#pragma unroll
+        for (int q = 0; q < K_OF<T>; q += 2) asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(v), "l"(pair(x[q], x[q + 1])));
+    }
+    float a, b;
+    halves(v, a, b);
+    r.o = a + b;
+}
 __device__ __forceinline__ void warp_join(Run& r) {
     const float m = warp_max(r.m);
     r.o = warp_sum(r.m == m ? r.o : r.o * rescale(r.m, m));
     r.m = m;
 }
-// What the warps leave for warp 0 at a row's end, and it for them: two of each in turn, so that a row's is written again
-// only behind the barrier of the row between, which warp 0 reaches after reading it.
-template <int THREADS>
+// What the warps leave for the first warp at a row's end (those of all blocks of a cluster for the first warp of each), and
+// it for them: two of each in turn, so that a row's is written again only behind the barrier of the row between, which a
+// first warp reaches after reading it.
+template <int NW>
 struct Meeting {
-    float2 run[2][THREADS / 32];
+    float2 run[2][NW];
     float xt[2];
     float4 grad[2];          // the maximum, the reference, the factor of a numerator and the target's derivative
+    // writes v to the place `at` of this and, in a cluster, of every block's Meeting
+    template <int C> __device__ __forceinline__ void tell(float& at, float v) {
+        if constexpr (C == 1) {
+            at = v;
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; c++) put(&at, c, v);
+        }
+    }
+    static __device__ __forceinline__ void put(float* at, int block, float v) {
+        uint32_t a;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(at)), "r"(block));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+    }
 };
-// Ends a counted row: the threads' sums join, warp 0 takes them to the row's log-probability, term and derivative.
-template <int MODE, int THREADS>
-__device__ __forceinline__ float4 block_end(const Rows& k, Meeting<THREADS>& at, int turn, Run& run, const End& end, double w, float scale, int64_t r,
-                                            bool grad) {
-    constexpr int NW = THREADS / 32;
+// Ends a counted row: the threads' sums join, a first warp takes them to the row's log-probability, term and derivative.
+template <int MODE, int NW, int C>
+__device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, int turn, Run& run, const End& end, double w, float scale, int64_t r,
+                                            bool grad, int rank) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     warp_join(run);
-    if (lane == 0) at.run[turn][warp] = make_float2(run.m, run.o);
-    __syncthreads();
+    if constexpr (C == 1) {
+        if (lane == 0) at.run[turn][warp] = make_float2(run.m, run.o);
+        __syncthreads();
+    } else {
+        if (lane < C) {
+            float* to = (float*)&at.run[turn][rank * NW + warp];
+            at.put(to, lane, run.m);
+            at.put(to + 1, lane, run.o);
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     if (warp == 0) {
         Run all;
-        if (lane < NW) { const float2 v = at.run[turn][lane]; all.m = v.x; all.o = v.y; }
+        for (int q = lane; q < NW * C; q += 32) {
+            const float2 v = at.run[turn][q];
+            const float m = fmaxf(all.m, v.x);
+            all.o = (all.m == m ? all.o : all.o * rescale(all.m, m)) + (v.x == m ? v.y : v.y * rescale(v.x, m));
+            all.m = m;
+        }
         warp_join(all);
-        raise(all, at.xt[turn]);                             // the sums leave the target out
-        const float c = ref_of(all.m), t = exponent(at.xt[turn], all.m, c), e = ex2(t);
+        const float xt = at.xt[turn];
+        if (xt > all.m) { all.o *= rescale(all.m, xt); all.m = xt; }       // the sums leave the target out
+        const float c = ref_of(all.m), t = exponent(xt, all.m, c), e = ex2(t);
         float term;
         const float lp = MODE == GRAD ? 0.f : row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
         if (lane == 0) {
-            if (MODE == LOGP && k.logp) k.logp[r] = lp;
-            if (k.part) k.part[r] = (double)term * w;
+            if (rank == 0) {
+                if (MODE == LOGP && k.logp) k.logp[r] = lp;
+                if (k.part) k.part[r] = (double)term * w;
+            }
             if (grad) {
                 const float inv = 1.f / (all.o + e);
                 at.grad[turn] = make_float4(all.m, c, -g * inv, g * (all.o * inv));
@@ -504,13 +554,13 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<THREADS>& at,
 }
 
 template <typename T>
-__device__ __forceinline__ void zero_row(T* d, int V, int threads) {
+__device__ __forceinline__ void zero_row(T* d, int V, int thread, int threads) {
     constexpr int K = K_OF<T>;
     const int off = row_off(d);
     float z[K];
 #pragma unroll
     for (int q = 0; q < K; q++) z[q] = 0.f;
-    for (int e0 = (int)threadIdx.x * K - off; e0 < V; e0 += threads * K) store_piece(d, e0, V, true, z);
+    for (int e0 = thread * K - off; e0 < V; e0 += threads * K) store_piece(d, e0, V, true, z);
 }
 
 template <typename T>
@@ -529,19 +579,29 @@ __device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V
 // for every step of either pass (an empty one where nothing is copied), so at least S - 1 groups lie behind the one that a
 // step needs: between a step's copy and its use lie the S - 1 steps that were copied after it, or a whole pass more.
 //
+// Only whole pieces go through the ring. The elements before the first and behind the last (up to K - 1 each) are held by a
+// lane each of the first warp.
+//
 // A row's target and place take tens of instructions, and every warp needs them: a warp works them out for 32 of its block's
 // rows at once, a lane each, and hands them round by shuffles.
-template <typename T, int THREADS, int U, int S, int MODE>
-__global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 / (THREADS / 32)) rows_ring_kernel(Rows k, int steps) {
-    constexpr int K = K_OF<T>, SPAN = THREADS * K;           // elements from a thread's piece to its next
+//
+// C: blocks of a cluster that share a row, each a span of its pieces; they leave each other what their warps found in
+// distributed shared memory, behind one cluster barrier a row.
+//
+// warps that a multiprocessor holds with P pieces a thread in the ring, 32 at most (64 registers a thread)
+template <int P> constexpr int RING_WARPS = 220 * 1024 / (P * 512) < 32 ? 220 * 1024 / (P * 512) : 32;
+template <typename T, int THREADS, int U, int S, int C, int MODE>
+__global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) rows_ring_kernel(Rows k, int steps) {
+    constexpr int K = K_OF<T>, SPAN = THREADS * K, NW = THREADS / 32;       // SPAN: elements from a thread's piece to its next
     extern __shared__ uint4 ring[];                          // [S][U][THREADS]
-    __shared__ Meeting<THREADS> meet;
+    __shared__ Meeting<NW * C> meet;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
-    const int tid = threadIdx.x, lane = tid & 31, V = (int)k.b.V;
-    const int64_t W = k.b.W, rows = k.b.n * W, stride = gridDim.x;
-    // all U pieces from e0 on lie inside the row
-    const auto inside = [&](int e0) { return e0 >= 0 && e0 + (U - 1) * SPAN + K <= V; };
+    const int tid = threadIdx.x, lane = tid & 31, V = (int)k.b.V, rank = C > 1 ? (int)blockIdx.x % C : 0;
+    const int64_t W = k.b.W, rows = k.b.n * W, stride = gridDim.x / C, first_row = blockIdx.x / C;
+    // a row's elements before its first whole piece, and its whole pieces; of those this block has span `rank`
+    const auto head_of = [&](const T* x) { return min((int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), V); };
+    const int p0 = tid + rank * steps * U * THREADS;         // this thread's first piece
 
     // 32 rows from `first` on, a lane each: window, position, target (-1 beyond the last row)
     struct Lot { int64_t i, t; int y; };
@@ -553,10 +613,10 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
     };
 
     // what is copied next: step in_j of the lowest row in in_left, the counted ones of a lot, into slot in_slot
-    int64_t in_first = blockIdx.x, in_at = 0;                // in_at: a lane's row in the logits
+    int64_t in_first = first_row, in_at = 0;                 // in_at: a lane's row in the logits
     unsigned in_left = 0;
-    const T* in_x = nullptr;
-    int in_j = 0, in_slot = 0, in_off = 0;
+    const T* in_x = nullptr;                                 // this thread's first piece
+    int in_j = 0, in_slot = 0, in_n = 0;                     // in_n: the row's whole pieces
     const auto find = [&]() {
         while (!in_left && in_first < rows) {
             const Lot q = lot_of(in_first);
@@ -565,25 +625,25 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
             in_first += 32 * stride;
         }
         if (in_left) {
-            in_x = (const T*)k.b.logits + __shfl_sync(~0u, in_at, __ffs(in_left) - 1);
-            in_off = row_off(in_x);
+            const T* x = (const T*)k.b.logits + __shfl_sync(~0u, in_at, __ffs(in_left) - 1);
+            const int head = head_of(x);
+            in_n = (V - head) / K;
+            in_x = x + head + (int64_t)p0 * K;
         }
     };
     find();
     const auto copy_next = [&]() {
         if (in_left) {
-            const int e0 = (tid + in_j * U * THREADS) * K - in_off;
+            const int p = p0 + in_j * U * THREADS;
+            const T* from = in_x + in_j * U * SPAN;
             uint4* to = &ring[in_slot * U * THREADS + tid];
-            if (inside(e0)) {
+            if (__all_sync(~0u, p + (U - 1) * THREADS < in_n)) {
 #pragma unroll
-                for (int u = 0; u < U; u++) copy16(to + u * THREADS, in_x + e0 + u * SPAN);
+                for (int u = 0; u < U; u++) copy16(to + u * THREADS, from + u * SPAN);
             } else {
-#pragma unroll 1
-                for (int u = 0; u < U; u++) {
-                    const int e = e0 + u * SPAN;
-                    if (whole<T>(e, V)) copy16(to + u * THREADS, in_x + e);
-                    else if (e < V) to[u * THREADS] = edge_piece(in_x, e, V);
-                }
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (p + u * THREADS < in_n) copy16(to + u * THREADS, from + u * SPAN);
             }
             if (++in_j == steps) {
                 in_j = 0;
@@ -598,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
     for (int s = 0; s < S; s++) copy_next();
 
     int slot = 0, turn = 0;
-    for (int64_t first = blockIdx.x; first < rows; first += 32 * stride) {
+    for (int64_t first = first_row; first < rows; first += 32 * stride) {
         const Lot lot = lot_of(first);
         const int64_t x_at = lot.i * k.b.logits_n + lot.t * k.b.logits_w, d_at = lot.i * k.b.grad_n + lot.t * k.b.grad_w;
         End ends = {0.f, 0.f, 0.f};
@@ -610,44 +670,67 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
             const int y = __shfl_sync(~0u, lot.y, l);
             T* const d = MODE != LOGP && k.b.grad ? (T*)k.b.grad + __shfl_sync(~0u, d_at, l) : nullptr;
             if (y < 0) {
-                if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
-                if (MODE != LOGP && d) zero_row(d, V, THREADS);
-                if (k.part && tid == 0) k.part[r] = 0;
+                if (rank == 0) {
+                    if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
+                    if (k.part && tid == 0) k.part[r] = 0;
+                }
+                if (MODE != LOGP && d) zero_row(d, V, tid + rank * THREADS, C * THREADS);
                 continue;
             }
             const T* const x = (const T*)k.b.logits + __shfl_sync(~0u, x_at, l);
-            const int off = row_off(x);
             const bool grad = MODE != LOGP && d;
-            // the target's piece: which thread's, and where in the row it starts
-            const int own_p = (y + off) / K, own_e0 = own_p * K - off, own_u = own_p / THREADS % U;
-            const int own_j = own_p % THREADS == tid ? own_p / (THREADS * U) : -1;
+            const int head = head_of(x), n = (V - head) / K, tail = head + n * K;
+            // an element at the row's ends
+            int edge = -1;
+            float ex = -INFINITY;
+            if (tid < 32 && rank == 0) {
+                edge = lane < head ? lane : lane >= 8 && tail + lane - 8 < V ? tail + lane - 8 : -1;
+                if (edge >= 0) ex = f32(x[edge]);
+            }
+            // the target's piece, where it is this thread's: its step and its place in the ring's step
+            int own_j = -1, own_u = 0;
+            if (y >= head && y < tail) {
+                const int q = (y - head) / K - p0;
+                if (q >= 0 && q % THREADS == 0 && q < steps * U * THREADS) { own_j = q / (THREADS * U); own_u = q / THREADS % U; }
+            }
             Run run;
             int at = slot;
             for (int j = 0; j < steps; j++) {
-                const int e0 = (tid + j * U * THREADS) * K - off;
+                const int p = p0 + j * U * THREADS;
                 uint4* const from = &ring[at * U * THREADS + tid];
                 copies_wait<S - 1>();
                 if (j == own_j) {                            // the target's logit out of the ring, -inf in its place
-                    T* own = (T*)(from + own_u * THREADS) + (y - own_e0);
-                    meet.xt[turn] = f32(*own);
+                    T* own = (T*)(from + own_u * THREADS) + (y - head) % K;
+                    meet.template tell<C>(meet.xt[turn], f32(*own));
                     *own = lowest<T>();
                 }
-                const bool in = inside(e0);
-                float m = -INFINITY;
-                if (in) {
+                uint4 raw[U];
+                if (__all_sync(~0u, p + (U - 1) * THREADS < n)) {
 #pragma unroll
-                    for (int u = 0; u < U; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
+                    for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
                 } else {
-#pragma unroll 1
-                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) m = fmaxf(m, piece_max<T>(from[u * THREADS]));
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        raw[u] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+                        if (p + u * THREADS < n) raw[u] = from[u * THREADS];
+                    }
                 }
-                raise(run, m);
-                if (in && !far(run.m)) {
+                float m = piece_max<T>(raw[0]);
 #pragma unroll
-                    for (int u = 0; u < U; u++) add<T, false>(run, from[u * THREADS]);
+                for (int u = 1; u < U; u++) m = fmaxf(m, piece_max<T>(raw[u]));
+                raise(run, m);
+                if (__any_sync(~0u, far(run.m))) {           // a maximum beyond 2^29, or none yet
+                    const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        float v[K];
+                        unpack<T>(raw[u], v);
+                        less(v, by);
+                        numerators(v, run.c);
+                        run.o += sum_of(v);
+                    }
                 } else {
-#pragma unroll 1
-                    for (int u = 0; u < U && e0 + u * SPAN < V; u++) add<T, true>(run, from[u * THREADS]);
+                    add_all<T, U>(run, raw);
                 }
                 if (++at == S) at = 0;
                 if (grad) copies_commit(); else copy_next();
@@ -655,6 +738,12 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
             End end = {0.f, 0.f, 0.f};
             double w = 1.0;
             if (tid < 32) {
+                if (edge == y) {
+                    meet.template tell<C>(meet.xt[turn], ex);
+                    ex = -INFINITY;
+                }
+                raise(run, ex);
+                if (!(ex == -INFINITY)) run.o += ex2(exponent(ex, run.m, run.c));
                 if (MODE != LOGP) end.a = __shfl_sync(~0u, ends.a, l);
                 if (MODE == POLICY) {
                     end.old = __shfl_sync(~0u, ends.old, l);
@@ -662,31 +751,36 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
                     w = __shfl_sync(~0u, ws, l);
                 }
             }
-            const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
+            const float4 g = block_end<MODE, NW, C>(k, meet, turn, run, end, w, scale, r, grad, rank);
             turn ^= 1;
             if (grad) {
-                const bool same = alike(x, d);
+                const bool plain = alike(x, d) && !far(g.x);
+                T* const to = d + head + (int64_t)p0 * K;
                 at = slot;
                 for (int j = 0; j < steps; j++) {
-                    const int e0 = (tid + j * U * THREADS) * K - off;
+                    const int p = p0 + j * U * THREADS;
                     const uint4* const from = &ring[at * U * THREADS + tid];
-                    if (same && inside(e0) && !far(g.x)) {
+                    if (plain) {
+                        const bool all = __all_sync(~0u, p + (U - 1) * THREADS < n);
 #pragma unroll
                         for (int u = 0; u < U; u++) {
+                            if (!all && p + u * THREADS >= n) continue;
                             float v[K];
                             unpack<T>(from[u * THREADS], v);
                             numerators(v, g.y);
                             times(v, g.z);
-                            *(uint4*)(d + e0 + u * SPAN) = pack<T>(v);
+                            *(uint4*)(to + (j * U + u) * SPAN) = pack<T>(v);
                         }
                     } else {
 #pragma unroll 1
-                        for (int u = 0; u < U && e0 + u * SPAN < V; u++) grad_piece(from[u * THREADS], d, e0 + u * SPAN, V, same, g);
+                        for (int u = 0; u < U && p + u * THREADS < n; u++)
+                            grad_piece(from[u * THREADS], d, head + (p + u * THREADS) * K, V, alike(x, d), g);
                     }
                     if (j == own_j) d[y] = from32<T>(g.w);
                     if (++at == S) at = 0;
                     copy_next();
                 }
+                if (edge >= 0) d[edge] = from32<T>(edge == y ? g.w : g.z * ex2(exponent(ex, g.x, g.y)));
             }
             slot = at;
         }
@@ -698,7 +792,7 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 256 ? 512 / THREADS : 16 /
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
     constexpr int K = K_OF<T>, THREADS = 512, U = 4;
-    __shared__ Meeting<THREADS> meet;
+    __shared__ Meeting<THREADS / 32> meet;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     const int tid = threadIdx.x, V = (int)k.b.V;
@@ -710,7 +804,7 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
         const int y = target(k.b, i, t);
         if (y < 0) {
             if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
-            if (MODE != LOGP && d) zero_row(d, V, THREADS);
+            if (MODE != LOGP && d) zero_row(d, V, tid, THREADS);
             if (k.part && tid == 0) k.part[r] = 0;
             continue;
         }
@@ -746,11 +840,12 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
                     if (q == y - e0) { meet.xt[turn] = f32(v[q]); v[q] = lowest<T>(); }
             }
             const uint4 others = *(const uint4*)v;
-            raise(run, piece_max<T>(others));
+            const float m = piece_max<T>(others);
+            if (m > run.m + HEADROOM) { run.o *= rescale(run.m, m); run.m = m; run.c = ref_of(m); }
             add<T, true>(run, others);
         });
         const bool grad = MODE != LOGP && d;
-        const float4 g = block_end<MODE, THREADS>(k, meet, turn, run, end, w, scale, r, grad);
+        const float4 g = block_end<MODE, THREADS / 32, 1>(k, meet, turn, run, end, w, scale, r, grad, 0);
         turn ^= 1;
         if (grad) {
             const bool same = alike(x, d);
@@ -896,9 +991,10 @@ const char* bad_batch(const pv_scored* b) {
 
 // How a batch is run, by its rows' 16-byte pieces (one more than their bytes say where a row may start inside one):
 // up to 256 in registers, G lanes a row; up to RING_MOST in a ring in shared memory, a block a row; else read twice.
-enum { GROUP, RING, LONG };
+enum { SHORT_ROWS, RING_ROWS, LONG_ROWS };
+constexpr int RING = 18;                                 // pieces a thread
 struct Plan { int form, pieces; bool aligned; int64_t tpw, tiles, spans; };
-constexpr int RING_MOST = 14 * 2 * 512;
+constexpr int RING_MOST = 2048 * RING;
 int size_of(int type) { return type == PV_T_FP32 ? 4 : 2; }
 // every row starts at a 16-byte boundary
 bool whole_pieces(const void* p, int64_t n, int64_t w, int64_t size) {
@@ -910,8 +1006,8 @@ Plan plan_of(const pv_scored& b) {
     p.aligned = whole_pieces(b.logits, b.logits_n, b.logits_w, size);
     const int64_t pieces = (b.V + k - 1 + (p.aligned ? 0 : k - 1)) / k;
     p.pieces = (int)std::min<int64_t>(pieces, 1 << 30);
-    p.form = pieces <= 256 ? GROUP : pieces <= RING_MOST ? RING : LONG;
-    p.tpw = p.form == GROUP ? (b.W + TILE - 1) / TILE : b.W;
+    p.form = pieces <= 256 ? SHORT_ROWS : pieces <= RING_MOST ? RING_ROWS : LONG_ROWS;
+    p.tpw = p.form == SHORT_ROWS ? (b.W + TILE - 1) / TILE : b.W;
     p.tiles = b.n * p.tpw;
     p.spans = (b.W + COUNT_SPAN - 1) / COUNT_SPAN;
     return p;
@@ -956,14 +1052,26 @@ void group_rows(const Rows& k, cudaStream_t st) {
     f<<<(unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most), WARPS * 32, SMEM, st>>>(k);
 }
 
-template <typename T, int THREADS, int U, int S, int MODE>
+template <typename T, int THREADS, int U, int S, int C, int MODE>
 void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
     constexpr int SMEM = S * U * THREADS * 16;
-    const auto f = rows_ring_kernel<T, THREADS, U, S, MODE>;
+    const auto f = rows_ring_kernel<T, THREADS, U, S, C, MODE>;
     static thread_local uint64_t set = 0;
     allow_smem((const void*)f, SMEM, set);
     static const unsigned most = grid_of(f, THREADS, SMEM, 1 << 20);
-    f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), THREADS, SMEM, st>>>(k, (pieces + U * THREADS - 1) / (U * THREADS));
+    const int steps = (pieces + C * U * THREADS - 1) / (C * U * THREADS);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(k.b.n * k.b.W, most / C) * C);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, f, k, steps);
 }
 
 template <typename T, int MODE, bool A>
@@ -981,16 +1089,27 @@ void group_rows_of(const Rows& k, const Plan& p, cudaStream_t st) {
 
 template <typename T, int MODE>
 void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
-    if (p.form == LONG) {
+    if (p.form == LONG_ROWS) {
         const auto f = rows_long_kernel<T, MODE>;
         static const unsigned most = grid_of(f, 512, 0, 1 << 20);
         f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
-    } else if (p.form == RING) {
-        if (p.pieces <= 640) ring_rows<T, 32, 4, 6, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 1280) ring_rows<T, 64, 4, 6, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 2560) ring_rows<T, 128, 4, 6, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 5120) ring_rows<T, 256, 4, 6, MODE>(k, p.pieces, st);
-        else ring_rows<T, 512, 2, 14, MODE>(k, p.pieces, st);
+    } else if (p.form == RING_ROWS) {
+        // without a gradient the ring need not hold a row: a warp a row where the rows fill the GPU with 16 warps a
+        // multiprocessor, else four warps or sixteen
+        if constexpr (MODE == LOGP) {
+            const int64_t rows = k.b.n * k.b.W;
+            if (rows >= SMS * 16) ring_rows<T, 32, 4, 3, 1, MODE>(k, p.pieces, st);
+            else if (rows >= SMS * 4) ring_rows<T, 128, 4, 3, 1, MODE>(k, p.pieces, st);
+            else ring_rows<T, 512, 4, 3, 1, MODE>(k, p.pieces, st);
+        } else {
+            if (p.pieces <= 32 * RING) ring_rows<T, 32, 4, 5, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 64 * RING) ring_rows<T, 64, 3, 6, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 128 * 16) ring_rows<T, 128, 4, 4, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 256 * RING) ring_rows<T, 256, 3, 6, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 512 * RING) ring_rows<T, 256, 3, 6, 2, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 1024 * RING) ring_rows<T, 256, 3, 6, 4, MODE>(k, p.pieces, st);
+            else ring_rows<T, 256, 3, 6, 8, MODE>(k, p.pieces, st);
+        }
     } else if (p.aligned && k.b.V % K_OF<T> == 0 && (MODE == LOGP || !k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T)))) {
         group_rows_of<T, MODE, true>(k, p, st);
     } else {
