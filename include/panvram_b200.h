@@ -447,19 +447,22 @@ typedef struct pv_scored {
 
 /* scratch bytes of pv_logprobs / pv_preference / pv_policy on this batch (0: bad arguments or an empty batch) */
 size_t pv_score_work_bytes(const pv_scored* b);
-/* logp[i W + t] = log softmax(logits[i, t])[target], 0 where not counted; sums[i] = its sum over the window. Either may
- * be NULL. b->grad is not used. */
-int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* work, size_t work_bytes, void* stream);
-/* b->grad[i, t] = up[i up_n + t up_w] * *scale * (one at the target - softmax). scale: a device float, or NULL for 1;
- * with skip_one, a *scale of exactly 1 leaves b->grad as it is (it then holds that gradient already). */
-int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t up_w, const float* scale, int skip_one, void* stream);
+/* bytes of the statistics that pv_logprobs_grad takes for this batch: 0 for rows short enough to be worked out again as
+ * they are read (up to about 4 KiB), else 16 a position */
+size_t pv_score_stat_bytes(const pv_scored* b);
+/* logp[i W + t] = log softmax(logits[i, t])[target], 0 where not counted; sums[i] = its sum over the window; stat: the
+ * rows' statistics (pv_score_stat_bytes, 16-byte aligned). Each may be NULL. b->grad is not used. */
+int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* stat, void* work, size_t work_bytes, void* stream);
+/* b->grad[i, t] = up[i up_n + t up_w] * *scale * (one at the target - softmax). scale: a device float, or NULL for 1. stat:
+ * what pv_logprobs or pv_preference left for the same batch (NULL where pv_score_stat_bytes is 0). */
+int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t up_w, const void* stat, const float* scale, void* stream);
 /* The preference loss: windows [0, n/2) preferred over windows [n/2, n), n even. With S the windows' sums of log
  * probabilities and R = ref[i ref_n]: margins[k] = (S - R)[k] - (S - R)[k + n/2], h = beta margins[k],
- * *loss = mean over k of -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h), and coef[i] its derivative by S[i].
- * If b->grad is given it receives the loss's gradient; else pv_logprobs_grad(b, coef, 1, 0, ...) gives it later.
- * margins (float [n/2]) may be NULL; coef float [n]. */
+ * *loss = mean over k of -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h), and coef[i] its derivative by S[i]:
+ * pv_logprobs_grad(b, coef, 1, 0, stat, ...) gives its gradient. margins (float [n/2]) and stat (as pv_logprobs) may be
+ * NULL; coef float [n]. */
 int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float beta, float smoothing, float* loss, float* margins,
-                  float* coef, void* work, size_t work_bytes, void* stream);
+                  float* coef, void* stat, void* work, size_t work_bytes, void* stream);
 /* The clipped policy loss. Per counted position, r = exp(logp - old) and A = adv:
  * -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1) with d = ref - logp. *loss is its mean over
  * the batch's counted positions, or (by_window) the mean over the windows that have any of their own means; 0 if there
@@ -472,7 +475,8 @@ typedef struct pv_policy_args {
     int32_t by_window;
 } pv_policy_args;
 int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* weight, void* work, size_t work_bytes, void* stream);
-/* b->grad = *scale times the loss's gradient, with the weights that pv_policy left (scale, skip_one: pv_logprobs_grad) */
+/* b->grad = *scale times the loss's gradient, with the weights that pv_policy left. scale: a device float, or NULL for 1;
+ * with skip_one, a *scale of exactly 1 leaves b->grad as it is (pv_policy has put that gradient there). */
 int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* weight, const float* scale, int skip_one, void* stream);
 
 /* A list of dense tensors on one device, each contiguous in memory: host arrays of their device addresses, element

@@ -129,9 +129,10 @@ for _name, _res, _args in (
         ("pv_rc_reference", _I32, [_P, _U64, _P, _P]),
         ("pv_windows_trace", _I32, [ctypes.POINTER(DevCohort), _P, _P, _I64, _I64, _P, _I32, _I32, _U32, _P, _P, _P, _SZ, _P, _SZ, _P]),
         ("pv_score_work_bytes", _SZ, [ctypes.POINTER(Scored)]),
-        ("pv_logprobs", _I32, [ctypes.POINTER(Scored), _P, _P, _P, _SZ, _P]),
-        ("pv_logprobs_grad", _I32, [ctypes.POINTER(Scored), _P, _I64, _I64, _P, _I32, _P]),
-        ("pv_preference", _I32, [ctypes.POINTER(Scored), _P, _I64, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _SZ, _P]),
+        ("pv_score_stat_bytes", _SZ, [ctypes.POINTER(Scored)]),
+        ("pv_logprobs", _I32, [ctypes.POINTER(Scored), _P, _P, _P, _P, _SZ, _P]),
+        ("pv_logprobs_grad", _I32, [ctypes.POINTER(Scored), _P, _I64, _I64, _P, _P, _P]),
+        ("pv_preference", _I32, [ctypes.POINTER(Scored), _P, _I64, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P, _SZ, _P]),
         ("pv_policy", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _P, _SZ, _P]),
         ("pv_policy_grad", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _I32, _P]),
         ("pv_grads_work_bytes", _SZ, [ctypes.POINTER(Tensors)]),

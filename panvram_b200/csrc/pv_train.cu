@@ -45,7 +45,9 @@ __device__ __forceinline__ float ex2(float v) {
 }
 
 // ---------------------------------------------------------------- what a row is scored against, and what follows from it
-enum { LOGP = 0, GRAD = 1, POLICY = 2 };
+// LOGP: log-probabilities; GRAD: gradient from given derivatives; GIVEN: the same with the rows' statistics at hand too;
+// POLICY: the policy loss's terms, and their gradient
+enum { LOGP = 0, GRAD = 1, POLICY = 2, GIVEN = 3 };
 
 struct Rows {
     pv_scored b;
@@ -53,12 +55,13 @@ struct Rows {
     // LOGP
     float* logp;             // or NULL
     double* part;            // a partial sum per tile (LOGP: of log-probabilities, POLICY: of loss terms), or NULL
-    // GRAD
+    float4* stat;            // or NULL; GIVEN reads them: a row's maximum, reference, 1 / s and the target's 1 - p
+    // GRAD, GIVEN
     const float* up; int64_t up_n, up_w;
     // POLICY
     pv_policy_args a;
     const double* weight;
-    // GRAD, POLICY
+    // GRAD, GIVEN, POLICY
     const float* scale; int32_t skip_one;
 };
 
@@ -146,7 +149,7 @@ struct End { float a, old, ref; };
 template <int MODE>
 __device__ __forceinline__ End end_args(const Rows& k, int64_t i, int64_t t) {
     End e = {0.f, 0.f, 0.f};
-    if (MODE == GRAD) e.a = k.up[i * k.up_n + t * k.up_w];
+    if (MODE == GRAD || MODE == GIVEN) e.a = k.up[i * k.up_n + t * k.up_w];
     if (MODE == POLICY) {
         e.a = k.a.adv[i * k.a.adv_n + t * k.a.adv_w];
         e.old = k.a.old[i * k.a.old_n + t * k.a.old_w];
@@ -536,16 +539,15 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
         if (xt > all.m) { all.o *= rescale(all.m, xt); all.m = xt; }       // the sums leave the target out
         const float c = ref_of(all.m), t = exponent(xt, all.m, c), e = ex2(t);
         float term;
-        const float lp = MODE == GRAD ? 0.f : row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
+        const float lp = row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
+        const float inv = 1.f / (all.o + e);
         if (lane == 0) {
             if (rank == 0) {
                 if (MODE == LOGP && k.logp) k.logp[r] = lp;
+                if (MODE == LOGP && k.stat) k.stat[r] = make_float4(all.m, c, inv, all.o * inv);
                 if (k.part) k.part[r] = (double)term * w;
             }
-            if (grad) {
-                const float inv = 1.f / (all.o + e);
-                at.grad[turn] = make_float4(all.m, c, -g * inv, g * (all.o * inv));
-            }
+            if (grad) at.grad[turn] = make_float4(all.m, c, -g * inv, g * (all.o * inv));
         }
     }
     if (!grad) return make_float4(0.f, 0.f, 0.f, 0.f);
@@ -663,7 +665,15 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
         const int64_t x_at = lot.i * k.b.logits_n + lot.t * k.b.logits_w, d_at = lot.i * k.b.grad_n + lot.t * k.b.grad_w;
         End ends = {0.f, 0.f, 0.f};
         double ws = 1.0;
-        if (tid < 32 && lot.y >= 0) { ends = end_args<MODE>(k, lot.i, lot.t); ws = weight_of<MODE>(k, lot.i); }
+        float4 stats = make_float4(0.f, 0.f, 0.f, 0.f);      // as a Meeting's grad
+        if ((MODE == GIVEN || tid < 32) && lot.y >= 0) {
+            ends = end_args<MODE>(k, lot.i, lot.t);
+            ws = weight_of<MODE>(k, lot.i);
+            if (MODE == GIVEN) {
+                const float4 v = k.stat[first + lane * stride];
+                stats = make_float4(v.x, v.y, -ends.a * scale * v.z, ends.a * scale * v.w);
+            }
+        }
         for (int l = 0; l < 32; l++) {
             const int64_t r = first + l * stride;
             if (r >= rows) break;
@@ -693,83 +703,96 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                 const int q = (y - head) / K - p0;
                 if (q >= 0 && q % THREADS == 0 && q < steps * U * THREADS) { own_j = q / (THREADS * U); own_u = q / THREADS % U; }
             }
-            Run run;
             int at = slot;
-            for (int j = 0; j < steps; j++) {
-                const int p = p0 + j * U * THREADS;
-                uint4* const from = &ring[at * U * THREADS + tid];
-                copies_wait<S - 1>();
-                if (j == own_j) {                            // the target's logit out of the ring, -inf in its place
-                    T* own = (T*)(from + own_u * THREADS) + (y - head) % K;
-                    meet.template tell<C>(meet.xt[turn], f32(*own));
-                    *own = lowest<T>();
-                }
-                uint4 raw[U];
-                if (__all_sync(~0u, p + (U - 1) * THREADS < n)) {
-#pragma unroll
-                    for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
-                } else {
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        raw[u] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
-                        if (p + u * THREADS < n) raw[u] = from[u * THREADS];
-                    }
-                }
-                float m = piece_max<T>(raw[0]);
-#pragma unroll
-                for (int u = 1; u < U; u++) m = fmaxf(m, piece_max<T>(raw[u]));
-                raise(run, m);
-                if (__any_sync(~0u, far(run.m))) {           // a maximum beyond 2^29, or none yet
-                    const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        float v[K];
-                        unpack<T>(raw[u], v);
-                        less(v, by);
-                        numerators(v, run.c);
-                        run.o += sum_of(v);
-                    }
-                } else {
-                    add_all<T, U>(run, raw);
-                }
-                if (++at == S) at = 0;
-                if (grad) copies_commit(); else copy_next();
-            }
-            End end = {0.f, 0.f, 0.f};
-            double w = 1.0;
-            if (tid < 32) {
-                if (edge == y) {
-                    meet.template tell<C>(meet.xt[turn], ex);
-                    ex = -INFINITY;
-                }
-                raise(run, ex);
-                if (!(ex == -INFINITY)) run.o += ex2(exponent(ex, run.m, run.c));
-                if (MODE != LOGP) end.a = __shfl_sync(~0u, ends.a, l);
-                if (MODE == POLICY) {
-                    end.old = __shfl_sync(~0u, ends.old, l);
-                    end.ref = __shfl_sync(~0u, ends.ref, l);
-                    w = __shfl_sync(~0u, ws, l);
-                }
-            }
-            const float4 g = block_end<MODE, NW, C>(k, meet, turn, run, end, w, scale, r, grad, rank);
-            turn ^= 1;
-            if (grad) {
-                const bool plain = alike(x, d) && !far(g.x);
-                T* const to = d + head + (int64_t)p0 * K;
-                at = slot;
+            float4 g;
+            if constexpr (MODE == GIVEN) {
+                g = make_float4(__shfl_sync(~0u, stats.x, l), __shfl_sync(~0u, stats.y, l), __shfl_sync(~0u, stats.z, l), __shfl_sync(~0u, stats.w, l));
+            } else {
+                Run run;
                 for (int j = 0; j < steps; j++) {
                     const int p = p0 + j * U * THREADS;
-                    const uint4* const from = &ring[at * U * THREADS + tid];
-                    if (plain) {
-                        const bool all = __all_sync(~0u, p + (U - 1) * THREADS < n);
+                    uint4* const from = &ring[at * U * THREADS + tid];
+                    copies_wait<S - 1>();
+                    if (j == own_j) {                        // the target's logit out of the ring, -inf in its place
+                        T* own = (T*)(from + own_u * THREADS) + (y - head) % K;
+                        meet.template tell<C>(meet.xt[turn], f32(*own));
+                        *own = lowest<T>();
+                    }
+                    uint4 raw[U];
+                    if (__all_sync(~0u, p + (U - 1) * THREADS < n)) {
+#pragma unroll
+                        for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
+                    } else {
 #pragma unroll
                         for (int u = 0; u < U; u++) {
-                            if (!all && p + u * THREADS >= n) continue;
+                            raw[u] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+                            if (p + u * THREADS < n) raw[u] = from[u * THREADS];
+                        }
+                    }
+                    float m = piece_max<T>(raw[0]);
+#pragma unroll
+                    for (int u = 1; u < U; u++) m = fmaxf(m, piece_max<T>(raw[u]));
+                    bool plain = true;
+                    if (__any_sync(~0u, m > run.m + HEADROOM || far(run.m))) {
+                        raise(run, m);
+                        plain = !__any_sync(~0u, far(run.m));
+                    }
+                    if (plain) {
+                        add_all<T, U>(run, raw);
+                    } else {                                 // a maximum beyond 2^29, or none yet
+                        const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
+#pragma unroll 1
+                        for (int u = 0; u < U; u++) {
+                            uint4 q = raw[0];
+#pragma unroll
+                            for (int h = 1; h < U; h++)
+                                if (h == u) q = raw[h];
+                            float v[K];
+                            unpack<T>(q, v);
+                            less(v, by);
+                            numerators(v, run.c);
+                            run.o += sum_of(v);
+                        }
+                    }
+                    if (++at == S) at = 0;
+                    if (grad) copies_commit(); else copy_next();
+                }
+                End end = {0.f, 0.f, 0.f};
+                double w = 1.0;
+                if (tid < 32) {
+                    float v = ex;
+                    if (edge == y) {
+                        meet.template tell<C>(meet.xt[turn], ex);
+                        v = -INFINITY;
+                    }
+                    raise(run, v);
+                    if (!(v == -INFINITY)) run.o += ex2(exponent(v, run.m, run.c));
+                    if (MODE == POLICY) {
+                        end.a = __shfl_sync(~0u, ends.a, l);
+                        end.old = __shfl_sync(~0u, ends.old, l);
+                        end.ref = __shfl_sync(~0u, ends.ref, l);
+                        w = __shfl_sync(~0u, ws, l);
+                    }
+                }
+                g = block_end<MODE, NW, C>(k, meet, turn, run, end, w, scale, r, grad, rank);
+                turn ^= 1;
+                if (grad) at = slot;
+            }
+            if (grad) {
+                const bool plain = alike(x, d) && !far(g.x);
+                T* to = d + head + (int64_t)p0 * K;
+                for (int j = 0; j < steps; j++, to += U * SPAN) {
+                    const int p = p0 + j * U * THREADS;
+                    const uint4* const from = &ring[at * U * THREADS + tid];
+                    if (MODE == GIVEN) copies_wait<S - 1>();
+                    if (__all_sync(~0u, plain && p + (U - 1) * THREADS < n)) {
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
                             float v[K];
                             unpack<T>(from[u * THREADS], v);
                             numerators(v, g.y);
                             times(v, g.z);
-                            *(uint4*)(to + (j * U + u) * SPAN) = pack<T>(v);
+                            *(uint4*)(to + u * SPAN) = pack<T>(v);
                         }
                     } else {
 #pragma unroll 1
@@ -788,13 +811,13 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
     copies_wait<0>();
 }
 
-// Rows of any length: read twice, the second time for the gradient.
-template <typename T, int MODE>
+// The policy loss over rows that no cluster holds: read twice, the second time for the gradient.
+template <typename T>
 __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
-    constexpr int K = K_OF<T>, THREADS = 512, U = 4;
+    constexpr int K = K_OF<T>, THREADS = 512, U = 4, MODE = POLICY;
     __shared__ Meeting<THREADS / 32> meet;
-    const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
-    if (MODE != LOGP && k.skip_one && scale == 1.f) return;
+    const float scale = k.scale ? *k.scale : 1.f;
+    if (k.skip_one && scale == 1.f) return;
     const int tid = threadIdx.x, V = (int)k.b.V;
     const int64_t rows = k.b.n * k.b.W;
     int turn = 0;
@@ -803,8 +826,7 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
         T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
         const int y = target(k.b, i, t);
         if (y < 0) {
-            if (MODE == LOGP && k.logp && tid == 0) k.logp[r] = 0.f;
-            if (MODE != LOGP && d) zero_row(d, V, tid, THREADS);
+            if (d) zero_row(d, V, tid, THREADS);
             if (k.part && tid == 0) k.part[r] = 0;
             continue;
         }
@@ -844,7 +866,7 @@ __global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
             if (m > run.m + HEADROOM) { run.o *= rescale(run.m, m); run.m = m; run.c = ref_of(m); }
             add<T, true>(run, others);
         });
-        const bool grad = MODE != LOGP && d;
+        const bool grad = d;
         const float4 g = block_end<MODE, THREADS / 32, 1>(k, meet, turn, run, end, w, scale, r, grad, 0);
         turn ^= 1;
         if (grad) {
@@ -990,7 +1012,8 @@ const char* bad_batch(const pv_scored* b) {
 }
 
 // How a batch is run, by its rows' 16-byte pieces (one more than their bytes say where a row may start inside one):
-// up to 256 in registers, G lanes a row; up to RING_MOST in a ring in shared memory, a block a row; else read twice.
+// up to 256 in registers, G lanes a row; more through a ring in shared memory, where the policy loss needs a row to fit it
+// (RING_MOST; longer ones it reads twice).
 enum { SHORT_ROWS, RING_ROWS, LONG_ROWS };
 constexpr int RING = 18;                                 // pieces a thread
 struct Plan { int form, pieces; bool aligned; int64_t tpw, tiles, spans; };
@@ -1089,31 +1112,32 @@ void group_rows_of(const Rows& k, const Plan& p, cudaStream_t st) {
 
 template <typename T, int MODE>
 void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
-    if (p.form == LONG_ROWS) {
-        const auto f = rows_long_kernel<T, MODE>;
-        static const unsigned most = grid_of(f, 512, 0, 1 << 20);
-        f<<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
-    } else if (p.form == RING_ROWS) {
-        // without a gradient the ring need not hold a row: a warp a row where the rows fill the GPU with 16 warps a
-        // multiprocessor, else four warps or sixteen
-        if constexpr (MODE == LOGP) {
-            const int64_t rows = k.b.n * k.b.W;
-            if (rows >= SMS * 16) ring_rows<T, 32, 4, 3, 1, MODE>(k, p.pieces, st);
-            else if (rows >= SMS * 4) ring_rows<T, 128, 4, 3, 1, MODE>(k, p.pieces, st);
-            else ring_rows<T, 512, 4, 3, 1, MODE>(k, p.pieces, st);
-        } else {
-            if (p.pieces <= 32 * RING) ring_rows<T, 32, 4, 5, 1, MODE>(k, p.pieces, st);
-            else if (p.pieces <= 64 * RING) ring_rows<T, 64, 3, 6, 1, MODE>(k, p.pieces, st);
-            else if (p.pieces <= 128 * 16) ring_rows<T, 128, 4, 4, 1, MODE>(k, p.pieces, st);
-            else if (p.pieces <= 256 * RING) ring_rows<T, 256, 3, 6, 1, MODE>(k, p.pieces, st);
-            else if (p.pieces <= 512 * RING) ring_rows<T, 256, 3, 6, 2, MODE>(k, p.pieces, st);
-            else if (p.pieces <= 1024 * RING) ring_rows<T, 256, 3, 6, 4, MODE>(k, p.pieces, st);
-            else ring_rows<T, 256, 3, 6, 8, MODE>(k, p.pieces, st);
+    if (p.form == SHORT_ROWS) {
+        if constexpr (MODE != GIVEN) {
+            if (p.aligned && k.b.V % K_OF<T> == 0 && (MODE == LOGP || !k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T))))
+                group_rows_of<T, MODE, true>(k, p, st);
+            else
+                group_rows_of<T, MODE, false>(k, p, st);
         }
-    } else if (p.aligned && k.b.V % K_OF<T> == 0 && (MODE == LOGP || !k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T)))) {
-        group_rows_of<T, MODE, true>(k, p, st);
-    } else {
-        group_rows_of<T, MODE, false>(k, p, st);
+    } else if constexpr (MODE == POLICY) {
+        if (p.pieces <= 32 * RING) ring_rows<T, 32, 4, 5, 1, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 64 * RING) ring_rows<T, 64, 3, 6, 1, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 128 * 16) ring_rows<T, 128, 4, 4, 1, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 256 * RING) ring_rows<T, 256, 3, 6, 1, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 512 * RING) ring_rows<T, 256, 3, 6, 2, MODE>(k, p.pieces, st);
+        else if (p.pieces <= 1024 * RING) ring_rows<T, 256, 3, 6, 4, MODE>(k, p.pieces, st);
+        else if (p.form == RING_ROWS) ring_rows<T, 256, 3, 6, 8, MODE>(k, p.pieces, st);
+        else {
+            static const unsigned most = grid_of(rows_long_kernel<T>, 512, 0, 1 << 20);
+            rows_long_kernel<T><<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
+        }
+    } else if constexpr (MODE != GRAD) {
+        // read once, a row need not fit the ring: a warp a row where the rows fill the GPU with 16 warps a multiprocessor,
+        // else four warps or sixteen
+        const int64_t rows = k.b.n * k.b.W;
+        if (rows >= SMS * 16) ring_rows<T, 32, 4, 3, 1, MODE>(k, p.pieces, st);
+        else if (rows >= SMS * 4) ring_rows<T, 128, 4, 3, 1, MODE>(k, p.pieces, st);
+        else ring_rows<T, 512, 4, 3, 1, MODE>(k, p.pieces, st);
     }
 }
 
@@ -1162,7 +1186,12 @@ size_t pv_score_work_bytes(const pv_scored* b) {
     return scratch_of(*b, plan_of(*b), nullptr).bytes;
 }
 
-int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* work, size_t work_bytes, void* stream) {
+size_t pv_score_stat_bytes(const pv_scored* b) {
+    if (bad_batch(b) || plan_of(*b).form == SHORT_ROWS) return 0;
+    return (size_t)b->n * b->W * sizeof(float4);
+}
+
+int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* stat, void* work, size_t work_bytes, void* stream) {
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     const Plan p = plan_of(*b);
     const Scratch s = scratch_of(*b, p, work);
@@ -1171,25 +1200,28 @@ int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* work, size_t
     Rows k = rows_of(*b, p);
     k.b.grad = nullptr;
     k.logp = logp;
+    k.stat = (float4*)stat;
     k.part = sums ? s.part : nullptr;
     const cudaStream_t st = (cudaStream_t)stream;
     if (const int e = launch_rows<LOGP>(k, p, st)) return e;
     return sums ? window_sums(p, b->n, s.part, sums, nullptr, st) : PV_OK;
 }
 
-int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t up_w, const float* scale, int skip_one, void* stream) {
+int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t up_w, const void* stat, const float* scale, void* stream) {
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !up) return fail(PV_EARG, "pv_logprobs_grad: NULL gradient");
     const Plan p = plan_of(*b);
+    if (p.form != SHORT_ROWS && (!stat || ((uintptr_t)stat & 15))) return fail(PV_EARG, "pv_logprobs_grad: rows of this length need their statistics");
     Rows k = rows_of(*b, p);
     k.up = up; k.up_n = up_n; k.up_w = up_w;
-    k.scale = scale; k.skip_one = scale && skip_one;
-    return launch_rows<GRAD>(k, p, (cudaStream_t)stream);
+    k.stat = (float4*)stat;
+    k.scale = scale;
+    return p.form == SHORT_ROWS ? launch_rows<GRAD>(k, p, (cudaStream_t)stream) : launch_rows<GIVEN>(k, p, (cudaStream_t)stream);
 }
 
 int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float beta, float smoothing, float* loss, float* margins, float* coef,
-                  void* work, size_t work_bytes, void* stream) {
+                  void* stat, void* work, size_t work_bytes, void* stream) {
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (b->n & 1) return fail(PV_EARG, "pv_preference: an odd number of windows");
     if (!loss || (b->n && (!ref || !coef))) return fail(PV_EARG, "pv_preference: NULL argument");
@@ -1201,6 +1233,7 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
         Rows k = rows_of(*b, p);
         k.b.grad = nullptr;
         k.part = s.part;
+        k.stat = (float4*)stat;
         if (const int e = launch_rows<LOGP>(k, p, st)) return e;
     }
     // up to 4,096 parts the one block adds itself (4 a lane), more a block a window before it
@@ -1212,8 +1245,7 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
         from = s.win;
     }
     pairs_kernel<<<1, 1024, 0, st>>>(from, parts, s.win, b->n, ref, ref_n, beta, smoothing, loss, margins, coef);
-    if (const int e = launched()) return e;
-    return b->grad ? pv_logprobs_grad(b, coef, 1, 0, nullptr, 0, stream) : PV_OK;
+    return launched();
 }
 
 int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* weight, void* work, size_t work_bytes, void* stream) {

@@ -127,13 +127,16 @@ def _wants_grad(logits):
 
 
 # ---------------------------------------------------------------------- log-probabilities
-def _logprobs(b, dev, window):
+def _logprobs(b, dev, window, keep=False):
+    """-> (log-probabilities, with `keep` a buffer that starts with the rows' statistics)"""
     with _on(dev):
         out = torch.empty((b.n,) if window else (b.n, b.W), dtype=torch.float32, device=dev)
-        kept, work, need = _work(b, dev) if window else (None, None, 0)
-        if _C._lib.pv_logprobs(ctypes.byref(b), None if window else out.data_ptr(), out.data_ptr() if window else None, work, need, _stream(dev)):
+        more = _C._lib.pv_score_stat_bytes(ctypes.byref(b)) if keep else 0
+        buf, work, need = _work(b, dev, more) if window or more else (None, None, 0)
+        if _C._lib.pv_logprobs(ctypes.byref(b), None if window else out.data_ptr(), out.data_ptr() if window else None,
+                               buf.data_ptr() if more else None, work, need, _stream(dev)):
             raise _failed("log-probabilities")
-    return out
+    return out, buf if more else None
 
 
 class _LogProbs(torch.autograd.Function):
@@ -142,7 +145,8 @@ class _LogProbs(torch.autograd.Function):
         # autograd's saved tensors refuse one that is changed in place before the backward pass; b points into them
         ctx.save_for_backward(logits, tokens, mask)
         ctx.b = b
-        return _logprobs(b, logits.device, window)
+        out, ctx.stat = _logprobs(b, logits.device, window, True)
+        return out
 
     @staticmethod
     @_once
@@ -151,7 +155,8 @@ class _LogProbs(torch.autograd.Function):
         up_n, up_w = (up.stride(0), 0) if up.dim() == 1 else up.stride()
         with _on(logits.device):
             b, g = _with_grad(ctx.b, logits)
-            if _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), up_n, up_w, None, 0, _stream(logits.device)):
+            if _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), up_n, up_w,
+                                        ctx.stat.data_ptr() if ctx.stat is not None else None, None, _stream(logits.device)):
                 raise _failed("log-probabilities' gradient")
         return g, None, None, None, None
 
@@ -165,19 +170,22 @@ def window_logprobs(logits, tokens, mask=None, shift=1, ignore=None, reduce="tok
     b = _batch(logits, tokens, mask, shift, ignore)
     if _wants_grad(logits):
         return _LogProbs.apply(logits, tokens, mask, b, reduce == "window")
-    return _logprobs(b, logits.device, reduce == "window")
+    return _logprobs(b, logits.device, reduce == "window")[0]
 
 
 # ---------------------------------------------------------------------- preference
-def _preference(b, dev, ref, beta, smoothing, margins):
-    """-> (loss, a buffer that starts with each window's derivative)"""
+def _preference(b, dev, ref, beta, smoothing, margins, keep=False):
+    """-> (loss, a buffer of the rows' statistics (with `keep`) and each window's derivative, those' address)"""
     with _on(dev):
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        coef, work, need = _work(b, dev, 4 * b.n)
+        more = _C._lib.pv_score_stat_bytes(ctypes.byref(b)) if keep else 0
+        buf, work, need = _work(b, dev, more + 4 * b.n)
+        coef = buf.data_ptr() + more
         if _C._lib.pv_preference(ctypes.byref(b), ref.data_ptr(), ref.stride(0), beta, smoothing, loss.data_ptr(),
-                                 margins.data_ptr() if margins is not None else None, coef.data_ptr(), work, need, _stream(dev)):
+                                 margins.data_ptr() if margins is not None else None, coef, buf.data_ptr() if more else None, work, need,
+                                 _stream(dev)):
             raise _failed("preference loss")
-    return loss, coef
+    return loss, buf, coef
 
 
 class _Preference(torch.autograd.Function):
@@ -185,7 +193,7 @@ class _Preference(torch.autograd.Function):
     def forward(ctx, logits, tokens, mask, b, ref, beta, smoothing, margins):
         ctx.save_for_backward(logits, tokens, mask)
         ctx.b = b
-        loss, ctx.coef = _preference(b, logits.device, ref, beta, smoothing, margins)
+        loss, ctx.buf, ctx.coef = _preference(b, logits.device, ref, beta, smoothing, margins, True)
         return loss
 
     @staticmethod
@@ -194,7 +202,8 @@ class _Preference(torch.autograd.Function):
         logits = ctx.saved_tensors[0]
         with _on(logits.device):
             b, g = _with_grad(ctx.b, logits)
-            if _C._lib.pv_logprobs_grad(ctypes.byref(b), ctx.coef.data_ptr(), 1, 0, up.data_ptr(), 0, _stream(logits.device)):
+            stat = ctx.buf.data_ptr() if ctx.buf.data_ptr() != ctx.coef else None
+            if _C._lib.pv_logprobs_grad(ctypes.byref(b), ctx.coef, 1, 0, stat, up.data_ptr(), _stream(logits.device)):
                 raise _failed("preference loss's gradient")
         return g, None, None, None, None, None, None, None
 

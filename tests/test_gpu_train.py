@@ -174,8 +174,10 @@ def test_unaligned_base_leaves_neighbours_alone(P, cuda, V, off):
             gbuf = torch.full((n * W * V + 64,), 7.0, dtype=x.dtype, device=cuda)
             d = gbuf[goff:goff + n * W * V].view(n, W, V)
             b = train._batch(a, t, None, 1, None)
+            stat = train._logprobs(b, cuda, False, True)[1]
             b.grad, b.grad_n, b.grad_w = d.data_ptr(), d.stride(0), d.stride(1)
-            assert _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), W, 1, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+            assert _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), W, 1, stat.data_ptr() if stat is not None else None, None,
+                                             torch.cuda.current_stream().cuda_stream) == 0
             close(d, *grad_of(x, p, y, ok, up.double()))
             assert (gbuf[:goff] == 7).all() and (gbuf[goff + n * W * V:] == 7).all()
 

@@ -110,9 +110,9 @@ def test_entry_points_refuse_a_bad_batch(kw):
     lib, b = _C._lib, _scored(**kw)
     a = _C.PolicyArgs(64, 64, None, 3, 1, 1, 0, 0, 0, 0.2, 0.2, 0.0, 1.0, 0)
     assert lib.pv_score_work_bytes(b) == 0
-    assert lib.pv_logprobs(b, 64, None, None, 0, None) == _C.PV_EARG and _message().startswith("batch")
-    assert lib.pv_logprobs_grad(b, 64, 0, 0, None, 0, None) == _C.PV_EARG
-    assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 40, None) == _C.PV_EARG
+    assert lib.pv_logprobs(b, 64, None, None, None, 0, None) == _C.PV_EARG and _message().startswith("batch")
+    assert lib.pv_logprobs_grad(b, 64, 0, 0, None, None, None) == _C.PV_EARG
+    assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, None, 64, 1 << 40, None) == _C.PV_EARG
     assert lib.pv_policy(b, ctypes.byref(a), 64, 64, 64, 1 << 40, None) == _C.PV_EARG
     assert lib.pv_policy_grad(b, ctypes.byref(a), 64, None, 0, None) == _C.PV_EARG
 
@@ -120,12 +120,16 @@ def test_entry_points_refuse_a_bad_batch(kw):
 def test_entry_points_refuse_missing_arguments():
     lib, b = _C._lib, _scored()
     good = dict(old=64, adv=64, ref=None, clip_low=0.2, clip_high=0.2, kl=0.0, scale=1.0)
-    assert lib.pv_logprobs(b, None, 64, None, 0, None) == _C.PV_EARG and "scratch" in _message()
-    assert lib.pv_logprobs(b, None, 64, 72, 1 << 30, None) == _C.PV_EARG and "scratch" in _message()      # not 16-byte aligned
-    assert lib.pv_logprobs_grad(b, 64, 0, 0, None, 0, None) == _C.PV_EARG                                  # no gradient to write
-    assert lib.pv_preference(_scored(n=3), 64, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 30, None) == _C.PV_EARG and "odd" in _message()
-    assert lib.pv_preference(b, None, 1, 0.1, 0.0, 64, None, 64, 64, 1 << 30, None) == _C.PV_EARG
-    assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, 64, 1, None) == _C.PV_EARG and "scratch" in _message()
+    assert lib.pv_logprobs(b, None, 64, None, None, 0, None) == _C.PV_EARG and "scratch" in _message()
+    assert lib.pv_logprobs(b, None, 64, None, 72, 1 << 30, None) == _C.PV_EARG and "scratch" in _message()      # not 16-byte aligned
+    assert lib.pv_logprobs_grad(b, 64, 0, 0, None, None, None) == _C.PV_EARG                                  # no gradient to write
+    long = _scored(V=100000, logits_w=100000, logits_n=300000, grad=64)
+    assert lib.pv_score_stat_bytes(b) == 0 and lib.pv_score_stat_bytes(long) == 16 * 2 * 3
+    for stat in (None, 72):                                                                                # missing, not aligned
+        assert lib.pv_logprobs_grad(long, 64, 0, 0, stat, None, None) == _C.PV_EARG and "statistics" in _message()
+    assert lib.pv_preference(_scored(n=3), 64, 1, 0.1, 0.0, 64, None, 64, None, 64, 1 << 30, None) == _C.PV_EARG and "odd" in _message()
+    assert lib.pv_preference(b, None, 1, 0.1, 0.0, 64, None, 64, None, 64, 1 << 30, None) == _C.PV_EARG
+    assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, None, 64, 1, None) == _C.PV_EARG and "scratch" in _message()
     for kw in ({"old": None}, {"adv": None}, {"clip_low": -1.0}, {"clip_high": float("nan")}, {"kl": 0.1}, {"scale": -1.0}):
         assert lib.pv_policy(b, ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, 64, 64, 1 << 30, None) == _C.PV_EARG
         assert lib.pv_policy_grad(_scored(grad=64), ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, None, 0, None) == _C.PV_EARG
