@@ -445,7 +445,7 @@ typedef struct pv_scored {
     int32_t mask_bytes;       /* 0 (none), 1 (uint8) or 4 (float) */
 } pv_scored;
 
-/* scratch bytes of pv_logprobs / pv_preference / pv_policy on this batch (0: bad arguments or an empty batch) */
+/* scratch bytes of pv_logprobs / pv_preference / pv_policy / pv_policy_grad on this batch (0: bad arguments or an empty batch) */
 size_t pv_score_work_bytes(const pv_scored* b);
 /* bytes of the statistics that pv_logprobs_grad takes for this batch: 0 for rows short enough to be worked out again as
  * they are read (up to about 4 KiB), else 16 a position */
@@ -477,7 +477,8 @@ typedef struct pv_policy_args {
 int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* weight, void* work, size_t work_bytes, void* stream);
 /* b->grad = *scale times the loss's gradient, with the weights that pv_policy left. scale: a device float, or NULL for 1;
  * with skip_one, a *scale of exactly 1 leaves b->grad as it is (pv_policy has put that gradient there). */
-int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* weight, const float* scale, int skip_one, void* stream);
+int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* weight, const float* scale, int skip_one, void* work,
+                   size_t work_bytes, void* stream);
 
 /* A list of dense tensors on one device, each contiguous in memory: host arrays of their device addresses, element
  * counts and PV_T_* types. */

@@ -134,7 +134,7 @@ for _name, _res, _args in (
         ("pv_logprobs_grad", _I32, [ctypes.POINTER(Scored), _P, _I64, _I64, _P, _P, _P]),
         ("pv_preference", _I32, [ctypes.POINTER(Scored), _P, _I64, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P, _SZ, _P]),
         ("pv_policy", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _P, _SZ, _P]),
-        ("pv_policy_grad", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _I32, _P]),
+        ("pv_policy_grad", _I32, [ctypes.POINTER(Scored), ctypes.POINTER(PolicyArgs), _P, _P, _I32, _P, _SZ, _P]),
         ("pv_grads_work_bytes", _SZ, [ctypes.POINTER(Tensors)]),
         ("pv_grad_norm", _I32, [ctypes.POINTER(Tensors), _P, _P, _SZ, _P]),
         ("pv_clip_grads", _I32, [ctypes.POINTER(Tensors), ctypes.POINTER(Tensors), ctypes.c_float, _P, _P, _SZ, _P]),

@@ -157,7 +157,9 @@ __device__ void scale_chunk(const T* p, O* o, int count, float f) {
         Vec<O, K> w;
 #pragma unroll
         for (int e = 0; e < K; e++) w.v[e] = from32<O>(f32(v.v[e]) * f);
-        *(Vec<O, K>*)(o + head + j * K) = w;
+        // streaming stores, which leave the gradients in L2 for the chunks to come
+#pragma unroll
+        for (int b = 0; b < (int)(sizeof(O) * K / 16); b++) __stcs((uint4*)(o + head + j * K) + b, ((const uint4*)&w)[b]);
     }
 }
 

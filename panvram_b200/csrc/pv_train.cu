@@ -56,6 +56,7 @@ struct Rows {
     float* logp;             // or NULL
     double* part;            // a partial sum per tile (LOGP: of log-probabilities, POLICY: of loss terms), or NULL
     float4* stat;            // or NULL; GIVEN reads them: a row's maximum, reference, 1 / s and the target's 1 - p
+    float* deriv;            // or NULL; POLICY: each row's derivative
     // GRAD, GIVEN
     const float* up; int64_t up_n, up_w;
     // POLICY
@@ -63,6 +64,7 @@ struct Rows {
     const double* weight;
     // GRAD, GIVEN, POLICY
     const float* scale; int32_t skip_one;
+    int32_t scaled;          // GIVEN: the derivatives have the scale in them
 };
 
 // the target of row (i, t), or -1 (token and mask are loaded side by side)
@@ -217,6 +219,27 @@ template <> __device__ __forceinline__ void unpack<__half>(const uint4& r, float
         x[2 * q] = f.x; x[2 * q + 1] = f.y;
     }
 }
+template <typename T> __device__ __forceinline__ void unpack_word(uint32_t w, float& a, float& b);
+template <> __device__ __forceinline__ void unpack_word<float>(uint32_t w, float& a, float& b) { a = b = __uint_as_float(w); }
+template <> __device__ __forceinline__ void unpack_word<__nv_bfloat16>(uint32_t w, float& a, float& b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xFFFF0000u);
+}
+template <> __device__ __forceinline__ void unpack_word<__half>(uint32_t w, float& a, float& b) {
+    const float2 f = __half22float2(*(const __half2*)&w);
+    a = f.x;
+    b = f.y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack_word(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack_word<float>(float a, float) { return __float_as_uint(a); }
+template <> __device__ __forceinline__ uint32_t pack_word<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&v;
+}
+template <> __device__ __forceinline__ uint32_t pack_word<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&v;
+}
 template <typename T> __device__ __forceinline__ uint4 pack(const float (&x)[K_OF<T>]);
 template <> __device__ __forceinline__ uint4 pack<float>(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
@@ -253,14 +276,9 @@ template <> __device__ __forceinline__ float piece_max<__half>(const uint4& r) {
 // first piece the row starts. The pieces at the row's ends are moved by element, so nothing outside the row is touched.
 template <typename T>
 __device__ __forceinline__ int row_off(const T* x) { return (int)(((uintptr_t)x & 15) / sizeof(T)); }
+// the elements before a row's first whole piece
 template <typename T>
-__device__ __forceinline__ uint4 edge_piece(const T* x, int e0, int V) {       // -inf outside the row
-    constexpr int K = K_OF<T>;
-    alignas(16) T v[K];
-#pragma unroll
-    for (int q = 0; q < K; q++) v[q] = e0 + q >= 0 && e0 + q < V ? x[e0 + q] : from32<T>(-INFINITY);
-    return *(const uint4*)v;
-}
+__device__ __forceinline__ int head_of(const T* x, int V) { return min((int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), V); }
 template <typename T>
 __device__ __forceinline__ bool whole(int e0, int V) { return e0 >= 0 && e0 + K_OF<T> <= V; }
 template <typename T>
@@ -270,6 +288,13 @@ __device__ __forceinline__ void store_piece(T* d, int e0, int V, bool aligned, c
 #pragma unroll
     for (int q = 0; q < K; q++)
         if (e0 + q >= 0 && e0 + q < V) d[e0 + q] = from32<T>(x[q]);
+}
+template <typename T>
+__device__ __forceinline__ void store_raw(T* d, bool aligned, const uint4& v) {
+    if (aligned) { *(uint4*)d = v; return; }
+    const T* q = (const T*)&v;
+#pragma unroll
+    for (int h = 0; h < K_OF<T>; h++) d[h] = q[h];
 }
 // the pieces of x and d fall alike
 template <typename T>
@@ -292,6 +317,36 @@ __device__ __forceinline__ void copy16(void* to, const void* from) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// ---------------------------------------------------------------- sums over pieces
+template <typename T, int U>
+__device__ __forceinline__ float sum_all(const uint4 (&raw)[U], float c, float o) {       // o and the numerators' sum
+    uint64_t v = pair(o, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float x[K_OF<T>];
+        unpack<T>(raw[u], x);
+        numerators(x, c);
+#pragma unroll
+        for (int q = 0; q < K_OF<T>; q += 2) asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(v), "l"(pair(x[q], x[q + 1])));
+    }
+    float a, b;
+    halves(v, a, b);
+    return a + b;
+}
+// the same about a maximum beyond 2^29 (or one of -inf and nothing else, with by 0)
+template <typename T, int U>
+__device__ __noinline__ float sum_far(const uint4* raw, int step, float by, float c, float o) {
+#pragma unroll 1
+    for (int u = 0; u < U; u++) {
+        float x[K_OF<T>];
+        unpack<T>(raw[u * step], x);
+        less(x, by);
+        numerators(x, c);
+        o += sum_of(x);
+    }
+    return o;
+}
+
 // ---------------------------------------------------------------- rows of up to 256 pieces: G lanes a row, NV pieces a lane
 // A warp takes tiles of 32 rows, 32 / G at a step. Its rows come through a ring of S steps of its own in shared memory: every
 // lane copies its own pieces in and reads them once, into registers, where the row stays until its gradient is out. A step's
@@ -300,10 +355,12 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 // the ring and -inf put in its place: the sum of the others and their maximum follow without a comparison an element.
 constexpr int TILE = 32, WARPS = 8;
 
-// A: rows of whole pieces, logits' and gradient's alike
+// A: rows of whole pieces, logits' and gradient's alike. Else (G 16 or more) the elements before a row's first whole piece and
+// behind its last are held by a lane each, as the rows start anywhere.
 template <typename T, int G, int NV, int S, int MODE, bool A>
-__global__ void __launch_bounds__(WARPS * 32) rows_group_kernel(Rows k) {
+__global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP) ? 3 : 2) rows_group_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G;
+    static_assert(A || G >= 16, "a lane for each element at a row's ends");
     extern __shared__ uint4 rings[];                         // [WARPS][S][NV][32]
     const int lane = threadIdx.x & 31, sub = lane % G, grp = lane / G, V = (int)k.b.V;
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
@@ -320,33 +377,33 @@ __global__ void __launch_bounds__(WARPS * 32) rows_group_kernel(Rows k) {
         const End none = {0.f, 0.f, 0.f};
         return y >= 0 ? end_args<MODE>(k, p.i, p.t * TILE + lane) : none;
     };
+    // the first row of this lane's group in a tile, and from it on a step's rows at a time
+    const auto x_of = [&](const Pos& p) { return (const T*)k.b.logits + p.i * k.b.logits_n + (p.t * TILE + grp) * k.b.logits_w; };
+    const int64_t x_step = RP * k.b.logits_w, d_step = RP * k.b.grad_w;
 
     // the tile being copied, its targets, and those of the one after it
     Pos in(first, k.tpw), in_next = in;
     in_next.next(stride, si, st, k.tpw);
     int in_y = target_of(in), in_y_next = target_of(in_next), in_s = 0, in_slot = 0;
-    const T* in_x = (const T*)k.b.logits + in.i * k.b.logits_n + in.t * TILE * k.b.logits_w;
+    const T* in_x = x_of(in);
     const auto copy_next = [&]() {
         if (in.r < tiles) {
-            const int row = in_s * RP + grp, y = __shfl_sync(~0u, in_y, row);
+            const int y = __shfl_sync(~0u, in_y, in_s * RP + grp);
             if (y >= 0) {
-                const T* x = in_x + row * k.b.logits_w;
-                const int off = A ? 0 : row_off(x);
+                const int head = A ? 0 : head_of(in_x, V), n = (V - head) / K;
+                uint4* const to = ring + in_slot * (NV * 32) + lane;
 #pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    const int e0 = (sub + j * G) * K - off;
-                    uint4* to = ring + (in_slot * NV + j) * 32 + lane;
-                    if (A ? e0 < V : whole<T>(e0, V)) copy16(to, x + e0);
-                    else if (!A) *to = edge_piece(x, e0, V);
-                }
+                for (int j = 0; j < NV; j++)
+                    if (sub + j * G < n) copy16(to + j * 32, in_x + head + (sub + j * G) * K);
             }
+            in_x += x_step;
             if (++in_s == G) {
                 in_s = 0;
                 in = in_next;
                 in_y = in_y_next;
                 in_next.next(stride, si, st, k.tpw);
                 in_y_next = target_of(in_next);
-                in_x = (const T*)k.b.logits + in.i * k.b.logits_n + in.t * TILE * k.b.logits_w;
+                in_x = x_of(in);
             }
         }
         if (++in_slot == S) in_slot = 0;
@@ -361,82 +418,309 @@ __global__ void __launch_bounds__(WARPS * 32) rows_group_kernel(Rows k) {
     End end_l = end_of(p, y_l);
     while (p.r < tiles) {
         const int64_t tile = p.r, i = p.i, t0 = p.t * TILE;
+        const T* x = x_of(p);
+        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + (t0 + grp) * k.b.grad_w : nullptr;
         p.next(stride, si, st, k.tpw);
         const int y_next = target_of(p);
         const End end_next = end_of(p, y_next);
         const int rows = (int)min((int64_t)TILE, W - t0);
         const double w = weight_of<MODE>(k, i);
-        const T* const x0 = (const T*)k.b.logits + i * k.b.logits_n + t0 * k.b.logits_w;
-        T* const d0 = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t0 * k.b.grad_w : nullptr;
-        float* const lp0 = MODE == LOGP && k.logp ? k.logp + i * W + t0 : nullptr;
         double sum = 0;
+        // LOGP: the row of this lane's number in the tile, its maximum, others' sum, target's exponent and numerator
+        float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
 #pragma unroll 1
         for (int s = 0; s < G; s++) {
-            const int row = s * RP + grp, y = __shfl_sync(~0u, y_l, row), off = A ? 0 : row_off(x0 + row * k.b.logits_w);
-            uint4* const own = ring + slot * NV * 32 + lane;
+            const int row = s * RP + grp, y = __shfl_sync(~0u, y_l, row);
+            const int head = A ? 0 : head_of(x, V), n = (V - head) / K, tail = head + n * K;
+            int edge = -1;
+            float ex = -INFINITY;
+            if (!A) {
+                edge = sub < head && sub < 8 ? sub : sub >= 8 && tail + sub - 8 < V ? tail + sub - 8 : -1;
+                if (y >= 0 && edge >= 0) ex = f32(x[edge]);
+            }
+            uint4* const base = ring + slot * (NV * 32);
+            uint4* const own = base + lane;
             copies_wait<S - 1>();
             __syncwarp();
-            const int piece = (max(y, 0) + off) / K;
-            T* const at = (T*)(ring + (slot * NV + piece / G) * 32 + grp * G + piece % G) + (max(y, 0) + off) % K;
-            const float xt = f32(*at);
+            const bool in_piece = A || (y >= head && y < tail);
+            const int place = in_piece ? max(y, 0) - head : 0, piece = place / K;
+            T* const at = (T*)(base + piece / G * 32 + grp * G + piece % G) + place % K;
+            float xt = f32(*at);
             __syncwarp();
-            if (piece % G == sub) *at = lowest<T>();
+            const bool owner = in_piece && piece % G == sub;
+            if (owner) *at = lowest<T>();
+            if (!A) {
+                const float v = __shfl_sync(~0u, ex, grp * G + (y < head ? max(y, 0) : 8 + y - tail) % G);
+                if (!in_piece) xt = v;
+                if (edge == y) ex = -INFINITY;
+            }
             uint4 raw[NV];
 #pragma unroll
-            for (int j = 0; j < NV; j++) raw[j] = own[j * 32];
-            copy_next();
-            if (++slot == S) slot = 0;
-            float m = piece_max<T>(raw[0]);
+            for (int j = 0; j < NV; j++) {
+                raw[j] = own[j * 32];
+                if (!A && sub + j * G >= n) raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+            }
+            float m = fmaxf(piece_max<T>(raw[0]), ex);
 #pragma unroll
             for (int j = 1; j < NV; j++) m = fmaxf(m, piece_max<T>(raw[j]));
 #pragma unroll
             for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
             m = fmaxf(m, xt);
             const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
-            float e[NV][K], o = 0.f;
+            const bool any_far = __any_sync(~0u, far(m));
+            float e[MODE == LOGP ? 1 : NV][K], o = 0.f;
+            if constexpr (MODE == LOGP) {
+                if (any_far) {
+#pragma unroll 1
+                    for (int j = 0; j < NV; j++)
+                        if (A || sub + j * G < n) o = sum_far<T, 1>(own + j * 32, 0, far(m) ? m : 0.f, c, o);
+                } else {
+                    o = sum_all<T, NV>(raw, c, 0.f);
+                }
+            } else {
 #pragma unroll
-            for (int j = 0; j < NV; j++) unpack<T>(raw[j], e[j]);
-            if (__any_sync(~0u, far(m))) {
-                const float by = far(m) ? m : 0.f;
+                for (int j = 0; j < NV; j++) unpack<T>(raw[j], e[j]);
+                if (any_far) {
+                    const float by = far(m) ? m : 0.f;
 #pragma unroll
-                for (int j = 0; j < NV; j++) less(e[j], by);
-            }
-#pragma unroll
-            for (int j = 0; j < NV; j++) {
-                numerators(e[j], c);
-                o += sum_of(e[j]);
-            }
-#pragma unroll
-            for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
-            const End end = {MODE != LOGP ? __shfl_sync(~0u, end_l.a, row) : 0.f, MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
-                             MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
-            float lp = 0.f, g = 0.f, term = 0.f;
-            if (y >= 0) {
-                if (MODE != GRAD) lp = row_logp(m, o, t, et);
-                g = row_end<MODE>(k, end, lp, (float)w, scale, term);
-                if (sub == 0) sum += (double)term;
-            }
-            if (MODE == LOGP) {
-                if (lp0 && sub == 0 && row < rows) lp0[row] = lp;
-            } else if (d0 && row < rows) {
-                T* d = d0 + row * k.b.grad_w;
-                const bool same = A || alike(x0 + row * k.b.logits_w, d);
-                const float inv = 1.f / (o + et), f = -g * inv;
+                    for (int j = 0; j < NV; j++) less(e[j], by);
+                }
 #pragma unroll
                 for (int j = 0; j < NV; j++) {
-                    const int e0 = (sub + j * G) * K - off;
-                    times(e[j], f);
-                    if (y < 0) {
-#pragma unroll
-                        for (int q = 0; q < K; q++) e[j][q] = 0.f;
-                    }
-                    if (e0 < V) {
-                        if (A) *(uint4*)(d + e0) = pack<T>(e[j]);
-                        else store_piece(d, e0, V, same, e[j]);
-                    }
+                    numerators(e[j], c);
+                    o += sum_of(e[j]);
                 }
-                if (y >= 0 && piece % G == sub) d[y] = from32<T>(g * (o * inv));
             }
+            const float ee = A ? 0.f : ex2(exponent(ex, m, c));
+            if (!A && edge >= 0) o += ee;
+            copy_next();
+            if (++slot == S) slot = 0;
+#pragma unroll
+            for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
+            if constexpr (MODE == LOGP) {
+                const int from = lane % RP * G;
+                const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, t, from), g = __shfl_sync(~0u, et, from);
+                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; }
+            } else {
+                const End end = {__shfl_sync(~0u, end_l.a, row), MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
+                                 MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
+                float g = 0.f, term = 0.f;
+                if (y >= 0) {
+                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, (float)w, scale, term);
+                    if (MODE == POLICY && sub == 0) sum += (double)term;
+                }
+                if (d && row < rows) {
+                    const bool same = A || alike(x, d);
+                    const float inv = 1.f / (o + et), f = -g * inv;
+#pragma unroll
+                    for (int j = 0; j < NV; j++) {
+                        times(e[j], f);
+                        uint4 v = pack<T>(e[j]);
+                        if (y < 0) v = make_uint4(0u, 0u, 0u, 0u);
+                        if (sub + j * G < n) store_raw(d + head + (sub + j * G) * K, same, v);
+                    }
+                    if (!A && edge >= 0) d[edge] = from32<T>(y < 0 ? 0.f : edge == y ? g * (o * inv) : f * ee);
+                    if (y >= 0 && owner) d[y] = from32<T>(g * (o * inv));
+                }
+                if (d) d += d_step;
+            }
+            x += x_step;
+        }
+        if (MODE == LOGP) {
+            const float lp = y_l >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
+            sum = (double)lp;
+            if (k.logp && lane < rows) k.logp[i * W + t0 + lane] = lp;
+        }
+        if (k.part) {
+            sum = warp_sum(sum);
+            if (lane == 0) k.part[tile] = sum * w;
+        }
+        y_l = y_next;
+        end_l = end_next;
+    }
+    copies_wait<0>();
+}
+
+// ---------------------------------------------------------------- short rows that start anywhere, one behind the other
+// Here a step's rows are copied as one stretch, in the 16-byte pieces it covers whole (the elements at the stretch's two ends
+// by a lane each), into an image of it in shared memory. A group of G lanes takes a row from the image in its 32-bit words,
+// lane by lane; of a first or last word that it shares with its neighbour it masks the half that is not its own. The gradient
+// replaces the logits in the image and leaves as the stretch came.
+template <typename T> __device__ __forceinline__ float word_max(uint32_t a, float m);
+template <> __device__ __forceinline__ float word_max<float>(uint32_t a, float m) { return fmaxf(m, __uint_as_float(a)); }
+template <> __device__ __forceinline__ float word_max<__nv_bfloat16>(uint32_t a, float m) {
+    return fmaxf(m, fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u)));
+}
+template <> __device__ __forceinline__ float word_max<__half>(uint32_t a, float m) {
+    const float2 f = __half22float2(*(const __half2*)&a);
+    return fmaxf(m, fmaxf(f.x, f.y));
+}
+
+// NW: words a lane
+template <typename T, int G, int NW, int S, int MODE>
+__global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) rows_flat_kernel(Rows k) {
+    constexpr int K = K_OF<T>, RP = 32 / G, E = 4 / (int)sizeof(T), N = (NW * E + 1) / 2 * 2;      // E: elements a word
+    constexpr int SLOT = (NW * 32 * 4 + 47) / 16;            // 16-byte pieces of an image
+    extern __shared__ uint4 rings[];                         // [WARPS][S][SLOT]
+    const int lane = threadIdx.x & 31, sub = lane % G, grp = lane / G, V = (int)k.b.V;
+    const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
+    if (MODE != LOGP && k.skip_one && scale == 1.f) return;
+    uint4* const ring = rings + (threadIdx.x >> 5) * (S * SLOT);
+
+    const int64_t W = k.b.W, tiles = k.b.n * k.tpw, stride = (int64_t)gridDim.x * WARPS, si = stride / k.tpw, st = stride - si * k.tpw;
+    const int64_t first = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    const auto target_of = [&](const Pos& p) { return p.r < tiles && p.t * TILE + lane < W ? target(k.b, p.i, p.t * TILE + lane) : -1; };
+    const auto end_of = [&](const Pos& p, int y) {
+        const End none = {0.f, 0.f, 0.f};
+        return y >= 0 ? end_args<MODE>(k, p.i, p.t * TILE + lane) : none;
+    };
+    const auto x_of = [&](const Pos& p) { return (const T*)k.b.logits + p.i * k.b.logits_n + p.t * TILE * V; };
+    const auto rows_of_tile = [&](const Pos& p) { return (int)min((int64_t)TILE, W - p.t * TILE); };
+    constexpr unsigned STEP = RP == 32 ? ~0u : (1u << RP) - 1;
+    // a step's stretch: how far into its first piece it starts, its elements
+    struct Stretch { int off, len; };
+    const auto stretch = [&](const T* x, int s, int rows) { return Stretch{row_off(x), max(0, min(RP, rows - s * RP)) * V}; };
+
+    Pos in(first, k.tpw), in_next = in;
+    in_next.next(stride, si, st, k.tpw);
+    unsigned in_on = __ballot_sync(~0u, target_of(in) >= 0);
+    int in_y_next = target_of(in_next), in_s = 0, in_slot = 0;
+    const T* in_x = x_of(in);
+    const auto copy_next = [&]() {
+        if (in.r < tiles) {
+            if (in_on >> (in_s * RP) & STEP) {
+                const Stretch q = stretch(in_x, in_s, rows_of_tile(in));
+                uint4* const to = ring + in_slot * SLOT;
+                const T* const from = in_x - q.off;
+                for (int p = lane + (q.off > 0); (p + 1) * K <= q.off + q.len; p += 32) copy16(to + p, from + p * K);
+            }
+            in_x += RP * V;
+            if (++in_s == G) {
+                in_s = 0;
+                in = in_next;
+                in_on = __ballot_sync(~0u, in_y_next >= 0);
+                in_next.next(stride, si, st, k.tpw);
+                in_y_next = target_of(in_next);
+                in_x = x_of(in);
+            }
+        }
+        if (++in_slot == S) in_slot = 0;
+        copies_commit();
+    };
+#pragma unroll 1
+    for (int s = 0; s < S; s++) copy_next();
+
+    int slot = 0;
+    Pos p(first, k.tpw);
+    int y_l = target_of(p);
+    End end_l = end_of(p, y_l);
+    while (p.r < tiles) {
+        const int64_t tile = p.r, i = p.i, t0 = p.t * TILE;
+        const T* x = x_of(p);
+        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t0 * V : nullptr;
+        const int rows = rows_of_tile(p);
+        p.next(stride, si, st, k.tpw);
+        const int y_next = target_of(p);
+        const End end_next = end_of(p, y_next);
+        const double w = weight_of<MODE>(k, i);
+        const unsigned on = __ballot_sync(~0u, y_l >= 0);
+        double sum = 0;
+        float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
+#pragma unroll 1
+        for (int s = 0; s < G; s++, x += RP * V) {
+            const int row = s * RP + grp, y = __shfl_sync(~0u, y_l, row);
+            const Stretch q = stretch(x, s, rows);
+            const bool any = on >> (s * RP) & STEP;
+            uint4* const base = ring + slot * SLOT;
+            T* const img = (T*)base;
+            // the stretch's elements before its first whole piece and behind its last
+            const int head = min((K - q.off) % K, q.len), tail = max(head, (q.off + q.len) / K * K - q.off);
+            const int edge = lane < 8 ? (lane < head ? lane : -1) : lane < 16 && tail + lane - 8 < q.len ? tail + lane - 8 : -1;
+            T ev = lowest<T>();
+            if (any && edge >= 0) ev = x[edge];
+            copies_wait<S - 1>();
+            if (edge >= 0) img[q.off + edge] = ev;
+            __syncwarp();
+            const int at = q.off + grp * V, w0 = at / E, w1 = (at + V - 1) / E, ty = at + max(y, 0);
+            float xt = 0.f;
+            if (y >= 0) xt = f32(img[ty]);
+            __syncwarp();
+            if (y >= 0 && sub == 0) img[ty] = lowest<T>();
+            __syncwarp();
+            uint32_t raw[NW];
+            float m = xt;
+            if (y < 0) m = 0.f;
+#pragma unroll
+            for (int j = 0; j < NW; j++) {
+                const int v = w0 + sub + j * G;
+                raw[j] = Traits<T>::LOW;
+                if (y >= 0 && v <= w1) raw[j] = ((const uint32_t*)base)[v];
+                if (E == 2) {
+                    if (j == 0 && sub == 0 && at % 2) raw[j] = raw[j] & 0xFFFF0000u | Traits<T>::LOW & 0xFFFFu;
+                    if (v == w1 && (at + V) % 2) raw[j] = raw[j] & 0xFFFFu | Traits<T>::LOW & 0xFFFF0000u;
+                }
+                m = word_max<T>(raw[j], m);
+            }
+#pragma unroll
+            for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
+            const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
+            float e[N];
+            e[N - 1] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NW; j++) {
+                if (E == 1) e[j] = __uint_as_float(raw[j]);
+                else unpack_word<T>(raw[j], e[2 * j < N ? 2 * j : 0], e[2 * j + 1 < N ? 2 * j + 1 : 0]);
+            }
+            if (__any_sync(~0u, far(m))) less(e, far(m) ? m : 0.f);
+            numerators(e, c);
+            float o = sum_of(e);
+#pragma unroll
+            for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
+            if constexpr (MODE == LOGP) {
+                const int from = lane % RP * G;
+                const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, t, from), g = __shfl_sync(~0u, et, from);
+                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; }
+            } else {
+                const End end = {__shfl_sync(~0u, end_l.a, row), MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
+                                 MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
+                float g = 0.f, term = 0.f;
+                if (y >= 0) {
+                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, (float)w, scale, term);
+                    if (MODE == POLICY && sub == 0) sum += (double)term;
+                }
+                if (d) {
+                    const float inv = 1.f / (o + et), f = -g * inv;
+                    times(e, f);
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < NW; j++) {
+                        const int v = w0 + sub + j * G;
+                        uint32_t z = E == 1 ? __float_as_uint(e[j]) : pack_word<T>(e[2 * j < N ? 2 * j : 0], e[2 * j + 1 < N ? 2 * j + 1 : 0]);
+                        if (y < 0) z = 0u;
+                        if (row < rows && v <= w1) {
+                            const bool low = E == 1 || !(j == 0 && sub == 0 && at % 2), high = E == 1 || !(v == w1 && (at + V) % 2);
+                            if (low && high) ((uint32_t*)base)[v] = z;
+                            else if (low) ((uint16_t*)base)[2 * v] = (uint16_t)z;
+                            else if (high) ((uint16_t*)base)[2 * v + 1] = (uint16_t)(z >> 16);
+                        }
+                    }
+                    __syncwarp();
+                    if (y >= 0 && sub == 0) img[ty] = from32<T>(g * (o * inv));
+                    __syncwarp();
+                    T* const to = d - q.off;
+                    for (int v = lane + (q.off > 0); (v + 1) * K <= q.off + q.len; v += 32) *(uint4*)(to + v * K) = base[v];
+                    if (edge >= 0) d[edge] = img[q.off + edge];
+                    d += RP * V;
+                }
+            }
+            __syncwarp();
+            copy_next();
+            if (++slot == S) slot = 0;
+        }
+        if (MODE == LOGP) {
+            const float lp = y_l >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
+            sum = (double)lp;
+            if (k.logp && lane < rows) k.logp[i * W + t0 + lane] = lp;
         }
         if (k.part) {
             sum = warp_sum(sum);
@@ -457,29 +741,6 @@ __device__ __forceinline__ void raise(Run& r, float m) {                        
     if (__any_sync(~0u, m > r.m + HEADROOM)) {
         if (m > r.m + HEADROOM) { r.o *= rescale(r.m, m); r.m = m; r.c = ref_of(m); }
     }
-}
-template <typename T, bool FAR>
-__device__ __forceinline__ void add(Run& r, const uint4& raw) {
-    float x[K_OF<T>];
-    unpack<T>(raw, x);
-    if (FAR) less(x, far(r.m) && r.m != -INFINITY ? r.m : 0.f);                     // nothing but -inf so far: numerators of 0
-    numerators(x, r.c);
-    r.o += sum_of(x);
-}
-template <typename T, int U>
-__device__ __forceinline__ void add_all(Run& r, const uint4 (&raw)[U]) {
-    uint64_t v = pair(r.o, 0.f);
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        float x[K_OF<T>];
-        unpack<T>(raw[u], x);
-        numerators(x, r.c);
-#pragma unroll
-        for (int q = 0; q < K_OF<T>; q += 2) asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(v), "l"(pair(x[q], x[q + 1])));
-    }
-    float a, b;
-    halves(v, a, b);
-    r.o = a + b;
 }
 __device__ __forceinline__ void warp_join(Run& r) {
     const float m = warp_max(r.m);
@@ -515,7 +776,9 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
                                             bool grad, int rank) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     warp_join(run);
-    if constexpr (C == 1) {
+    if constexpr (NW * C == 1) {
+        __syncwarp();
+    } else if constexpr (C == 1) {
         if (lane == 0) at.run[turn][warp] = make_float2(run.m, run.o);
         __syncthreads();
     } else {
@@ -527,14 +790,17 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     if (warp == 0) {
-        Run all;
-        for (int q = lane; q < NW * C; q += 32) {
-            const float2 v = at.run[turn][q];
-            const float m = fmaxf(all.m, v.x);
-            all.o = (all.m == m ? all.o : all.o * rescale(all.m, m)) + (v.x == m ? v.y : v.y * rescale(v.x, m));
-            all.m = m;
+        Run all = run;
+        if constexpr (NW * C > 1) {
+            all = Run();
+            for (int q = lane; q < NW * C; q += 32) {
+                const float2 v = at.run[turn][q];
+                const float m = fmaxf(all.m, v.x);
+                all.o = (all.m == m ? all.o : all.o * rescale(all.m, m)) + (v.x == m ? v.y : v.y * rescale(v.x, m));
+                all.m = m;
+            }
+            warp_join(all);
         }
-        warp_join(all);
         const float xt = at.xt[turn];
         if (xt > all.m) { all.o *= rescale(all.m, xt); all.m = xt; }       // the sums leave the target out
         const float c = ref_of(all.m), t = exponent(xt, all.m, c), e = ex2(t);
@@ -544,14 +810,15 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
         if (lane == 0) {
             if (rank == 0) {
                 if (MODE == LOGP && k.logp) k.logp[r] = lp;
-                if (MODE == LOGP && k.stat) k.stat[r] = make_float4(all.m, c, inv, all.o * inv);
+                if (k.stat) k.stat[r] = make_float4(all.m, c, inv, all.o * inv);
+                if (MODE == POLICY && k.deriv) k.deriv[r] = g;
                 if (k.part) k.part[r] = (double)term * w;
             }
             if (grad) at.grad[turn] = make_float4(all.m, c, -g * inv, g * (all.o * inv));
         }
     }
     if (!grad) return make_float4(0.f, 0.f, 0.f, 0.f);
-    __syncthreads();
+    if constexpr (NW * C == 1) __syncwarp(); else __syncthreads();
     return at.grad[turn];
 }
 
@@ -601,8 +868,7 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     const int tid = threadIdx.x, lane = tid & 31, V = (int)k.b.V, rank = C > 1 ? (int)blockIdx.x % C : 0;
     const int64_t W = k.b.W, rows = k.b.n * W, stride = gridDim.x / C, first_row = blockIdx.x / C;
-    // a row's elements before its first whole piece, and its whole pieces; of those this block has span `rank`
-    const auto head_of = [&](const T* x) { return min((int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)), V); };
+    // of a row's whole pieces this block has span `rank`
     const int p0 = tid + rank * steps * U * THREADS;         // this thread's first piece
 
     // 32 rows from `first` on, a lane each: window, position, target (-1 beyond the last row)
@@ -628,7 +894,7 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
         }
         if (in_left) {
             const T* x = (const T*)k.b.logits + __shfl_sync(~0u, in_at, __ffs(in_left) - 1);
-            const int head = head_of(x);
+            const int head = head_of(x, V);
             in_n = (V - head) / K;
             in_x = x + head + (int64_t)p0 * K;
         }
@@ -671,7 +937,8 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
             ws = weight_of<MODE>(k, lot.i);
             if (MODE == GIVEN) {
                 const float4 v = k.stat[first + lane * stride];
-                stats = make_float4(v.x, v.y, -ends.a * scale * v.z, ends.a * scale * v.w);
+                const float g = k.scaled ? ends.a : ends.a * scale;
+                stats = make_float4(v.x, v.y, -g * v.z, g * v.w);
             }
         }
         for (int l = 0; l < 32; l++) {
@@ -689,7 +956,7 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
             }
             const T* const x = (const T*)k.b.logits + __shfl_sync(~0u, x_at, l);
             const bool grad = MODE != LOGP && d;
-            const int head = head_of(x), n = (V - head) / K, tail = head + n * K;
+            const int head = head_of(x, V), n = (V - head) / K, tail = head + n * K;
             // an element at the row's ends
             int edge = -1;
             float ex = -INFINITY;
@@ -738,21 +1005,12 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                         plain = !__any_sync(~0u, far(run.m));
                     }
                     if (plain) {
-                        add_all<T, U>(run, raw);
+                        run.o = sum_all<T, U>(raw, run.c, run.o);
                     } else {                                 // a maximum beyond 2^29, or none yet
                         const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
 #pragma unroll 1
-                        for (int u = 0; u < U; u++) {
-                            uint4 q = raw[0];
-#pragma unroll
-                            for (int h = 1; h < U; h++)
-                                if (h == u) q = raw[h];
-                            float v[K];
-                            unpack<T>(q, v);
-                            less(v, by);
-                            numerators(v, run.c);
-                            run.o += sum_of(v);
-                        }
+                        for (int u = 0; u < U; u++)
+                            if (p + u * THREADS < n) run.o = sum_far<T, 1>(from + u * THREADS, 0, by, run.c, run.o);
                     }
                     if (++at == S) at = 0;
                     if (grad) copies_commit(); else copy_next();
@@ -809,74 +1067,6 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
         }
     }
     copies_wait<0>();
-}
-
-// The policy loss over rows that no cluster holds: read twice, the second time for the gradient.
-template <typename T>
-__global__ void __launch_bounds__(512) rows_long_kernel(Rows k) {
-    constexpr int K = K_OF<T>, THREADS = 512, U = 4, MODE = POLICY;
-    __shared__ Meeting<THREADS / 32> meet;
-    const float scale = k.scale ? *k.scale : 1.f;
-    if (k.skip_one && scale == 1.f) return;
-    const int tid = threadIdx.x, V = (int)k.b.V;
-    const int64_t rows = k.b.n * k.b.W;
-    int turn = 0;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int64_t i = r / k.b.W, t = r - i * k.b.W;
-        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t * k.b.grad_w : nullptr;
-        const int y = target(k.b, i, t);
-        if (y < 0) {
-            if (d) zero_row(d, V, tid, THREADS);
-            if (k.part && tid == 0) k.part[r] = 0;
-            continue;
-        }
-        const T* x = (const T*)k.b.logits + i * k.b.logits_n + t * k.b.logits_w;
-        const int off = row_off(x);
-        End end = {0.f, 0.f, 0.f};
-        double w = 1.0;
-        if (tid < 32) { end = end_args<MODE>(k, i, t); w = weight_of<MODE>(k, i); }
-        // pieces of the row, U at a time in flight; 64-bit places, as the last step may pass 2^31
-        const auto pieces = [&](auto&& f) {
-            for (int64_t p0 = tid; p0 * K - off < V; p0 += THREADS * U) {
-                uint4 raw[U];
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int64_t e0 = (p0 + u * THREADS) * K - off;
-                    if (e0 >= V) continue;
-                    raw[u] = whole<T>((int)e0, V) ? *(const uint4*)(x + e0) : edge_piece(x, (int)e0, V);
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int64_t e0 = (p0 + u * THREADS) * K - off;
-                    if (e0 < V) f(raw[u], (int)e0);
-                }
-            }
-        };
-        Run run;
-        pieces([&](const uint4& raw, int e0) {
-            alignas(16) T v[K];
-            *(uint4*)v = raw;
-            if (y >= e0 && y < e0 + K) {                     // the target's logit, and -inf in its place
-#pragma unroll
-                for (int q = 0; q < K; q++)
-                    if (q == y - e0) { meet.xt[turn] = f32(v[q]); v[q] = lowest<T>(); }
-            }
-            const uint4 others = *(const uint4*)v;
-            const float m = piece_max<T>(others);
-            if (m > run.m + HEADROOM) { run.o *= rescale(run.m, m); run.m = m; run.c = ref_of(m); }
-            add<T, true>(run, others);
-        });
-        const bool grad = d;
-        const float4 g = block_end<MODE, THREADS / 32, 1>(k, meet, turn, run, end, w, scale, r, grad, 0);
-        turn ^= 1;
-        if (grad) {
-            const bool same = alike(x, d);
-            pieces([&](const uint4& raw, int e0) {
-                grad_piece(raw, d, e0, V, same, g);
-                if (y >= e0 && y < e0 + K) d[y] = from32<T>(g.w);
-            });
-        }
-    }
 }
 
 // ---------------------------------------------------------------- small kernels around the rows
@@ -1012,12 +1202,16 @@ const char* bad_batch(const pv_scored* b) {
 }
 
 // How a batch is run, by its rows' 16-byte pieces (one more than their bytes say where a row may start inside one):
-// up to 256 in registers, G lanes a row; more through a ring in shared memory, where the policy loss needs a row to fit it
-// (RING_MOST; longer ones it reads twice).
-enum { SHORT_ROWS, RING_ROWS, LONG_ROWS };
+// up to 256 in registers, G lanes a row; more through a ring in shared memory. Where the policy loss is to give a gradient
+// a row has to fit the ring (RING_MOST); longer ones it reads twice, the second time with their statistics at hand (131,072
+// bf16 words a row, 2,048 rows: 295 us, and 342 us by clusters of four blocks that hold a row; 65,541: 1,115 us and 890).
+// Rows of up to 136 words (32 bits) that do not start at 16-byte boundaries, but lie one behind the other, are copied as
+// stretches (262,144 rows of 259 bf16 words: log-probabilities in 55 us that way and in 73 us with 16 lanes a row and the
+// ends by themselves; longer ones fill more lanes, 131,072 rows of 1,003: 87 us with 32 lanes a row).
+enum { FLAT_ROWS, SHORT_ROWS, RING_ROWS, LONG_ROWS };
 constexpr int RING = 18;                                 // pieces a thread
 struct Plan { int form, pieces; bool aligned; int64_t tpw, tiles, spans; };
-constexpr int RING_MOST = 2048 * RING;
+constexpr int RING_MOST = 512 * RING;                    // two blocks of 256 threads
 int size_of(int type) { return type == PV_T_FP32 ? 4 : 2; }
 // every row starts at a 16-byte boundary
 bool whole_pieces(const void* p, int64_t n, int64_t w, int64_t size) {
@@ -1029,24 +1223,32 @@ Plan plan_of(const pv_scored& b) {
     p.aligned = whole_pieces(b.logits, b.logits_n, b.logits_w, size);
     const int64_t pieces = (b.V + k - 1 + (p.aligned ? 0 : k - 1)) / k;
     p.pieces = (int)std::min<int64_t>(pieces, 1 << 30);
-    p.form = pieces <= 256 ? SHORT_ROWS : pieces <= RING_MOST ? RING_ROWS : LONG_ROWS;
-    p.tpw = p.form == SHORT_ROWS ? (b.W + TILE - 1) / TILE : b.W;
+    const int64_t words = b.type == PV_T_FP32 ? b.V : b.V / 2 + 1;
+    const bool whole = p.aligned && b.V % k == 0;
+    const bool flat = !whole && words <= 136 && b.logits_w == b.V &&
+                      (!b.grad || (b.grad_w == b.V && (((uintptr_t)b.logits ^ (uintptr_t)b.grad) & 15) == 0 && ((b.logits_n - b.grad_n) * size & 15) == 0));
+    p.form = flat ? FLAT_ROWS : pieces <= 256 ? SHORT_ROWS : pieces <= RING_MOST ? RING_ROWS : LONG_ROWS;
+    p.tpw = p.form <= SHORT_ROWS ? (b.W + TILE - 1) / TILE : b.W;
     p.tiles = b.n * p.tpw;
     p.spans = (b.W + COUNT_SPAN - 1) / COUNT_SPAN;
     return p;
 }
-// scratch: a double per tile, a double per window, an int per (window, span)
-struct Scratch { double *part, *win; int32_t* counts; size_t bytes; };
+// scratch: a double per tile, a double per window, an int per (window, span); the policy loss of long rows: their statistics
+// and derivatives
+struct Scratch { double *part, *win; float4* stat; float* deriv; int32_t* counts; size_t bytes; };
 Scratch scratch_of(const pv_scored& b, const Plan& p, void* work) {
     Scratch s;
-    const size_t a = (size_t)p.tiles * 8, w = (size_t)b.n * 8, c = ((size_t)b.n * p.spans * 4 + 15) / 16 * 16;
-    s.part = (double*)work;
-    s.win = (double*)((char*)work + a);
-    s.counts = (int32_t*)((char*)work + a + w);
-    s.bytes = a + w + c;
+    char* at = (char*)work;
+    s.bytes = 0;
+    const auto take = [&](size_t n) { char* r = at + s.bytes; s.bytes += (n + 15) / 16 * 16; return r; };
+    s.part = (double*)take((size_t)p.tiles * 8);
+    s.win = (double*)take((size_t)b.n * 8);
+    s.counts = (int32_t*)take((size_t)b.n * p.spans * 4);
+    const size_t rows = p.form == LONG_ROWS ? (size_t)b.n * b.W : 0;
+    s.stat = (float4*)take(rows * 16);
+    s.deriv = (float*)take(rows * 4);
     return s;
 }
-
 // a persistent grid: as many blocks as are resident, at most one per `per_block` of the work
 template <typename F>
 unsigned grid_of(F* f, int threads, size_t smem, int64_t blocks) {
@@ -1067,7 +1269,7 @@ int allow_smem(const void* f, int bytes, uint64_t& set) {
 
 template <typename T, int G, int NV, int MODE, bool A>
 void group_rows(const Rows& k, cudaStream_t st) {
-    constexpr int S = NV <= 4 ? 4 : 3, SMEM = WARPS * S * NV * 512;
+    constexpr int S = NV <= 4 ? 3 : 2, SMEM = WARPS * S * NV * 512;
     const auto f = rows_group_kernel<T, G, NV, S, MODE, A>;
     static thread_local uint64_t set = 0;
     allow_smem((const void*)f, SMEM, set);
@@ -1097,39 +1299,55 @@ void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
     cudaLaunchKernelEx(&cfg, f, k, steps);
 }
 
-template <typename T, int MODE, bool A>
-void group_rows_of(const Rows& k, const Plan& p, cudaStream_t st) {
-    if (p.pieces <= 1) group_rows<T, 1, 1, MODE, A>(k, st);
-    else if (p.pieces <= 2) group_rows<T, 1, 2, MODE, A>(k, st);
-    else if (p.pieces <= 4) group_rows<T, 1, 4, MODE, A>(k, st);
-    else if (p.pieces <= 8) group_rows<T, 2, 4, MODE, A>(k, st);
-    else if (p.pieces <= 16) group_rows<T, 4, 4, MODE, A>(k, st);
-    else if (p.pieces <= 32) group_rows<T, 8, 4, MODE, A>(k, st);
-    else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, A>(k, st);
-    else if (p.pieces <= 128) group_rows<T, 32, 4, MODE, A>(k, st);
-    else group_rows<T, 32, 8, MODE, A>(k, st);
+template <typename T, int G, int NW, int MODE>
+void flat_rows(const Rows& k, cudaStream_t st) {
+    constexpr int S = 3, SMEM = WARPS * S * ((NW * 32 * 4 + 47) / 16) * 16;
+    const auto f = rows_flat_kernel<T, G, NW, S, MODE>;
+    static thread_local uint64_t set = 0;
+    allow_smem((const void*)f, SMEM, set);
+    static const unsigned most = grid_of(f, WARPS * 32, SMEM, 1 << 20);
+    f<<<(unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most), WARPS * 32, SMEM, st>>>(k);
+}
+
+template <typename T, int MODE>
+void short_rows(const Rows& k, const Plan& p, cudaStream_t st) {
+    const bool whole = p.aligned && k.b.V % K_OF<T> == 0 && (!k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T)));
+    if (p.form == FLAT_ROWS) {
+        const int words = sizeof(T) == 4 ? (int)k.b.V : (int)k.b.V / 2 + 1;
+        if (words <= 4) flat_rows<T, 1, 4, MODE>(k, st);
+        else if (words <= 8) flat_rows<T, 1, 8, MODE>(k, st);
+        else if (words <= 17) flat_rows<T, 1, 17, MODE>(k, st);
+        else if (words <= 34) flat_rows<T, 2, 17, MODE>(k, st);
+        else if (words <= 68) flat_rows<T, 4, 17, MODE>(k, st);
+        else flat_rows<T, 8, 17, MODE>(k, st);
+    } else if (!whole) {
+        if (p.pieces <= 16) group_rows<T, 16, 1, MODE, false>(k, st);
+        else if (p.pieces <= 32) group_rows<T, 16, 2, MODE, false>(k, st);
+        else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, false>(k, st);
+        else if (p.pieces <= 128) group_rows<T, 32, 4, MODE, false>(k, st);
+        else group_rows<T, 32, 8, MODE, false>(k, st);
+    } else if (p.pieces <= 1) group_rows<T, 1, 1, MODE, true>(k, st);
+    else if (p.pieces <= 2) group_rows<T, 1, 2, MODE, true>(k, st);
+    else if (p.pieces <= 4) group_rows<T, 1, 4, MODE, true>(k, st);
+    else if (p.pieces <= 8) group_rows<T, 2, 4, MODE, true>(k, st);
+    else if (p.pieces <= 16) group_rows<T, 4, 4, MODE, true>(k, st);
+    else if (p.pieces <= 32) group_rows<T, 8, 4, MODE, true>(k, st);
+    else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, true>(k, st);
+    else if (p.pieces <= 128) group_rows<T, 32, 4, MODE, true>(k, st);
+    else group_rows<T, 32, 8, MODE, true>(k, st);
 }
 
 template <typename T, int MODE>
 void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
-    if (p.form == SHORT_ROWS) {
-        if constexpr (MODE != GIVEN) {
-            if (p.aligned && k.b.V % K_OF<T> == 0 && (MODE == LOGP || !k.b.grad || whole_pieces(k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T))))
-                group_rows_of<T, MODE, true>(k, p, st);
-            else
-                group_rows_of<T, MODE, false>(k, p, st);
-        }
-    } else if constexpr (MODE == POLICY) {
-        if (p.pieces <= 32 * RING) ring_rows<T, 32, 4, 5, 1, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 64 * RING) ring_rows<T, 64, 3, 6, 1, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 128 * 16) ring_rows<T, 128, 4, 4, 1, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 256 * RING) ring_rows<T, 256, 3, 6, 1, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 512 * RING) ring_rows<T, 256, 3, 6, 2, MODE>(k, p.pieces, st);
-        else if (p.pieces <= 1024 * RING) ring_rows<T, 256, 3, 6, 4, MODE>(k, p.pieces, st);
-        else if (p.form == RING_ROWS) ring_rows<T, 256, 3, 6, 8, MODE>(k, p.pieces, st);
-        else {
-            static const unsigned most = grid_of(rows_long_kernel<T>, 512, 0, 1 << 20);
-            rows_long_kernel<T><<<(unsigned)std::min<int64_t>(k.b.n * k.b.W, most), 512, 0, st>>>(k);
+    if (p.form <= SHORT_ROWS) {
+        if constexpr (MODE != GIVEN) short_rows<T, MODE>(k, p, st);
+    } else if (MODE == POLICY && k.b.grad) {
+        if constexpr (MODE == POLICY) {
+            if (p.pieces <= 32 * RING) ring_rows<T, 32, 4, 5, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 64 * RING) ring_rows<T, 64, 3, 6, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 128 * 16) ring_rows<T, 128, 4, 4, 1, MODE>(k, p.pieces, st);
+            else if (p.pieces <= 256 * RING) ring_rows<T, 256, 3, 6, 1, MODE>(k, p.pieces, st);
+            else ring_rows<T, 256, 3, 6, 2, MODE>(k, p.pieces, st);
         }
     } else if constexpr (MODE != GRAD) {
         // read once, a row need not fit the ring: a warp a row where the rows fill the GPU with 16 warps a multiprocessor,
@@ -1177,6 +1395,25 @@ int bad_policy(const pv_scored* b, const pv_policy_args* a) {
     return PV_OK;
 }
 
+int policy_rows(const pv_scored* b, const pv_policy_args* a, const Plan& p, const Scratch& s, double* part, const double* weight, const float* scale,
+                       int skip_one, cudaStream_t st) {
+    Rows k = rows_of(*b, p);
+    k.part = part;
+    k.a = *a;
+    k.weight = weight;
+    k.scale = scale; k.skip_one = scale && skip_one;
+    if (!b->grad || p.form != LONG_ROWS) return launch_rows<POLICY>(k, p, st);
+    k.b.grad = nullptr;
+    k.stat = s.stat;
+    k.deriv = s.deriv;
+    if (const int e = launch_rows<POLICY>(k, p, st)) return e;
+    Rows q = rows_of(*b, p);
+    q.stat = s.stat;
+    q.up = s.deriv; q.up_n = b->W; q.up_w = 1;
+    q.scale = scale; q.skip_one = k.skip_one; q.scaled = 1;
+    return launch_rows<GIVEN>(q, p, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1187,7 +1424,7 @@ size_t pv_score_work_bytes(const pv_scored* b) {
 }
 
 size_t pv_score_stat_bytes(const pv_scored* b) {
-    if (bad_batch(b) || plan_of(*b).form == SHORT_ROWS) return 0;
+    if (bad_batch(b) || plan_of(*b).form <= SHORT_ROWS) return 0;
     return (size_t)b->n * b->W * sizeof(float4);
 }
 
@@ -1212,12 +1449,12 @@ int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t 
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !up) return fail(PV_EARG, "pv_logprobs_grad: NULL gradient");
     const Plan p = plan_of(*b);
-    if (p.form != SHORT_ROWS && (!stat || ((uintptr_t)stat & 15))) return fail(PV_EARG, "pv_logprobs_grad: rows of this length need their statistics");
+    if (p.form > SHORT_ROWS && (!stat || ((uintptr_t)stat & 15))) return fail(PV_EARG, "pv_logprobs_grad: rows of this length need their statistics");
     Rows k = rows_of(*b, p);
     k.up = up; k.up_n = up_n; k.up_w = up_w;
     k.stat = (float4*)stat;
     k.scale = scale;
-    return p.form == SHORT_ROWS ? launch_rows<GRAD>(k, p, (cudaStream_t)stream) : launch_rows<GIVEN>(k, p, (cudaStream_t)stream);
+    return p.form <= SHORT_ROWS ? launch_rows<GRAD>(k, p, (cudaStream_t)stream) : launch_rows<GIVEN>(k, p, (cudaStream_t)stream);
 }
 
 int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float beta, float smoothing, float* loss, float* margins, float* coef,
@@ -1261,27 +1498,22 @@ int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* 
         if (!one) count_kernel<<<(unsigned)std::min<int64_t>(b->n * p.spans, SMS * 8), 256, 0, st>>>(*b, p.spans, s.counts);
         weights_kernel<<<1, 1024, 0, st>>>(*b, one ? nullptr : s.counts, p.spans, a->by_window, (double)a->scale, weight);
         if (const int e = launched()) return e;
-        Rows k = rows_of(*b, p);
-        k.part = s.part;
-        k.a = *a;
-        k.weight = weight;
-        if (const int e = launch_rows<POLICY>(k, p, st)) return e;
+        if (const int e = policy_rows(b, a, p, s, s.part, weight, nullptr, 0, st)) return e;
     }
     total_kernel<<<1, 1024, 0, st>>>(s.part, p.tiles, loss);
     return launched();
 }
 
-int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* weight, const float* scale, int skip_one, void* stream) {
+int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* weight, const float* scale, int skip_one, void* work, size_t work_bytes,
+                   void* stream) {
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (const int e = bad_policy(b, a)) return e;
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !weight || !a->old || !a->adv) return fail(PV_EARG, "pv_policy_grad: NULL argument");
     const Plan p = plan_of(*b);
-    Rows k = rows_of(*b, p);
-    k.a = *a;
-    k.weight = weight;
-    k.scale = scale; k.skip_one = scale && skip_one;
-    return launch_rows<POLICY>(k, p, (cudaStream_t)stream);
+    const Scratch s = scratch_of(*b, p, work);
+    if (p.form == LONG_ROWS && check_work(s, work, work_bytes)) return PV_EARG;
+    return policy_rows(b, a, p, s, nullptr, weight, scale, skip_one, (cudaStream_t)stream);
 }
 
 }  // extern "C"

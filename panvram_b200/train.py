@@ -242,13 +242,14 @@ def _policy_args(b, old, adv, ref, clip, kl, by_window, scale, dev):
 
 
 def _policy(b, dev, a):
-    """-> (loss, a buffer that starts with the windows' weights); b's gradient too, if it names one"""
+    """-> (loss, (a buffer that starts with the windows' weights, its scratch's address and bytes)); b's gradient too, if it
+    names one"""
     with _on(dev):
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        weight, work, need = _work(b, dev, 8 * b.n)
-        if _C._lib.pv_policy(ctypes.byref(b), ctypes.byref(a), loss.data_ptr(), weight.data_ptr(), work, need, _stream(dev)):
+        buf, work, need = _work(b, dev, 8 * b.n)
+        if _C._lib.pv_policy(ctypes.byref(b), ctypes.byref(a), loss.data_ptr(), buf.data_ptr(), work, need, _stream(dev)):
             raise _failed("policy loss")
-    return loss, weight
+    return loss, (buf, work, need)
 
 
 class _Policy(torch.autograd.Function):
@@ -262,7 +263,7 @@ class _Policy(torch.autograd.Function):
         ctx.b, ctx.a, ctx.grad = b, a, None
         if logits.dtype != torch.float16:
             b, ctx.grad = _with_grad(b, logits)
-        loss, ctx.weight = _policy(b, logits.device, a)
+        loss, ctx.work = _policy(b, logits.device, a)
         return loss
 
     @staticmethod
@@ -272,7 +273,9 @@ class _Policy(torch.autograd.Function):
         made, ctx.grad = ctx.grad, None
         with _on(logits.device):
             b, g = _with_grad(ctx.b, logits, made)
-            if _C._lib.pv_policy_grad(ctypes.byref(b), ctypes.byref(ctx.a), ctx.weight.data_ptr(), up.data_ptr(), made is not None,
+            # the loss's scratch again: it is done with, and long rows need some
+            buf, work, need = ctx.work
+            if _C._lib.pv_policy_grad(ctypes.byref(b), ctypes.byref(ctx.a), buf.data_ptr(), up.data_ptr(), made is not None, work, need,
                                       _stream(logits.device)):
                 raise _failed("policy loss's gradient")
         return g, None, None, None, None, None
@@ -319,7 +322,9 @@ def _tensors(ts, name):
     """-> (pv_tensors, the arrays it points to, the tensors as a list, their types, whether all are contiguous)"""
     ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
     try:
-        types = array("B", [_TYPES[t.dtype] for t in ts])
+        types = [t.dtype for t in ts]
+        same = bool(ts) and types.count(types[0]) == len(ts)
+        types = array("B", [_TYPES[types[0]]]) * len(ts) if same else array("B", [_TYPES[t] for t in types])
     except (KeyError, AttributeError):
         raise ValueError(f"{name}: bf16, fp16 or fp32 tensors") from None
     plain = all([t.is_contiguous() for t in ts])
@@ -353,8 +358,8 @@ def grad_norm(grads):
 
 def clip_grads(grads, max_norm, out=None):
     """Scale the gradients by min(1, max_norm / (norm + 1e-6)) -> their norm before it (grad_norm), no wait for the device.
-    In place; or into `out`, one tensor per gradient of its shape and strides, of its type or float32 (an optimizer's
-    full-precision gradients), then always written. A tensor that is written may not share memory with another. A norm of
+    In place; or into `out`, one tensor per gradient, of its type or float32 (an optimizer's full-precision gradients) and as
+    many elements, contiguous as it is (else of its shape and strides); then always written. A tensor that is written may not share memory with another. A norm of
     infinity scales finite elements to 0, NaN makes every element NaN, as the formula says."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
@@ -363,9 +368,13 @@ def clip_grads(grads, max_norm, out=None):
     o, written = None, ts
     if out is not None:
         o, okept, written, otypes, oplain = _tensors(out, "out")
-        if [t.shape for t in ts] != [t.shape for t in written] or not (plain and oplain) and any(a.stride() != b.stride() for a, b in zip(ts, written)):
-            raise ValueError("out: one tensor per gradient, of its shape and strides")
-        if any([b != 2 and a != b for a, b in zip(types, otypes)]):
+        if plain and oplain:
+            alike = kept[1] == okept[1]
+        else:
+            alike = len(ts) == len(written) and all(a.shape == b.shape and a.stride() == b.stride() for a, b in zip(ts, written))
+        if not alike:
+            raise ValueError("out: one tensor per gradient, of its size and laid out alike")
+        if types != otypes and any([b != 2 and a != b for a, b in zip(types, otypes)]):
             raise ValueError("out: of the gradient's type, or float32")
         if written[0].device != ts[0].device:
             raise ValueError("out: on the gradients' device")

@@ -345,8 +345,8 @@ def test_policy(P, cuda, n, W, V, shift, kind):
         assert torch.equal(again, d)
         half = P.policy_loss(x, t, old, adv, ref, clip, kl, m, shift, reduce=reduce, scale=0.5)           # exact in every step
         assert torch.equal(half, 0.5 * got) and (kind == "fp16" or torch.equal(torch.autograd.grad(half, x)[0], 0.5 * d))
-        with torch.no_grad():
-            assert torch.equal(P.policy_loss(x, t, old, adv, ref, clip, kl, m, shift, reduce=reduce), got)
+        with torch.no_grad():                                # without a gradient rows may be split otherwise: another order of the same sums
+            close(P.policy_loss(x, t, old, adv, ref, clip, kl, m, shift, reduce=reduce), loss, l_err + 2 * E32 * loss.abs() + 1e-12, "no gradient")
 
 
 def test_policy_does_not_read_what_is_not_counted(P, cuda):

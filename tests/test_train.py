@@ -114,7 +114,7 @@ def test_entry_points_refuse_a_bad_batch(kw):
     assert lib.pv_logprobs_grad(b, 64, 0, 0, None, None, None) == _C.PV_EARG
     assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, None, 64, 1 << 40, None) == _C.PV_EARG
     assert lib.pv_policy(b, ctypes.byref(a), 64, 64, 64, 1 << 40, None) == _C.PV_EARG
-    assert lib.pv_policy_grad(b, ctypes.byref(a), 64, None, 0, None) == _C.PV_EARG
+    assert lib.pv_policy_grad(b, ctypes.byref(a), 64, None, 0, None, 0, None) == _C.PV_EARG
 
 
 def test_entry_points_refuse_missing_arguments():
@@ -132,7 +132,8 @@ def test_entry_points_refuse_missing_arguments():
     assert lib.pv_preference(b, 64, 1, 0.1, 0.0, 64, None, 64, None, 64, 1, None) == _C.PV_EARG and "scratch" in _message()
     for kw in ({"old": None}, {"adv": None}, {"clip_low": -1.0}, {"clip_high": float("nan")}, {"kl": 0.1}, {"scale": -1.0}):
         assert lib.pv_policy(b, ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, 64, 64, 1 << 30, None) == _C.PV_EARG
-        assert lib.pv_policy_grad(_scored(grad=64), ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, None, 0, None) == _C.PV_EARG
+        assert lib.pv_policy_grad(_scored(grad=64), ctypes.byref(_C.PolicyArgs(**{**good, **kw})), 64, None, 0, None, 0, None) == _C.PV_EARG
+    assert lib.pv_policy_grad(long, ctypes.byref(_C.PolicyArgs(**good)), 64, None, 0, None, 0, None) == _C.PV_EARG and "scratch" in _message()
     assert lib.pv_policy(b, None, 64, 64, 64, 1 << 30, None) == _C.PV_EARG
     assert lib.pv_policy(b, ctypes.byref(_C.PolicyArgs(**good)), 64, 64, 64, 8, None) == _C.PV_EARG
 
