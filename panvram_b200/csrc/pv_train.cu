@@ -770,6 +770,10 @@ struct Meeting {
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
     }
 };
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Ends a counted row: the threads' sums join, a first warp takes them to the row's log-probability, term and derivative.
 template <int MODE, int NW, int C>
 __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, int turn, Run& run, const End& end, double w, float scale, int64_t r,
@@ -787,7 +791,7 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
             at.put(to, lane, run.m);
             at.put(to + 1, lane, run.o);
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_barrier();
     }
     if (warp == 0) {
         Run all = run;
@@ -856,7 +860,7 @@ __device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V
 //
 // C: blocks of a cluster that share a row, each a span of its pieces; they leave each other what their warps found in
 // distributed shared memory, behind one cluster barrier a row.
-//
+
 // warps that a multiprocessor holds with P pieces a thread in the ring, 32 at most (64 registers a thread)
 template <int P> constexpr int RING_WARPS = 220 * 1024 / (P * 512) < 32 ? 220 * 1024 / (P * 512) : 32;
 template <typename T, int THREADS, int U, int S, int C, int MODE>
@@ -924,6 +928,7 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
     };
 #pragma unroll 1
     for (int s = 0; s < S; s++) copy_next();
+    if (C > 1) cluster_barrier();                            // every block of the cluster runs before one writes to another
 
     int slot = 0, turn = 0;
     for (int64_t first = first_row; first < rows; first += 32 * stride) {

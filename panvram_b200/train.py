@@ -13,7 +13,7 @@ What lies at other positions, NaN and infinities included, is not read into any 
 
 Kernels run on torch's current stream of the logits' (gradients') device, without a wait; scratch comes from torch's
 allocator on that stream. Logits are bf16, fp16 or fp32 [n, W, V] with any strides between windows and positions; their
-gradient has their type. Arguments other than the logits are constants. A loss keeps the logits, tokens and mask for its
+gradient has their type, and no second derivative. Arguments other than the logits are constants. A loss keeps the logits, tokens and mask for its
 backward pass: with Cohort.sampler, run it before the sampler's next call overwrites its windows."""
 import ctypes
 import math
@@ -116,10 +116,27 @@ def _with_grad(b, logits, g=None):
     return b, g
 
 
+class _NoSecond(torch.autograd.Function):
+    """a gradient that may be used, but not differentiated by the logits"""
+
+    @staticmethod
+    def forward(ctx, g, logits):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, up):
+        raise RuntimeError("panvram_b200: no second derivative")
+
+
 def _once(backward):
-    """no second derivative: refused where one is asked for (torch's own wrapper, entered only where a graph is being made)"""
-    refusing = torch.autograd.function.once_differentiable(backward)
-    return lambda ctx, up: refusing(ctx, up) if torch.is_grad_enabled() else backward(ctx, up)
+    """a backward pass whose gradient refuses a second one (which only a pass that makes a graph could ask for)"""
+    def run(ctx, up):
+        if not torch.is_grad_enabled():
+            return backward(ctx, up)
+        with torch.no_grad():
+            out = backward(ctx, up)
+        return (_NoSecond.apply(out[0], ctx.saved_tensors[0]),) + out[1:]
+    return run
 
 
 def _wants_grad(logits):

@@ -393,6 +393,98 @@ def test_empty(P, cuda, n, W):
     assert P.window_logprobs(x, t, reduce="window").tolist() == [0.0] * n
 
 
+def test_offsets_beyond_32_bits(P, cuda):
+    """windows and positions that lie more than 2^32 elements apart"""
+    for V, far_w in ((40, False), (41, True), (3000, False), (70001, False)):
+        n, W = 2, 3
+        buf = torch.empty(2 * 2_200_000_001 + 3 * V, dtype=torch.bfloat16, device=cuda)
+        sn, sw = (2 * 2_200_000_001, V) if not far_w else (V, 2_200_000_001)
+        x = buf.as_strided((n, W, V), (sn, sw, 1))
+        x.copy_(torch.randn(n, W, V, device=cuda))
+        t = torch.randint(0, V, (n, W), device=cuda)
+        lp, p, y, ok = oracle(x, t, None, 0)
+        a = x.detach().requires_grad_(True)
+        got = P.window_logprobs(a, t, shift=0)
+        close(got, lp.detach(), tol_lp(V, lp.detach()))
+        close(torch.autograd.grad(got.sum(), a)[0], *grad_of(x, p, y, ok, torch.ones(n, W, device=cuda).double()))
+        old, adv = lp.detach().float() + 0.01, torch.ones(n, device=cuda)
+        d = torch.autograd.grad(P.policy_loss(a, t, old, adv, shift=0), a)[0]
+        r = (lp.detach() - old.double()).exp()
+        el = tol_lp(V, lp.detach()) + E32 * 2 * old.abs()
+        close(d, *grad_of(x, p, y, ok, -r / 6, r / 6 * (el + 4 * E32)))
+
+
+@pytest.mark.parametrize("n, W, V", [(20, 8000, 2057), (2, 4000, 40001), (3, 1 << 19, 5), (40, 8192, 24)])
+def test_more_rows_than_the_blocks_look_up_at_once(P, cuda, n, W, V):
+    """every row of a batch that keeps each block busy for many rows, a stretch of them not counted"""
+    x, t, m = make(cuda, n, W, V, "bf16", "ids", "bool", seed=1)
+    m[1, W // 3:2 * W // 3] = False
+    up = torch.randn(n, W, device=cuda, generator=torch.Generator(device=cuda).manual_seed(2))
+    a = x.requires_grad_(True)
+    got = P.window_logprobs(a, t, m)
+    (d,) = torch.autograd.grad(got, a, up)
+    x = x.detach()
+    old = torch.empty_like(up)
+    lps = []
+    for i in range(n):
+        lp, p, y, ok = oracle(x[i:i + 1], t[i:i + 1], m[i:i + 1], 1)
+        close(got[i:i + 1], lp.detach(), tol_lp(V, lp.detach()), i)
+        close(d[i:i + 1], *grad_of(x[i:i + 1], p, y, ok, up[i:i + 1].double()), i)
+        old[i] = lp.detach()[0].float() + 0.01
+        lps.append((lp.detach(), ok))
+    del d
+    count = sum(int(ok.sum()) for _, ok in lps)
+    loss = P.policy_loss(a, t, old, up[:, 0], mask=m)
+    (d,) = torch.autograd.grad(loss, a)
+    total, err = 0.0, 0.0
+    for i in range(n):
+        lp, ok = lps[i]
+        _, p, y, _ = oracle(x[i:i + 1], t[i:i + 1], m[i:i + 1], 1)
+        r = torch.where(ok, (lp - old[i:i + 1].double()).exp() * up[i, 0].double(), 0.0)
+        el = tol_lp(V, lp) + 2 * E32 * old[i:i + 1].abs()
+        close(d[i:i + 1], *grad_of(x[i:i + 1], p, y, ok, -r / count, r.abs() / count * (el + 4 * E32)), i)
+        total -= float(r.sum())
+        err += float((r.abs() * (el + 4 * E32)).sum())
+    assert abs(float(loss) - total / count) <= err / count + 2 * E32 * abs(total / count)
+
+
+def test_shapes_at_random(P, cuda):
+    import random
+    rng = random.Random(7)
+    for _ in range(60):
+        V = int(round(math.exp(rng.uniform(0, math.log(40000)))))
+        W = rng.randint(1, max(2, min(400, 600000 // V)))
+        n = 2 * rng.randint(1, 3)
+        kind, shift = rng.choice(list(TYPES)), rng.choice((0, 1, 2))
+        tokens, mask, pad = rng.choice(("ids", "bases")), rng.choice((None, "bool", "uint8", "float")), rng.choice((0, 0, 0, 1, 5, 8))
+        x, t, m = make(cuda, n, W, V, kind, tokens, mask, shift, seed=rng.randint(0, 1 << 20), pad=pad)
+        what = (n, W, V, kind, shift, tokens, mask, pad)
+        lp, p, y, ok = oracle(x, t, m, shift)
+        a = x.detach().requires_grad_(True)
+        got = P.window_logprobs(a, t, m, shift)
+        close(got, lp.detach(), tol_lp(V, lp.detach()), what)
+        up = torch.randn(n, W, device=cuda)
+        close(torch.autograd.grad(got, a, up)[0], *grad_of(x, p, y, ok, up.double()), what)
+        old, ref, adv = policy_inputs(lp, (0.2, 0.2), cuda, V)
+        reduce = rng.choice(("token", "window"))
+        loss, g, p, y, ok, l_err, g_err = policy_oracle(x, t, m, old, adv, ref, (0.2, 0.2), 0.1, reduce, shift)
+        got = P.policy_loss(a, t, old, adv, ref, 0.2, 0.1, m, shift, reduce=reduce)
+        close(got, loss, l_err + 2 * E32 * loss.abs() + 1e-12, what)
+        close(torch.autograd.grad(got, a)[0], *grad_of(x, p, y, ok, g, g_err), what)
+
+
+def test_second_derivatives_are_refused(P, cuda):
+    x, t, _ = make(cuda, 2, 8, 16, "fp32", "ids")
+    x.requires_grad_(True)
+    f = torch.zeros(2, 8, device=cuda)
+    for loss in (P.window_logprobs(x, t).sum(), P.preference_loss(x, t, f[:, 0]), P.policy_loss(x, t, f, f)):
+        (want,) = torch.autograd.grad(loss, x, retain_graph=True)
+        (d,) = torch.autograd.grad(loss, x, create_graph=True)
+        assert torch.equal(d, want)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad((d * d).sum(), x)
+
+
 def test_gradients_against_differences(P, cuda):
     """the kernels' gradients along a direction, against central differences of the 64-bit losses: h^2 times the third
     derivative (below 10 here) and the gradients' own rounding"""
