@@ -86,6 +86,11 @@ __device__ __forceinline__ float exponent(float x, float m, float c) { return fa
 // what a sum of numerators with the maximum m is multiplied by, to be one with the maximum M >= m
 __device__ __forceinline__ float rescale(float m, float M) { return ex2(far(m) || far(M) ? (m - M) * LOG2E : ref_of(m) - ref_of(M)); }
 
+__device__ __forceinline__ float reciprocal(float v) {          // of sums of numerators: about 1 or more, so nothing is flushed
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -135,15 +140,19 @@ __device__ __forceinline__ void times(float (&x)[K], float f) {
 // outweigh the others the sum is about 1 or more, and log1p of what it is above 1 is its logarithm.
 __device__ __forceinline__ float row_logp(float m, float o, float t, float e) {
     const bool sure = e >= o;
-    const float l = log1pf(sure ? o / e : (o + e) - 1.f);
+    const float l = log1pf(sure ? o * reciprocal(e) : (o + e) - 1.f);
     return m == -INFINITY ? NAN : (sure ? 0.f : t * LN2) - l;            // -inf: nothing to normalise by
 }
 
-// exp(d) - d - 1: by its series near 0, where the difference would lose its digits
-__device__ __forceinline__ float kl_term(float d, float em1) {
-    if (fabsf(d) < 0.25f)
-        return d * d * (0.5f + d * (1.f / 6 + d * (1.f / 24 + d * (1.f / 120 + d * (1.f / 720 + d * (1.f / 5040 + d * (1.f / 40320)))))));
-    return em1 - d;
+// exp(d) - 1 and exp(d) - d - 1, near 0 by the series of the latter, where the differences would lose their digits
+__device__ __forceinline__ void kl_terms(float d, float& em1, float& kl) {
+    if (fabsf(d) < 0.25f) {
+        kl = d * d * (0.5f + d * (1.f / 6 + d * (1.f / 24 + d * (1.f / 120 + d * (1.f / 720 + d * (1.f / 5040 + d * (1.f / 40320)))))));
+        em1 = d + kl;
+    } else {
+        em1 = expf(d) - 1.f;
+        kl = em1 - d;
+    }
 }
 
 // What a counted row's end reads, loaded before its logits are waited for.
@@ -173,8 +182,9 @@ __device__ __forceinline__ float row_end(const Rows& k, const End& e, float lp, 
     float g = free ? -one : 0.f;
     term = free ? -one : -two;
     if (k.a.ref) {
-        const float d = e.ref - lp, em1 = expm1f(d);
-        term += k.a.kl * kl_term(d, em1);
+        float em1, kl;
+        kl_terms(e.ref - lp, em1, kl);
+        term += k.a.kl * kl;
         g -= k.a.kl * em1;
     }
     return g * w * scale;
@@ -311,8 +321,9 @@ struct Pos {
     }
 };
 
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {                   // to: an address in shared memory
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -353,6 +364,12 @@ __device__ __noinline__ float sum_far(const uint4* raw, int step, float by, floa
 // copy follows S - 1 groups behind its use. The targets of the tile being copied are loaded a tile ahead of it, those and the
 // arguments of the tile being worked on a tile ahead of that, so neither is waited for. The target's logit is read out of
 // the ring and -inf put in its place: the sum of the others and their maximum follow without a comparison an element.
+//
+// On a B200, 524,288 rows of 128 bf16 words: log-probabilities 35 us (3.8 TB/s), policy loss and gradient 56 us (4.8 TB/s
+// read and written). Bound by instructions: a step has about 250 of its own (targets, addresses, shuffles, the row's end)
+// beside 4 a word, so 32 words a lane is little; 64 words, half the lanes, lose more by the warps that no longer fit (1,048,576
+// rows: 146 us, and 112 us with 32). Three blocks a multiprocessor for log-probabilities (64 us, two 69), two where the
+// numerators are kept for the gradient (112 us, three spill: 153).
 constexpr int TILE = 32, WARPS = 8;
 
 // A: rows of whole pieces, logits' and gradient's alike. Else (G 16 or more) the elements before a row's first whole piece and
@@ -366,6 +383,7 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     uint4* const ring = rings + (threadIdx.x >> 5) * (S * NV * 32);
+    const uint32_t ring_at = shared_at(ring + lane);
     // pieces beyond a row's end are never copied: -inf from here on
 #pragma unroll
     for (int s = 0; s < S * NV; s++) ring[s * 32 + lane] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
@@ -391,10 +409,10 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
             const int y = __shfl_sync(~0u, in_y, in_s * RP + grp);
             if (y >= 0) {
                 const int head = A ? 0 : head_of(in_x, V), n = (V - head) / K;
-                uint4* const to = ring + in_slot * (NV * 32) + lane;
+                const uint32_t to = ring_at + in_slot * (NV * 512);
 #pragma unroll
                 for (int j = 0; j < NV; j++)
-                    if (sub + j * G < n) copy16(to + j * 32, in_x + head + (sub + j * G) * K);
+                    if (sub + j * G < n) copy16(to + j * 512, in_x + head + (sub + j * G) * K);
             }
             in_x += x_step;
             if (++in_s == G) {
@@ -425,6 +443,7 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
         const End end_next = end_of(p, y_next);
         const int rows = (int)min((int64_t)TILE, W - t0);
         const double w = weight_of<MODE>(k, i);
+        const float wf = (float)w;
         double sum = 0;
         // LOGP: the row of this lane's number in the tile, its maximum, others' sum, target's exponent and numerator
         float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
@@ -443,11 +462,11 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
             copies_wait<S - 1>();
             __syncwarp();
             const bool in_piece = A || (y >= head && y < tail);
-            const int place = in_piece ? max(y, 0) - head : 0, piece = place / K;
+            const unsigned place = in_piece ? (unsigned)(max(y, 0) - head) : 0u, piece = place / K;
             T* const at = (T*)(base + piece / G * 32 + grp * G + piece % G) + place % K;
             float xt = f32(*at);
             __syncwarp();
-            const bool owner = in_piece && piece % G == sub;
+            const bool owner = in_piece && (int)(piece % G) == sub;
             if (owner) *at = lowest<T>();
             if (!A) {
                 const float v = __shfl_sync(~0u, ex, grp * G + (y < head ? max(y, 0) : 8 + y - tail) % G);
@@ -506,17 +525,18 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
                                  MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
                 float g = 0.f, term = 0.f;
                 if (y >= 0) {
-                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, (float)w, scale, term);
+                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, wf, scale, term);
                     if (MODE == POLICY && sub == 0) sum += (double)term;
                 }
+                const bool some_off = __any_sync(~0u, y < 0);
                 if (d && row < rows) {
                     const bool same = A || alike(x, d);
-                    const float inv = 1.f / (o + et), f = -g * inv;
+                    const float inv = reciprocal(o + et), f = -g * inv;
 #pragma unroll
                     for (int j = 0; j < NV; j++) {
                         times(e[j], f);
                         uint4 v = pack<T>(e[j]);
-                        if (y < 0) v = make_uint4(0u, 0u, 0u, 0u);
+                        if (some_off && y < 0) v = make_uint4(0u, 0u, 0u, 0u);
                         if (sub + j * G < n) store_raw(d + head + (sub + j * G) * K, same, v);
                     }
                     if (!A && edge >= 0) d[edge] = from32<T>(y < 0 ? 0.f : edge == y ? g * (o * inv) : f * ee);
@@ -546,6 +566,10 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
 // by a lane each), into an image of it in shared memory. A group of G lanes takes a row from the image in its 32-bit words,
 // lane by lane; of a first or last word that it shares with its neighbour it masks the half that is not its own. The gradient
 // replaces the logits in the image and leaves as the stretch came.
+//
+// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 21 us, policy loss and gradient 31 us, bound by the work of a
+// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 57 and 104 us, bound by
+// instructions as the rows above, with a load and a mask a word more.
 template <typename T> __device__ __forceinline__ float word_max(uint32_t a, float m);
 template <> __device__ __forceinline__ float word_max<float>(uint32_t a, float m) { return fmaxf(m, __uint_as_float(a)); }
 template <> __device__ __forceinline__ float word_max<__nv_bfloat16>(uint32_t a, float m) {
@@ -566,6 +590,7 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
     const float scale = MODE != LOGP && k.scale ? *k.scale : 1.f;
     if (MODE != LOGP && k.skip_one && scale == 1.f) return;
     uint4* const ring = rings + (threadIdx.x >> 5) * (S * SLOT);
+    const uint32_t ring_at = shared_at(ring);
 
     const int64_t W = k.b.W, tiles = k.b.n * k.tpw, stride = (int64_t)gridDim.x * WARPS, si = stride / k.tpw, st = stride - si * k.tpw;
     const int64_t first = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
@@ -590,9 +615,9 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
         if (in.r < tiles) {
             if (in_on >> (in_s * RP) & STEP) {
                 const Stretch q = stretch(in_x, in_s, rows_of_tile(in));
-                uint4* const to = ring + in_slot * SLOT;
+                const uint32_t to = ring_at + in_slot * (SLOT * 16);
                 const T* const from = in_x - q.off;
-                for (int p = lane + (q.off > 0); (p + 1) * K <= q.off + q.len; p += 32) copy16(to + p, from + p * K);
+                for (int p = lane + (q.off > 0); (p + 1) * K <= q.off + q.len; p += 32) copy16(to + p * 16, from + p * K);
             }
             in_x += RP * V;
             if (++in_s == G) {
@@ -689,7 +714,7 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
                     if (MODE == POLICY && sub == 0) sum += (double)term;
                 }
                 if (d) {
-                    const float inv = 1.f / (o + et), f = -g * inv;
+                    const float inv = reciprocal(o + et), f = -g * inv;
                     times(e, f);
                     __syncwarp();
 #pragma unroll
@@ -810,7 +835,7 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
         const float c = ref_of(all.m), t = exponent(xt, all.m, c), e = ex2(t);
         float term;
         const float lp = row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
-        const float inv = 1.f / (all.o + e);
+        const float inv = reciprocal(all.o + e);
         if (lane == 0) {
             if (rank == 0) {
                 if (MODE == LOGP && k.logp) k.logp[r] = lp;
@@ -860,6 +885,13 @@ __device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V
 //
 // C: blocks of a cluster that share a row, each a span of its pieces; they leave each other what their warps found in
 // distributed shared memory, behind one cluster barrier a row.
+//
+// On a B200: log-probabilities of 32,768 rows of 16,384 bf16 words 199 us (5.4 TB/s), their gradient from kept statistics 353
+// us (6.1 TB/s, read and written): bound by memory. The policy loss and gradient of 16,384 rows of 65,541 words 889 us (4.8
+// TB/s): two 2^x and some 15 instructions a word at 24 warps a multiprocessor, which wait on each other at a row's end.
+// Threads a row, the fewest that hold it, since each warp pays a row's overhead (16,380 rows of 4,101 words: 68 us with
+// 32 threads, 85 with 64, 102 with 128; 8,192 of 16,384: 104 us with 128, 132 with 256). Pieces kept in registers between the
+// passes, so that copies go on during both, lost to their warps' latency (16,384 words: 523 us, and 397 us from the ring).
 
 // warps that a multiprocessor holds with P pieces a thread in the ring, 32 at most (64 registers a thread)
 template <int P> constexpr int RING_WARPS = 220 * 1024 / (P * 512) < 32 ? 220 * 1024 / (P * 512) : 32;
@@ -884,11 +916,15 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
         return q;
     };
 
-    // what is copied next: step in_j of the lowest row in in_left, the counted ones of a lot, into slot in_slot
+    // what is copied next: step in_j of the lowest row in in_left, the counted ones of a lot, to in_to in the ring
+    constexpr uint32_t STEP = U * THREADS * 16;
+    const uint32_t ring_at = shared_at(ring + tid), ring_end = ring_at + S * STEP;
     int64_t in_first = first_row, in_at = 0;                 // in_at: a lane's row in the logits
     unsigned in_left = 0;
-    const T* in_x = nullptr;                                 // this thread's first piece
-    int in_j = 0, in_slot = 0, in_n = 0;                     // in_n: the row's whole pieces
+    const T* in_x = nullptr;                                 // this thread's next piece
+    int in_j = 0, in_full = 0, in_n = 0;                     // the first steps whose pieces are all in the row; the row's whole pieces
+    uint32_t in_to = ring_at;
+    const auto full_of = [&](int n) { return n / (U * THREADS) - rank * steps; };
     const auto find = [&]() {
         while (!in_left && in_first < rows) {
             const Lot q = lot_of(in_first);
@@ -900,37 +936,40 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
             const T* x = (const T*)k.b.logits + __shfl_sync(~0u, in_at, __ffs(in_left) - 1);
             const int head = head_of(x, V);
             in_n = (V - head) / K;
+            in_full = full_of(in_n);
             in_x = x + head + (int64_t)p0 * K;
         }
     };
     find();
     const auto copy_next = [&]() {
         if (in_left) {
-            const int p = p0 + in_j * U * THREADS;
-            const T* from = in_x + in_j * U * SPAN;
-            uint4* to = &ring[in_slot * U * THREADS + tid];
-            if (__all_sync(~0u, p + (U - 1) * THREADS < in_n)) {
+            if (in_j < in_full) {
 #pragma unroll
-                for (int u = 0; u < U; u++) copy16(to + u * THREADS, from + u * SPAN);
+                for (int u = 0; u < U; u++) copy16(in_to + u * (THREADS * 16), in_x + u * SPAN);
             } else {
+                const int p = p0 + in_j * U * THREADS;
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if (p + u * THREADS < in_n) copy16(to + u * THREADS, from + u * SPAN);
+                    if (p + u * THREADS < in_n) copy16(in_to + u * (THREADS * 16), in_x + u * SPAN);
             }
+            in_x += U * SPAN;
             if (++in_j == steps) {
                 in_j = 0;
                 in_left &= in_left - 1;
                 find();
             }
         }
-        if (++in_slot == S) in_slot = 0;
+        in_to += STEP;
+        if (in_to == ring_end) in_to = ring_at;
         copies_commit();
     };
 #pragma unroll 1
     for (int s = 0; s < S; s++) copy_next();
     if (C > 1) cluster_barrier();                            // every block of the cluster runs before one writes to another
 
-    int slot = 0, turn = 0;
+    uint4* const own_ring = ring + tid;
+    uint4* slot = own_ring;                                  // the row's first step
+    int turn = 0;
     for (int64_t first = first_row; first < rows; first += 32 * stride) {
         const Lot lot = lot_of(first);
         const int64_t x_at = lot.i * k.b.logits_n + lot.t * k.b.logits_w, d_at = lot.i * k.b.grad_n + lot.t * k.b.grad_w;
@@ -975,15 +1014,19 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                 const int q = (y - head) / K - p0;
                 if (q >= 0 && q % THREADS == 0 && q < steps * U * THREADS) { own_j = q / (THREADS * U); own_u = q / THREADS % U; }
             }
-            int at = slot;
+            uint4* from = slot;
+            const auto on = [&]() {
+                from += U * THREADS;
+                if (from == own_ring + S * U * THREADS) from = own_ring;
+            };
+            const int full = full_of(n);
             float4 g;
             if constexpr (MODE == GIVEN) {
                 g = make_float4(__shfl_sync(~0u, stats.x, l), __shfl_sync(~0u, stats.y, l), __shfl_sync(~0u, stats.z, l), __shfl_sync(~0u, stats.w, l));
             } else {
                 Run run;
+#pragma unroll 1
                 for (int j = 0; j < steps; j++) {
-                    const int p = p0 + j * U * THREADS;
-                    uint4* const from = &ring[at * U * THREADS + tid];
                     copies_wait<S - 1>();
                     if (j == own_j) {                        // the target's logit out of the ring, -inf in its place
                         T* own = (T*)(from + own_u * THREADS) + (y - head) % K;
@@ -991,10 +1034,11 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                         *own = lowest<T>();
                     }
                     uint4 raw[U];
-                    if (__all_sync(~0u, p + (U - 1) * THREADS < n)) {
+                    if (j < full) {
 #pragma unroll
                         for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
                     } else {
+                        const int p = p0 + j * U * THREADS;
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             raw[u] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
@@ -1015,9 +1059,9 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                         const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
 #pragma unroll 1
                         for (int u = 0; u < U; u++)
-                            if (p + u * THREADS < n) run.o = sum_far<T, 1>(from + u * THREADS, 0, by, run.c, run.o);
+                            if (p0 + (j * U + u) * THREADS < n) run.o = sum_far<T, 1>(from + u * THREADS, 0, by, run.c, run.o);
                     }
-                    if (++at == S) at = 0;
+                    on();
                     if (grad) copies_commit(); else copy_next();
                 }
                 End end = {0.f, 0.f, 0.f};
@@ -1039,16 +1083,15 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                 }
                 g = block_end<MODE, NW, C>(k, meet, turn, run, end, w, scale, r, grad, rank);
                 turn ^= 1;
-                if (grad) at = slot;
+                if (grad) from = slot;
             }
             if (grad) {
-                const bool plain = alike(x, d) && !far(g.x);
+                const int plain = alike(x, d) && !far(g.x) ? full : 0;
                 T* to = d + head + (int64_t)p0 * K;
+#pragma unroll 1
                 for (int j = 0; j < steps; j++, to += U * SPAN) {
-                    const int p = p0 + j * U * THREADS;
-                    const uint4* const from = &ring[at * U * THREADS + tid];
                     if (MODE == GIVEN) copies_wait<S - 1>();
-                    if (__all_sync(~0u, plain && p + (U - 1) * THREADS < n)) {
+                    if (j < plain) {
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             float v[K];
@@ -1058,17 +1101,18 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                             *(uint4*)(to + u * SPAN) = pack<T>(v);
                         }
                     } else {
+                        const int p = p0 + j * U * THREADS;
 #pragma unroll 1
                         for (int u = 0; u < U && p + u * THREADS < n; u++)
                             grad_piece(from[u * THREADS], d, head + (p + u * THREADS) * K, V, alike(x, d), g);
                     }
                     if (j == own_j) d[y] = from32<T>(g.w);
-                    if (++at == S) at = 0;
+                    on();
                     copy_next();
                 }
                 if (edge >= 0) d[edge] = from32<T>(edge == y ? g.w : g.z * ex2(exponent(ex, g.x, g.y)));
             }
-            slot = at;
+            slot = from;
         }
     }
     copies_wait<0>();
@@ -1144,8 +1188,8 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const double* part, int64_t
     if (threadIdx.x == 0) *loss = m ? (float)(all / (double)m) : 0.f;
 }
 
-// Counted positions of each window, turned into weights: up to COUNT_ONE positions by one block, a warp a window; more by a
-// block per (window, span of it) first.
+// Counted positions of each window, turned into weights: up to COUNT_ONE positions by one block, a warp a window (4,072
+// positions 6 us; 16,384 take it 36 us); more by a block per (window, span of it) first (16,384 positions 6 us and 3).
 constexpr int COUNT_SPAN = 2048, COUNT_ONE = 4096;
 __global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, int32_t* counts) {
     for (int64_t q = blockIdx.x; q < b.n * spans; q += gridDim.x) {
@@ -1355,10 +1399,10 @@ void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
             else ring_rows<T, 256, 3, 6, 2, MODE>(k, p.pieces, st);
         }
     } else if constexpr (MODE != GRAD) {
-        // read once, a row need not fit the ring: a warp a row where the rows fill the GPU with 16 warps a multiprocessor,
-        // else four warps or sixteen
+        // read once, a row need not fit the ring: a warp a row where the rows fill the GPU with 16 warps a multiprocessor
+        // (16,380 rows of 4,101 words: 41 us, four warps a row 67; 8,192 of 16,384: 55 and 56), else four warps or sixteen
         const int64_t rows = k.b.n * k.b.W;
-        if (rows >= SMS * 16) ring_rows<T, 32, 4, 3, 1, MODE>(k, p.pieces, st);
+        if (rows >= SMS * 16) ring_rows<T, 32, MODE == GIVEN ? 4 : 3, MODE == GIVEN ? 3 : 4, 1, MODE>(k, p.pieces, st);
         else if (rows >= SMS * 4) ring_rows<T, 128, 4, 3, 1, MODE>(k, p.pieces, st);
         else ring_rows<T, 512, 4, 3, 1, MODE>(k, p.pieces, st);
     }
@@ -1478,7 +1522,7 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
         k.stat = (float4*)stat;
         if (const int e = launch_rows<LOGP>(k, p, st)) return e;
     }
-    // up to 4,096 parts the one block adds itself (4 a lane), more a block a window before it
+    // up to 4,096 parts the one block adds itself (3 us; 32,768 take it 12 us), more a block a window before it (4 us and 3)
     int64_t parts = p.tpw;
     const double* from = s.part;
     if (p.tiles > 4096) {
