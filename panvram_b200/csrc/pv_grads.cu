@@ -2,15 +2,17 @@
 // (include/panvram_b200.h pv_grad_norm, pv_clip_grads).
 //
 // The tensors' addresses, counts and types travel as a kernel parameter, so a call copies no table to the device and
-// can be captured. A block takes chunks of CHUNK elements in turn, whatever tensor they lie in, and leaves one partial
-// sum in 64 bits; the scaling kernel's blocks each add those partial sums in the same order, so no launch is spent on
-// it and the result does not change from call to call. Squares are added eight (or four) at a time in 32 bits and then
-// in 64; where such a group leaves the range of 32 bits (elements beyond about 1e18 or all below 1e-13) it is squared
-// again in 64 bits, so the norm neither overflows nor underflows before it is rounded to float at the end.
+// can be captured. The blocks share the elements evenly, in units of UNIT, over as many tensors as a run of units spans,
+// and leave one partial sum each, in 64 bits; the scaling kernel's blocks each add those partial sums in the same
+// order, so no launch is spent on it and the result does not change from call to call. Squares are added eight (or four) at
+// a time in 32 bits and then in 64; where such a group leaves the range of 32 bits (elements beyond about 1e18 or all below
+// 1e-13) it is squared again in 64 bits, so the norm neither overflows nor underflows before it is rounded to float at the end.
 //
-// Bound by memory: on a B200 the norm of 1.0e9 bf16 elements in 290 tensors takes 254 us (7.9 TB/s, reading alone), 1.0e8
-// bf16 clipped into float in 146 tensors 37 + 108 us (the second 5.6 TB/s read and written). The elements are read twice where they are scaled, as the factor
-// needs the whole norm; the scaling takes the chunks in reverse, from what the norm's pass left in L2.
+// Bound by memory: on a B200 the norm of 8.4e8 bf16 elements in 122 tensors takes 262 us (6.4 TB/s); 8.4e7 in 146 tensors,
+// clipped into float, 39 + 86 us (the second 5.9 TB/s read and written). A contiguous run a block takes 69 us there for the
+// norm, rounds without the even share of the rest 37 + 108 us.
+// The elements are read twice where they are scaled, as the factor needs the whole norm; the scaling begins
+// with what the norm's pass read last and left in L2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,13 +30,13 @@ namespace {
 
 using pvb::g_cuda_err;
 
-constexpr int CHUNK = 16384, THREADS = 256, SMS = 148, GRID = SMS * 8;
+constexpr int UNIT = 2048, RUN = 8, THREADS = 256, SMS = 148, GRID = SMS * 8;
 
 template <int N>
 struct Table {
     uint64_t ptr[N], out[N];
     int64_t numel[N];
-    uint32_t first[N + 1];           // a tensor's first chunk
+    uint32_t first[N + 1];           // a tensor's first unit
     uint8_t type[N], otype[N];
     int32_t count;
 };
@@ -50,7 +52,7 @@ template <> __device__ __forceinline__ float from32<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T, int N> struct alignas(16) Vec { T v[N]; };
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
 
 template <int K>
 __device__ __forceinline__ double squares(const float (&x)[K]) {
@@ -81,7 +83,7 @@ __device__ double block_sum(double v) {                      // every thread of 
     return sh[32];
 }
 
-// the tensor that chunk c lies in: the last whose first chunk is not after it (empty tensors share their successor's)
+// the tensor that unit c lies in: the last whose first unit is not after it (empty tensors share their successor's)
 template <int N>
 __device__ __forceinline__ int tensor_of(const Table<N>& t, uint32_t c) {
     int lo = 0, hi = t.count;
@@ -96,8 +98,34 @@ __device__ __forceinline__ int tensor_of(const Table<N>& t, uint32_t c) {
 template <typename T>
 __device__ __forceinline__ int to_boundary(const T* p) { return (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T)); }
 
+// f(tensor, first element, count) for the elements of this block: RUN units in every round over the blocks, and an even share
+// of the units that are left; BACK: in reverse
+template <bool BACK, int N, typename F>
+__device__ __forceinline__ void spans(const Table<N>& t, F&& f) {
+    const uint64_t units = t.first[t.count], round = (uint64_t)RUN * gridDim.x, rounds = units / round, done = rounds * round, left = units - done;
+    const auto run = [&](uint32_t begin, uint32_t end) {
+        int i = begin < end ? tensor_of(t, begin) : 0;
+        while (begin < end) {
+            const uint32_t first = t.first[i], to = min(end, t.first[i + 1]);
+            if (to > begin) {
+                const int64_t at = (int64_t)(begin - first) * UNIT;
+                f(i, at, (int)min((int64_t)(to - begin) * UNIT, t.numel[i] - at));
+                begin = to;
+            }
+            i++;
+        }
+    };
+    const auto share = [&]() { run((uint32_t)(done + left * blockIdx.x / gridDim.x), (uint32_t)(done + left * (blockIdx.x + 1) / gridDim.x)); };
+    if (BACK) share();
+    for (uint64_t k = 0; k < rounds; k++) {
+        const uint32_t begin = (uint32_t)((BACK ? rounds - 1 - k : k) * round + (uint64_t)RUN * blockIdx.x);
+        run(begin, begin + RUN);
+    }
+    if (!BACK) share();
+}
+
 template <typename T>
-__device__ double chunk_squares(const T* p, int count) {
+__device__ double span_squares(const T* p, int count) {
     constexpr int K = 16 / sizeof(T);
     const int head = min(to_boundary(p), count), nv = (count - head) / K, tail = head + nv * K;
     double s = 0;
@@ -120,16 +148,13 @@ __device__ double chunk_squares(const T* p, int count) {
 template <int N>
 __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ Table<N> t, double* part) {
     double s = 0;
-    for (uint32_t c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const int i = tensor_of(t, c);
-        const int64_t at = (int64_t)(c - t.first[i]) * CHUNK;
-        const int count = (int)min((int64_t)CHUNK, t.numel[i] - at);
+    spans<false>(t, [&](int i, int64_t at, int count) {
         switch (t.type[i]) {
-            case PV_T_BF16: s += chunk_squares((const __nv_bfloat16*)t.ptr[i] + at, count); break;
-            case PV_T_FP16: s += chunk_squares((const __half*)t.ptr[i] + at, count); break;
-            default: s += chunk_squares((const float*)t.ptr[i] + at, count);
+            case PV_T_BF16: s += span_squares((const __nv_bfloat16*)t.ptr[i] + at, count); break;
+            case PV_T_FP16: s += span_squares((const __half*)t.ptr[i] + at, count); break;
+            default: s += span_squares((const float*)t.ptr[i] + at, count);
         }
-    }
+    });
     s = block_sum(s);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
@@ -145,25 +170,25 @@ __global__ void __launch_bounds__(THREADS) finish_norm_kernel(const double* part
     if (threadIdx.x == 0) *norm = (float)s;
 }
 
+// Sixteen bytes a store and a thread next to a thread, whatever the elements become: widened ones are loaded eight bytes a
+// thread. Streaming stores, which leave the gradients in L2 for the spans to come.
 template <typename T, typename O>
-__device__ void scale_chunk(const T* p, O* o, int count, float f) {
-    constexpr int K = 16 / sizeof(T);
-    int head = min(to_boundary(p), count), nv = (count - head) / K;
-    if (((uintptr_t)(o + head) & 15) != 0) { head = count; nv = 0; }     // the two differ in alignment: element by element
+__device__ void scale_span(const T* p, O* o, int count, float f) {
+    constexpr int K = 16 / sizeof(O);
+    int head = min(to_boundary(o), count), nv = (count - head) / K;
+    if (((uintptr_t)(p + head) & (sizeof(T) * K - 1)) != 0) { head = count; nv = 0; }     // the two differ in alignment: element by element
     const int tail = head + nv * K;
     for (int j = threadIdx.x; j < head; j += THREADS) o[j] = from32<O>(f32(p[j]) * f);
     for (int j = tail + threadIdx.x; j < count; j += THREADS) o[j] = from32<O>(f32(p[j]) * f);
-    const uint4* q = (const uint4*)(p + head);
+    const auto* q = (const Vec<T, K>*)(p + head);
+    uint4* w = (uint4*)(o + head);
 #pragma unroll 4
     for (int j = threadIdx.x; j < nv; j += THREADS) {
-        const uint4 raw = q[j];
-        const Vec<T, K>& v = *(const Vec<T, K>*)&raw;
-        Vec<O, K> w;
+        const Vec<T, K> v = q[j];
+        Vec<O, K> r;
 #pragma unroll
-        for (int e = 0; e < K; e++) w.v[e] = from32<O>(f32(v.v[e]) * f);
-        // streaming stores, which leave the gradients in L2 for the chunks to come
-#pragma unroll
-        for (int b = 0; b < (int)(sizeof(O) * K / 16); b++) __stcs((uint4*)(o + head + j * K) + b, ((const uint4*)&w)[b]);
+        for (int e = 0; e < K; e++) r.v[e] = from32<O>(f32(v.v[e]) * f);
+        __stcs(w + j, *(const uint4*)&r);
     }
 }
 
@@ -174,25 +199,20 @@ __global__ void __launch_bounds__(THREADS) clip_kernel(const __grid_constant__ T
     const float f = r >= 1.0 ? 1.f : (float)r;               // NaN stays
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)s;
     if (in_place && f == 1.f) return;
-    // last chunks first: the norm's pass left those in L2
-    for (int64_t q = (int64_t)t.first[t.count] - 1 - blockIdx.x; q >= 0; q -= gridDim.x) {
-        const uint32_t c = (uint32_t)q;
-        const int i = tensor_of(t, c);
-        const int64_t at = (int64_t)(c - t.first[i]) * CHUNK;
-        const int count = (int)min((int64_t)CHUNK, t.numel[i] - at);
+    spans<true>(t, [&](int i, int64_t at, int count) {
         const bool wide = t.otype[i] == PV_T_FP32;
         switch (t.type[i]) {
             case PV_T_BF16:
-                if (wide) scale_chunk((const __nv_bfloat16*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
-                else scale_chunk((const __nv_bfloat16*)t.ptr[i] + at, (__nv_bfloat16*)t.out[i] + at, count, f);
+                if (wide) scale_span((const __nv_bfloat16*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
+                else scale_span((const __nv_bfloat16*)t.ptr[i] + at, (__nv_bfloat16*)t.out[i] + at, count, f);
                 break;
             case PV_T_FP16:
-                if (wide) scale_chunk((const __half*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
-                else scale_chunk((const __half*)t.ptr[i] + at, (__half*)t.out[i] + at, count, f);
+                if (wide) scale_span((const __half*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
+                else scale_span((const __half*)t.ptr[i] + at, (__half*)t.out[i] + at, count, f);
                 break;
-            default: scale_chunk((const float*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
+            default: scale_span((const float*)t.ptr[i] + at, (float*)t.out[i] + at, count, f);
         }
-    }
+    });
 }
 
 // ---------------------------------------------------------------- host
@@ -253,7 +273,7 @@ int64_t fill(Table<N>& t, const pv_tensors* g, const pv_tensors* out, int64_t fr
         t.out[k] = out ? out->ptr[i] : g->ptr[i];
         t.otype[k] = out ? out->type[i] : g->type[i];
         t.first[k] = (uint32_t)c;
-        c += (uint64_t)((g->numel[i] + CHUNK - 1) / CHUNK);
+        c += (uint64_t)((g->numel[i] + UNIT - 1) / UNIT);
     }
     t.first[t.count] = (uint32_t)c;
     return c < (1ull << 32) ? (int64_t)c : -1;
@@ -264,9 +284,9 @@ template <int N>
 int one(const pv_tensors* g, const pv_tensors* out, int64_t from, int64_t to, bool clip, double* part, int64_t* parts, float max_norm, bool in_place,
         float* norm, cudaStream_t st) {
     static thread_local Table<N> t;
-    const int64_t chunks = fill(t, g, out, from, to);
-    if (chunks < 0) return fail(PV_EARG, "tensors: too many elements in one list");
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks, GRID));
+    const int64_t units = fill(t, g, out, from, to);
+    if (units < 0) return fail(PV_EARG, "tensors: too many elements in one list");
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(units, GRID));
     if (clip) {
         clip_kernel<N><<<grid, THREADS, 0, st>>>(t, part, *parts, max_norm, in_place, norm);
     } else {
