@@ -17,6 +17,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "panvram_b200.h"
 
@@ -1033,33 +1034,37 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                         meet.template tell<C>(meet.xt[turn], f32(*own));
                         *own = lowest<T>();
                     }
-                    uint4 raw[U];
-                    if (j < full) {
+                    // Q pieces of this thread, the u-th on
+                    const auto pieces = [&](auto Q, int u) {
+                        constexpr int q = decltype(Q)::value;
+                        uint4 raw[q];
 #pragma unroll
-                        for (int u = 0; u < U; u++) raw[u] = from[u * THREADS];
-                    } else {
-                        const int p = p0 + j * U * THREADS;
-#pragma unroll
-                        for (int u = 0; u < U; u++) {
-                            raw[u] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
-                            if (p + u * THREADS < n) raw[u] = from[u * THREADS];
+                        for (int h = 0; h < q; h++) {
+                            raw[h] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
+                            if (q > 1 || p0 + (j * U + u) * THREADS < n) raw[h] = from[(u + h) * THREADS];
                         }
-                    }
-                    float m = piece_max<T>(raw[0]);
+                        float m = piece_max<T>(raw[0]);
 #pragma unroll
-                    for (int u = 1; u < U; u++) m = fmaxf(m, piece_max<T>(raw[u]));
-                    bool plain = true;
-                    if (__any_sync(~0u, m > run.m + HEADROOM || far(run.m))) {
-                        raise(run, m);
-                        plain = !__any_sync(~0u, far(run.m));
-                    }
-                    if (plain) {
-                        run.o = sum_all<T, U>(raw, run.c, run.o);
-                    } else {                                 // a maximum beyond 2^29, or none yet
-                        const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
+                        for (int h = 1; h < q; h++) m = fmaxf(m, piece_max<T>(raw[h]));
+                        bool plain = true;
+                        if (__any_sync(~0u, m > run.m + HEADROOM || far(run.m))) {
+                            raise(run, m);
+                            plain = !__any_sync(~0u, far(run.m));
+                        }
+                        if (plain) {
+                            run.o = sum_all<T, q>(raw, run.c, run.o);
+                        } else {                             // a maximum beyond 2^29, or none yet
+                            const float by = far(run.m) && run.m != -INFINITY ? run.m : 0.f;
 #pragma unroll 1
-                        for (int u = 0; u < U; u++)
-                            if (p0 + (j * U + u) * THREADS < n) run.o = sum_far<T, 1>(from + u * THREADS, 0, by, run.c, run.o);
+                            for (int h = 0; h < q; h++)
+                                if (p0 + (j * U + u + h) * THREADS < n) run.o = sum_far<T, 1>(from + (u + h) * THREADS, 0, by, run.c, run.o);
+                        }
+                    };
+                    if (j < full) {
+                        pieces(std::integral_constant<int, U>(), 0);
+                    } else {                                 // one at a time, while any thread has one
+#pragma unroll 1
+                        for (int u = 0; u < U && p0 - tid + (j * U + u) * THREADS < n; u++) pieces(std::integral_constant<int, 1>(), u);
                     }
                     on();
                     if (grad) copies_commit(); else copy_next();
@@ -1086,25 +1091,29 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                 if (grad) from = slot;
             }
             if (grad) {
-                const int plain = alike(x, d) && !far(g.x) ? full : 0;
+                const bool plain = alike(x, d) && !far(g.x);
                 T* to = d + head + (int64_t)p0 * K;
 #pragma unroll 1
                 for (int j = 0; j < steps; j++, to += U * SPAN) {
                     if (MODE == GIVEN) copies_wait<S - 1>();
-                    if (j < plain) {
+                    const auto piece = [&](int u) {
+                        float v[K];
+                        unpack<T>(from[u * THREADS], v);
+                        numerators(v, g.y);
+                        times(v, g.z);
+                        *(uint4*)(to + u * SPAN) = pack<T>(v);
+                    };
+                    if (plain && j < full) {
 #pragma unroll
-                        for (int u = 0; u < U; u++) {
-                            float v[K];
-                            unpack<T>(from[u * THREADS], v);
-                            numerators(v, g.y);
-                            times(v, g.z);
-                            *(uint4*)(to + u * SPAN) = pack<T>(v);
-                        }
+                        for (int u = 0; u < U; u++) piece(u);
                     } else {
-                        const int p = p0 + j * U * THREADS;
 #pragma unroll 1
-                        for (int u = 0; u < U && p + u * THREADS < n; u++)
-                            grad_piece(from[u * THREADS], d, head + (p + u * THREADS) * K, V, alike(x, d), g);
+                        for (int u = 0; u < U; u++) {
+                            const int p = p0 + (j * U + u) * THREADS;
+                            if (p >= n) break;
+                            if (plain) piece(u);
+                            else grad_piece(from[u * THREADS], d, head + p * K, V, alike(x, d), g);
+                        }
                     }
                     if (j == own_j) d[y] = from32<T>(g.w);
                     on();
@@ -1402,7 +1411,7 @@ void typed_rows(const Rows& k, const Plan& p, cudaStream_t st) {
         // read once, a row need not fit the ring: a warp a row where the rows fill the GPU with 16 warps a multiprocessor
         // (16,380 rows of 4,101 words: 41 us, four warps a row 67; 8,192 of 16,384: 55 and 56), else four warps or sixteen
         const int64_t rows = k.b.n * k.b.W;
-        if (rows >= SMS * 16) ring_rows<T, 32, MODE == GIVEN ? 4 : 3, MODE == GIVEN ? 3 : 4, 1, MODE>(k, p.pieces, st);
+        if (rows >= SMS * 16) ring_rows<T, 32, MODE == GIVEN ? 4 : 6, MODE == GIVEN ? 3 : 2, 1, MODE>(k, p.pieces, st);
         else if (rows >= SMS * 4) ring_rows<T, 128, 4, 3, 1, MODE>(k, p.pieces, st);
         else ring_rows<T, 512, 4, 3, 1, MODE>(k, p.pieces, st);
     }
