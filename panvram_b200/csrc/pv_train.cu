@@ -1143,19 +1143,35 @@ __device__ double block_sum(double v) {                      // every thread of 
     return sh[32];
 }
 
-// a block per window: the sum of its tiles
-__global__ void __launch_bounds__(256) window_sums_kernel(const double* part, int64_t n, int64_t tpw, float* sums, double* sums64) {
-    for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+// the sums of each window's tiles: a warp a window up to SUMS_WARP tiles, else a block
+constexpr int SUMS_WARP = 512;
+__global__ void __launch_bounds__(1024) window_sums_kernel(const double* part, int64_t n, int64_t tpw, float* sums, double* sums64) {
+    const bool warp = tpw <= SUMS_WARP;
+    const int first = warp ? threadIdx.x & 31 : threadIdx.x, step = warp ? 32 : 1024;
+    for (int64_t i = warp ? (int64_t)blockIdx.x * 32 + (threadIdx.x >> 5) : blockIdx.x; i < n; i += warp ? (int64_t)gridDim.x * 32 : gridDim.x) {
         double v = 0;
-        for (int64_t j = threadIdx.x; j < tpw; j += blockDim.x) v += part[i * tpw + j];
-        v = block_sum(v);
-        if (threadIdx.x == 0) {
+#pragma unroll 8
+        for (int64_t j = first; j < tpw; j += step) v += part[i * tpw + j];
+        v = warp ? warp_sum(v) : block_sum(v);
+        if (first == 0) {
             if (sums) sums[i] = (float)v;
             if (sums64) sums64[i] = v;
         }
     }
 }
 
+// a block per FOLD of `count` partial sums
+constexpr int FOLD = 4096;
+__global__ void __launch_bounds__(256) fold_kernel(const double* part, int64_t count, double* out) {
+    double v = 0;
+#pragma unroll
+    for (int u = 0; u < FOLD / 256; u++) {
+        const int64_t j = (int64_t)blockIdx.x * FOLD + u * 256 + threadIdx.x;
+        if (j < count) v += part[j];
+    }
+    v = block_sum(v);
+    if (threadIdx.x == 0) out[blockIdx.x] = v;
+}
 // one block: the sum of `count` partial sums
 __global__ void __launch_bounds__(1024) total_kernel(const double* part, int64_t count, float* out) {
     double v = 0;
@@ -1198,19 +1214,46 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const double* part, int64_t
 }
 
 // Counted positions of each window, turned into weights: up to COUNT_ONE positions by one block, a warp a window (4,072
-// positions 6 us; 16,384 take it 36 us); more by a block per (window, span of it) first (16,384 positions 6 us and 3).
-constexpr int COUNT_SPAN = 2048, COUNT_ONE = 4096;
-__global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, int32_t* counts) {
-    for (int64_t q = blockIdx.x; q < b.n * spans; q += gridDim.x) {
-        const int64_t i = q / spans, t0 = (q - i * spans) * COUNT_SPAN;
-        int v = 0;
+// positions 7 us; 16,384 take it 36 us); more by a warp per (window, span of it) first (16,384 positions 3 us and 3).
+constexpr int COUNT_SPAN = 256, COUNT_ONE = 4096;
+// this lane's part of the counted positions [t0, t0 + COUNT_SPAN) of window i: eight tokens and masks in flight
+template <typename Token, typename Mask>
+__device__ __forceinline__ int count_span(const pv_scored& b, int64_t i, int64_t t0, int lane) {
+    constexpr bool MASK = !std::is_void<Mask>::value;
+    using M = typename std::conditional<MASK, Mask, uint8_t>::type;
+    const Token* tokens = (const Token*)b.tokens + i * b.tokens_n;
+    const M* mask = (const M*)b.mask + i * b.mask_n;
+    Token y[8];
+    M m[8];
+    bool in[8];
 #pragma unroll
-        for (int u = 0; u < COUNT_SPAN / 256; u++) {
-            const int64_t t = t0 + threadIdx.x + u * 256;
-            v += t < b.W && target(b, i, t) >= 0;
-        }
-        v = (int)block_sum((double)v);
-        if (threadIdx.x == 0) counts[q] = v;
+    for (int u = 0; u < 8; u++) {
+        const int64_t at = t0 + u * 32 + lane + b.shift, from = at < b.W ? at : 0;
+        in[u] = at < b.W;
+        y[u] = tokens[from * b.tokens_w];
+        if (MASK) m[u] = mask[from * b.mask_w];
+    }
+    int v = 0;
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+        const int64_t w = y[u];
+        v += in[u] && w >= 0 && w < b.V && w != b.ignore && (!MASK || m[u] != (M)0);
+    }
+    return v;
+}
+__global__ void __launch_bounds__(256) count_kernel(pv_scored b, int64_t spans, int32_t* counts) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t q = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); q < b.n * spans; q += (int64_t)gridDim.x * 8) {
+        const int64_t i = q / spans, t0 = (q - i * spans) * COUNT_SPAN;
+        int v;
+        if (b.token_bytes == 1)
+            v = b.mask_bytes == 0 ? count_span<uint8_t, void>(b, i, t0, lane) : b.mask_bytes == 1 ? count_span<uint8_t, uint8_t>(b, i, t0, lane)
+                                                                                               : count_span<uint8_t, float>(b, i, t0, lane);
+        else
+            v = b.mask_bytes == 0 ? count_span<int64_t, void>(b, i, t0, lane) : b.mask_bytes == 1 ? count_span<int64_t, uint8_t>(b, i, t0, lane)
+                                                                                               : count_span<int64_t, float>(b, i, t0, lane);
+        v = (int)__reduce_add_sync(~0u, (unsigned)v);
+        if (lane == 0) counts[q] = v;
     }
 }
 __global__ void __launch_bounds__(1024) weights_kernel(pv_scored b, const int32_t* counts, int64_t spans, int by_window, double scale,
@@ -1218,16 +1261,27 @@ __global__ void __launch_bounds__(1024) weights_kernel(pv_scored b, const int32_
     double all = 0, some = 0;
     const int64_t n = b.n;
     const int lane = threadIdx.x & 31;
-    for (int64_t i = threadIdx.x >> 5; i < n; i += 32) {
-        int c = 0;
-        if (counts) {
-            for (int64_t j = lane; j < spans; j += 32) c += counts[i * spans + j];
-        } else {
+    if (counts && spans <= 32) {                             // a thread a window
 #pragma unroll 4
-            for (int64_t t = lane; t < b.W; t += 32) c += target(b, i, t) >= 0;
+        for (int64_t i = threadIdx.x; i < n; i += 1024) {
+            int c = 0;
+            for (int64_t j = 0; j < spans; j++) c += counts[i * spans + j];
+            weight[i] = (double)c;
+            all += (double)c;
+            some += c > 0;
         }
-        c = (int)__reduce_add_sync(~0u, (unsigned)c);
-        if (lane == 0) { weight[i] = (double)c; all += (double)c; some += c > 0; }
+    } else {
+        for (int64_t i = threadIdx.x >> 5; i < n; i += 32) {
+            int c = 0;
+            if (counts) {
+                for (int64_t j = lane; j < spans; j += 32) c += counts[i * spans + j];
+            } else {
+#pragma unroll 4
+                for (int64_t t = lane; t < b.W; t += 32) c += target(b, i, t) >= 0;
+            }
+            c = (int)__reduce_add_sync(~0u, (unsigned)c);
+            if (lane == 0) { weight[i] = (double)c; all += (double)c; some += c > 0; }
+        }
     }
     all = block_sum(all);
     some = block_sum(some);
@@ -1291,7 +1345,7 @@ Plan plan_of(const pv_scored& b) {
     p.spans = (b.W + COUNT_SPAN - 1) / COUNT_SPAN;
     return p;
 }
-// scratch: a double per tile, a double per window, an int per (window, span); the policy loss of long rows: their statistics
+// scratch: a double per tile, a double per window (and per FOLD tiles), an int per (window, span); the policy loss of long rows: their statistics
 // and derivatives
 struct Scratch { double *part, *win; float4* stat; float* deriv; int32_t* counts; size_t bytes; };
 Scratch scratch_of(const pv_scored& b, const Plan& p, void* work) {
@@ -1300,7 +1354,7 @@ Scratch scratch_of(const pv_scored& b, const Plan& p, void* work) {
     s.bytes = 0;
     const auto take = [&](size_t n) { char* r = at + s.bytes; s.bytes += (n + 15) / 16 * 16; return r; };
     s.part = (double*)take((size_t)p.tiles * 8);
-    s.win = (double*)take((size_t)b.n * 8);
+    s.win = (double*)take(std::max<size_t>((size_t)b.n, ((size_t)p.tiles + FOLD - 1) / FOLD) * 8);
     s.counts = (int32_t*)take((size_t)b.n * p.spans * 4);
     const size_t rows = p.form == LONG_ROWS ? (size_t)b.n * b.W : 0;
     s.stat = (float4*)take(rows * 16);
@@ -1441,7 +1495,8 @@ int check_work(const Scratch& s, const void* work, size_t have) {
 }
 
 int window_sums(const Plan& p, int64_t n, const double* part, float* sums, double* sums64, cudaStream_t st) {
-    window_sums_kernel<<<(unsigned)std::min<int64_t>(n, SMS * 8), 256, 0, st>>>(part, n, p.tpw, sums, sums64);
+    const int64_t blocks = p.tpw <= SUMS_WARP ? (n + 31) / 32 : n;
+    window_sums_kernel<<<(unsigned)std::min<int64_t>(blocks, SMS * 2), 1024, 0, st>>>(part, n, p.tpw, sums, sums64);
     return launched();
 }
 
@@ -1553,12 +1608,19 @@ int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* 
     const cudaStream_t st = (cudaStream_t)stream;
     if (b->n) {
         const bool one = b->n * b->W <= COUNT_ONE;
-        if (!one) count_kernel<<<(unsigned)std::min<int64_t>(b->n * p.spans, SMS * 8), 256, 0, st>>>(*b, p.spans, s.counts);
+        if (!one) count_kernel<<<(unsigned)std::min<int64_t>((b->n * p.spans + 7) / 8, SMS * 8), 256, 0, st>>>(*b, p.spans, s.counts);
         weights_kernel<<<1, 1024, 0, st>>>(*b, one ? nullptr : s.counts, p.spans, a->by_window, (double)a->scale, weight);
         if (const int e = launched()) return e;
         if (const int e = policy_rows(b, a, p, s, s.part, weight, nullptr, 0, st)) return e;
     }
-    total_kernel<<<1, 1024, 0, st>>>(s.part, p.tiles, loss);
+    // up to 16,384 parts one block adds at once (3 us), more after a block has added each FOLD of them
+    if (p.tiles <= 4 * FOLD) {
+        total_kernel<<<1, 1024, 0, st>>>(s.part, p.tiles, loss);
+    } else {
+        const int64_t folds = (p.tiles + FOLD - 1) / FOLD;
+        fold_kernel<<<(unsigned)folds, 256, 0, st>>>(s.part, p.tiles, s.win);
+        total_kernel<<<1, 1024, 0, st>>>(s.win, folds, loss);
+    }
     return launched();
 }
 

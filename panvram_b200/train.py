@@ -395,8 +395,8 @@ def clip_grads(grads, max_norm, out=None):
             raise ValueError("out: of the gradient's type, or float32")
         if written[0].device != ts[0].device:
             raise ValueError("out: on the gradients' device")
-    if True in [t.requires_grad for t in written] and any(t.requires_grad and t.is_leaf for t in written) and torch.is_grad_enabled():
-        raise ValueError("clip_grads: pass the gradients (p.grad), not parameters")
+    if True in [t.requires_grad for t in written]:
+        raise ValueError("clip_grads: pass gradients (p.grad), not parameters, and none that autograd has a graph for")
     dev = _device(ts[0], "gradients")
     with _on(dev):
         norm, work, need = _norm_buffers(g, dev)
