@@ -53,6 +53,7 @@ enum { LOGP = 0, GRAD = 1, POLICY = 2, GIVEN = 3 };
 struct Rows {
     pv_scored b;
     int64_t tpw;             // tiles (of TILE rows, or of one) per window
+    int64_t stride, stride_n; int32_t stride_t;      // short rows: from a warp's tile to its next; in windows, and tiles of one
     // LOGP
     float* logp;             // or NULL
     double* part;            // a partial sum per tile (LOGP: of log-probabilities, POLICY: of loss terms), or NULL
@@ -312,13 +313,81 @@ template <typename T>
 __device__ __forceinline__ bool alike(const T* x, const T* d) { return (((uintptr_t)x ^ (uintptr_t)d) & 15) == 0; }
 
 // ---------------------------------------------------------------- asynchronous copies into shared memory
-// places r, r + stride, ... of n windows of W, with their windows and positions
-struct Pos {
-    int64_t r, i, t;
-    __device__ __forceinline__ Pos(int64_t r, int64_t W) : r(r), i(r / W), t(r % W) {}
-    __device__ __forceinline__ void next(int64_t stride, int64_t si, int64_t st, int64_t W) {
-        r += stride; i += si; t += st;
-        if (t >= W) { t -= W; i++; }
+// A warp's tiles of TILE rows: first, first + stride, ... of those of all windows in turn, tpw to a window. The stride, as
+// windows and tiles of one, comes with the launch, so that what follows from it alone stays out of the threads' registers.
+constexpr int TILE = 32, WARPS = 8;
+struct Tiles {
+    int64_t r;               // the tile
+    int t;                   // its place in its window
+    __device__ __forceinline__ Tiles(const Rows& k) : r((int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5)), t((int)(r % k.tpw)) {}
+    __device__ __forceinline__ bool live(const Rows& k) const { return r < k.b.n * k.tpw; }
+    __device__ __forceinline__ bool next(const Rows& k) {    // whether the place in the window has wrapped
+        r += k.stride;
+        t += k.stride_t;
+        if (t < (int)k.tpw) return false;
+        t -= (int)k.tpw;
+        return true;
+    }
+};
+// The address of an element (window, position), in an array with strides n and w in elements of `size` bytes, that goes from
+// tile to tile by additions.
+__device__ __forceinline__ const char* place(const Rows& k, const Tiles& at, const void* base, int64_t n, int64_t w, int64_t size, int64_t ahead) {
+    return (const char*)base + (at.r / k.tpw * n + ((int64_t)at.t * TILE + ahead) * w) * size;
+}
+__device__ __forceinline__ void walk(const Rows& k, const char*& p, bool wrapped, int64_t n, int64_t w, int64_t size) {
+    p += (k.stride_n * n + (int64_t)k.stride_t * TILE * w) * size;
+    if (wrapped) p += (n - k.tpw * TILE * w) * size;
+}
+// The targets of a tile's rows, a lane each (-1: not counted).
+struct Targets {
+    Tiles at;
+    const char *tok, *mask;
+    __device__ __forceinline__ Targets(const Rows& k, int lane)
+        : at(k), tok(place(k, at, k.b.tokens, k.b.tokens_n, k.b.tokens_w, k.b.token_bytes, lane + (int64_t)k.b.shift)),
+          mask(place(k, at, k.b.mask, k.b.mask_n, k.b.mask_w, k.b.mask_bytes, lane + (int64_t)k.b.shift)) {}
+    __device__ __forceinline__ int get(const Rows& k, int lane) const {
+        if (!at.live(k) || (int64_t)at.t * TILE + lane + k.b.shift >= k.b.W) return -1;
+        const int64_t y = k.b.token_bytes == 1 ? *(const uint8_t*)tok : *(const int64_t*)tok;
+        bool on = true;
+        if (k.b.mask_bytes == 1) on = *(const uint8_t*)mask != 0;
+        else if (k.b.mask_bytes == 4) on = *(const float*)mask != 0.f;
+        return !on || y < 0 || y >= k.b.V || y == k.b.ignore ? -1 : (int)y;
+    }
+    __device__ __forceinline__ void next(const Rows& k) {
+        const bool w = at.next(k);
+        walk(k, tok, w, k.b.tokens_n, k.b.tokens_w, k.b.token_bytes);
+        if (k.b.mask_bytes) walk(k, mask, w, k.b.mask_n, k.b.mask_w, k.b.mask_bytes);
+    }
+};
+// What their ends read, a lane each.
+template <int MODE>
+struct Ends {
+    const char *a, *old, *ref;
+    __device__ __forceinline__ Ends(const Rows& k, const Tiles& at, int lane) : a(nullptr), old(nullptr), ref(nullptr) {
+        if (MODE == GRAD) a = place(k, at, k.up, k.up_n, k.up_w, 4, lane);
+        if (MODE == POLICY) {
+            a = place(k, at, k.a.adv, k.a.adv_n, k.a.adv_w, 4, lane);
+            old = place(k, at, k.a.old, k.a.old_n, k.a.old_w, 4, lane);
+            ref = place(k, at, k.a.ref, k.a.ref_n, k.a.ref_w, 4, lane);
+        }
+    }
+    __device__ __forceinline__ End get(const Rows& k, bool row) const {
+        End e = {0.f, 0.f, 0.f};
+        if (MODE == LOGP || !row) return e;
+        e.a = *(const float*)a;
+        if (MODE == POLICY) {
+            e.old = *(const float*)old;
+            if (k.a.ref) e.ref = *(const float*)ref;
+        }
+        return e;
+    }
+    __device__ __forceinline__ void next(const Rows& k, bool wrapped) {
+        if (MODE == GRAD) walk(k, a, wrapped, k.up_n, k.up_w, 4);
+        if (MODE == POLICY) {
+            walk(k, a, wrapped, k.a.adv_n, k.a.adv_w, 4);
+            walk(k, old, wrapped, k.a.old_n, k.a.old_w, 4);
+            if (k.a.ref) walk(k, ref, wrapped, k.a.ref_n, k.a.ref_w, 4);
+        }
     }
 };
 
@@ -362,21 +431,19 @@ __device__ __noinline__ float sum_far(const uint4* raw, int step, float by, floa
 // ---------------------------------------------------------------- rows of up to 256 pieces: G lanes a row, NV pieces a lane
 // A warp takes tiles of 32 rows, 32 / G at a step. Its rows come through a ring of S steps of its own in shared memory: every
 // lane copies its own pieces in and reads them once, into registers, where the row stays until its gradient is out. A step's
-// copy follows S - 1 groups behind its use. The targets of the tile being copied are loaded a tile ahead of it, those and the
-// arguments of the tile being worked on a tile ahead of that, so neither is waited for. The target's logit is read out of
+// copy goes S - 1 groups ahead of its use. The targets of a tile are loaded a tile ahead of its copies and wait with them in
+// the ring; the arguments of its rows are loaded before the first of them is waited for. The target's logit is read out of
 // the ring and -inf put in its place: the sum of the others and their maximum follow without a comparison an element.
 //
-// On a B200, 524,288 rows of 128 bf16 words: log-probabilities 35 us (3.8 TB/s), policy loss and gradient 56 us (4.8 TB/s
+// On a B200, 524,288 rows of 128 bf16 words: log-probabilities 35 us (3.8 TB/s), policy loss and gradient 54 us (5.0 TB/s
 // read and written). Bound by instructions: a step has about 250 of its own (targets, addresses, shuffles, the row's end)
 // beside 4 a word, so 32 words a lane is little; 64 words, half the lanes, lose more by the warps that no longer fit (1,048,576
 // rows: 146 us, and 112 us with 32). Three blocks a multiprocessor for log-probabilities (64 us, two 69), two where the
 // numerators are kept for the gradient (112 us, three spill: 153).
-constexpr int TILE = 32, WARPS = 8;
-
 // A: rows of whole pieces, logits' and gradient's alike. Else (G 16 or more) the elements before a row's first whole piece and
 // behind its last are held by a lane each, as the rows start anywhere.
 template <typename T, int G, int NV, int S, int MODE, bool A>
-__global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP) ? 3 : 2) rows_group_kernel(Rows k) {
+__global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE == LOGP) ? 3 : 2) rows_group_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G;
     static_assert(A || G >= 16, "a lane for each element at a row's ends");
     extern __shared__ uint4 rings[];                         // [WARPS][S][NV][32]
@@ -389,25 +456,21 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
 #pragma unroll
     for (int s = 0; s < S * NV; s++) ring[s * 32 + lane] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
 
-    const int64_t W = k.b.W, tiles = k.b.n * k.tpw, stride = (int64_t)gridDim.x * WARPS, si = stride / k.tpw, st = stride - si * k.tpw;
-    const int64_t first = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const auto target_of = [&](const Pos& p) { return p.r < tiles && p.t * TILE + lane < W ? target(k.b, p.i, p.t * TILE + lane) : -1; };
-    const auto end_of = [&](const Pos& p, int y) {
-        const End none = {0.f, 0.f, 0.f};
-        return y >= 0 ? end_args<MODE>(k, p.i, p.t * TILE + lane) : none;
-    };
-    // the first row of this lane's group in a tile, and from it on a step's rows at a time
-    const auto x_of = [&](const Pos& p) { return (const T*)k.b.logits + p.i * k.b.logits_n + (p.t * TILE + grp) * k.b.logits_w; };
-    const int64_t x_step = RP * k.b.logits_w, d_step = RP * k.b.grad_w;
+    int* const ys = (int*)(rings + WARPS * S * NV * 32) + (threadIdx.x >> 5) * (S * 32);      // [WARPS][S][32]: the steps' targets
 
+    const int64_t x_step = RP * k.b.logits_w, d_step = RP * k.b.grad_w;
     // the tile being copied, its targets, and those of the one after it
-    Pos in(first, k.tpw), in_next = in;
-    in_next.next(stride, si, st, k.tpw);
-    int in_y = target_of(in), in_y_next = target_of(in_next), in_s = 0, in_slot = 0;
-    const T* in_x = x_of(in);
+    Tiles in(k);
+    const char* in_at = place(k, in, k.b.logits, k.b.logits_n, k.b.logits_w, sizeof(T), grp);
+    const T* in_x = (const T*)in_at;                         // of this lane's group, a step's rows on at a time
+    Targets look(k, lane);
+    int in_y = look.get(k, lane), in_s = 0, in_slot = 0;
+    look.next(k);
+    int in_y_next = look.get(k, lane);
     const auto copy_next = [&]() {
-        if (in.r < tiles) {
+        if (in.live(k)) {
             const int y = __shfl_sync(~0u, in_y, in_s * RP + grp);
+            if (sub == 0) ys[in_slot * 32 + grp] = y;
             if (y >= 0) {
                 const int head = A ? 0 : head_of(in_x, V), n = (V - head) / K;
                 const uint32_t to = ring_at + in_slot * (NV * 512);
@@ -418,11 +481,11 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
             in_x += x_step;
             if (++in_s == G) {
                 in_s = 0;
-                in = in_next;
                 in_y = in_y_next;
-                in_next.next(stride, si, st, k.tpw);
-                in_y_next = target_of(in_next);
-                in_x = x_of(in);
+                walk(k, in_at, in.next(k), k.b.logits_n, k.b.logits_w, sizeof(T));
+                in_x = (const T*)in_at;
+                look.next(k);
+                in_y_next = look.get(k, lane);
             }
         }
         if (++in_slot == S) in_slot = 0;
@@ -432,25 +495,27 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
     for (int s = 0; s < S; s++) copy_next();
 
     int slot = 0;
-    Pos p(first, k.tpw);
-    int y_l = target_of(p);
-    End end_l = end_of(p, y_l);
-    while (p.r < tiles) {
-        const int64_t tile = p.r, i = p.i, t0 = p.t * TILE;
-        const T* x = x_of(p);
-        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + (t0 + grp) * k.b.grad_w : nullptr;
-        p.next(stride, si, st, k.tpw);
-        const int y_next = target_of(p);
-        const End end_next = end_of(p, y_next);
-        const int rows = (int)min((int64_t)TILE, W - t0);
+    Tiles p(k);
+    int64_t i = p.r / k.tpw;                                 // its window
+    const char* x_at = A ? nullptr : place(k, p, k.b.logits, k.b.logits_n, k.b.logits_w, sizeof(T), grp);
+    const char* d_at = MODE == LOGP ? nullptr : place(k, p, k.b.grad, k.b.grad_n, k.b.grad_w, sizeof(T), grp);
+    Ends<MODE> ends(k, p, lane);
+    while (p.live(k)) {
+        const T* x = (const T*)x_at;
+        T* d = MODE != LOGP && k.b.grad ? (T*)d_at : nullptr;
+        const int rows = (int)min((int64_t)TILE, k.b.W - (int64_t)p.t * TILE);
+        const End end_l = ends.get(k, lane < rows);
         const double w = weight_of<MODE>(k, i);
         const float wf = (float)w;
         double sum = 0;
         // LOGP: the row of this lane's number in the tile, its maximum, others' sum, target's exponent and numerator
         float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
+        int my_y = -1;
 #pragma unroll 1
         for (int s = 0; s < G; s++) {
-            const int row = s * RP + grp, y = __shfl_sync(~0u, y_l, row);
+            copies_wait<S - 1>();
+            __syncwarp();
+            const int row = s * RP + grp, y = ys[slot * 32 + grp];
             const int head = A ? 0 : head_of(x, V), n = (V - head) / K, tail = head + n * K;
             int edge = -1;
             float ex = -INFINITY;
@@ -460,8 +525,6 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
             }
             uint4* const base = ring + slot * (NV * 32);
             uint4* const own = base + lane;
-            copies_wait<S - 1>();
-            __syncwarp();
             const bool in_piece = A || (y >= head && y < tail);
             const unsigned place = in_piece ? (unsigned)(max(y, 0) - head) : 0u, piece = place / K;
             T* const at = (T*)(base + piece / G * 32 + grp * G + piece % G) + place % K;
@@ -520,7 +583,8 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
             if constexpr (MODE == LOGP) {
                 const int from = lane % RP * G;
                 const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, t, from), g = __shfl_sync(~0u, et, from);
-                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; }
+                const int h = __shfl_sync(~0u, y, from);
+                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; my_y = h; }
             } else {
                 const End end = {__shfl_sync(~0u, end_l.a, row), MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
                                  MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
@@ -545,19 +609,22 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
                 }
                 if (d) d += d_step;
             }
-            x += x_step;
+            if (!A) x += x_step;
         }
         if (MODE == LOGP) {
-            const float lp = y_l >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
+            const float lp = my_y >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
             sum = (double)lp;
-            if (k.logp && lane < rows) k.logp[i * W + t0 + lane] = lp;
+            if (k.logp && lane < rows) k.logp[i * k.b.W + (int64_t)p.t * TILE + lane] = lp;
         }
         if (k.part) {
             sum = warp_sum(sum);
-            if (lane == 0) k.part[tile] = sum * w;
+            if (lane == 0) k.part[p.r] = sum * w;
         }
-        y_l = y_next;
-        end_l = end_next;
+        const bool wrapped = p.next(k);
+        ends.next(k, wrapped);
+        i += k.stride_n + wrapped;
+        if (!A) walk(k, x_at, wrapped, k.b.logits_n, k.b.logits_w, sizeof(T));
+        if (MODE != LOGP) walk(k, d_at, wrapped, k.b.grad_n, k.b.grad_w, sizeof(T));
     }
     copies_wait<0>();
 }
@@ -568,8 +635,8 @@ __global__ void __launch_bounds__(WARPS * 32, NV < 4 || (NV == 4 && MODE == LOGP
 // lane by lane; of a first or last word that it shares with its neighbour it masks the half that is not its own. The gradient
 // replaces the logits in the image and leaves as the stretch came.
 //
-// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 21 us, policy loss and gradient 31 us, bound by the work of a
-// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 57 and 104 us, bound by
+// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 20 us, policy loss and gradient 34 us, bound by the work of a
+// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 57 and 100 us, bound by
 // instructions as the rows above, with a load and a mask a word more.
 template <typename T> __device__ __forceinline__ float word_max(uint32_t a, float m);
 template <> __device__ __forceinline__ float word_max<float>(uint32_t a, float m) { return fmaxf(m, __uint_as_float(a)); }
@@ -583,7 +650,7 @@ template <> __device__ __forceinline__ float word_max<__half>(uint32_t a, float 
 
 // NW: words a lane
 template <typename T, int G, int NW, int S, int MODE>
-__global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) rows_flat_kernel(Rows k) {
+__global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && NW < 16) ? 3 : 2) rows_flat_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G, E = 4 / (int)sizeof(T), N = (NW * E + 1) / 2 * 2;      // E: elements a word
     constexpr int SLOT = (NW * 32 * 4 + 47) / 16;            // 16-byte pieces of an image
     extern __shared__ uint4 rings[];                         // [WARPS][S][SLOT]
@@ -593,28 +660,24 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
     uint4* const ring = rings + (threadIdx.x >> 5) * (S * SLOT);
     const uint32_t ring_at = shared_at(ring);
 
-    const int64_t W = k.b.W, tiles = k.b.n * k.tpw, stride = (int64_t)gridDim.x * WARPS, si = stride / k.tpw, st = stride - si * k.tpw;
-    const int64_t first = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const auto target_of = [&](const Pos& p) { return p.r < tiles && p.t * TILE + lane < W ? target(k.b, p.i, p.t * TILE + lane) : -1; };
-    const auto end_of = [&](const Pos& p, int y) {
-        const End none = {0.f, 0.f, 0.f};
-        return y >= 0 ? end_args<MODE>(k, p.i, p.t * TILE + lane) : none;
-    };
-    const auto x_of = [&](const Pos& p) { return (const T*)k.b.logits + p.i * k.b.logits_n + p.t * TILE * V; };
-    const auto rows_of_tile = [&](const Pos& p) { return (int)min((int64_t)TILE, W - p.t * TILE); };
-    constexpr unsigned STEP = RP == 32 ? ~0u : (1u << RP) - 1;
+    int* const ys = (int*)(rings + WARPS * S * SLOT) + (threadIdx.x >> 5) * (S * 32);         // [WARPS][S][32]: the steps' targets
+    const auto rows_of_tile = [&](const Tiles& p) { return (int)min((int64_t)TILE, k.b.W - (int64_t)p.t * TILE); };
     // a step's stretch: how far into its first piece it starts, its elements
     struct Stretch { int off, len; };
     const auto stretch = [&](const T* x, int s, int rows) { return Stretch{row_off(x), max(0, min(RP, rows - s * RP)) * V}; };
 
-    Pos in(first, k.tpw), in_next = in;
-    in_next.next(stride, si, st, k.tpw);
-    unsigned in_on = __ballot_sync(~0u, target_of(in) >= 0);
-    int in_y_next = target_of(in_next), in_s = 0, in_slot = 0;
-    const T* in_x = x_of(in);
+    Tiles in(k);
+    const char* in_at = place(k, in, k.b.logits, k.b.logits_n, V, sizeof(T), 0);
+    const T* in_x = (const T*)in_at;
+    Targets look(k, lane);
+    int in_y = look.get(k, lane), in_s = 0, in_slot = 0;
+    look.next(k);
+    int in_y_next = look.get(k, lane);
     const auto copy_next = [&]() {
-        if (in.r < tiles) {
-            if (in_on >> (in_s * RP) & STEP) {
+        if (in.live(k)) {
+            const int y = __shfl_sync(~0u, in_y, in_s * RP + grp);
+            if (sub == 0) ys[in_slot * 32 + grp] = y;
+            if (__any_sync(~0u, y >= 0)) {
                 const Stretch q = stretch(in_x, in_s, rows_of_tile(in));
                 const uint32_t to = ring_at + in_slot * (SLOT * 16);
                 const T* const from = in_x - q.off;
@@ -623,11 +686,11 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
             in_x += RP * V;
             if (++in_s == G) {
                 in_s = 0;
-                in = in_next;
-                in_on = __ballot_sync(~0u, in_y_next >= 0);
-                in_next.next(stride, si, st, k.tpw);
-                in_y_next = target_of(in_next);
-                in_x = x_of(in);
+                in_y = in_y_next;
+                walk(k, in_at, in.next(k), k.b.logits_n, V, sizeof(T));
+                in_x = (const T*)in_at;
+                look.next(k);
+                in_y_next = look.get(k, lane);
             }
         }
         if (++in_slot == S) in_slot = 0;
@@ -637,26 +700,28 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
     for (int s = 0; s < S; s++) copy_next();
 
     int slot = 0;
-    Pos p(first, k.tpw);
-    int y_l = target_of(p);
-    End end_l = end_of(p, y_l);
-    while (p.r < tiles) {
-        const int64_t tile = p.r, i = p.i, t0 = p.t * TILE;
-        const T* x = x_of(p);
-        T* d = k.b.grad ? (T*)k.b.grad + i * k.b.grad_n + t0 * V : nullptr;
+    Tiles p(k);
+    int64_t i = p.r / k.tpw;                                 // its window
+    const char* x_at = place(k, p, k.b.logits, k.b.logits_n, V, sizeof(T), 0);
+    const char* d_at = MODE == LOGP ? nullptr : place(k, p, k.b.grad, k.b.grad_n, V, sizeof(T), 0);
+    Ends<MODE> ends(k, p, lane);
+    while (p.live(k)) {
+        const T* x = (const T*)x_at;
+        T* d = MODE != LOGP && k.b.grad ? (T*)d_at : nullptr;
         const int rows = rows_of_tile(p);
-        p.next(stride, si, st, k.tpw);
-        const int y_next = target_of(p);
-        const End end_next = end_of(p, y_next);
+        const End end_l = ends.get(k, lane < rows);
         const double w = weight_of<MODE>(k, i);
-        const unsigned on = __ballot_sync(~0u, y_l >= 0);
+        const float wf = (float)w;
         double sum = 0;
         float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
+        int my_y = -1;
 #pragma unroll 1
         for (int s = 0; s < G; s++, x += RP * V) {
-            const int row = s * RP + grp, y = __shfl_sync(~0u, y_l, row);
+            copies_wait<S - 1>();
+            __syncwarp();
+            const int row = s * RP + grp, y = ys[slot * 32 + grp];
             const Stretch q = stretch(x, s, rows);
-            const bool any = on >> (s * RP) & STEP;
+            const bool any = __any_sync(~0u, y >= 0);
             uint4* const base = ring + slot * SLOT;
             T* const img = (T*)base;
             // the stretch's elements before its first whole piece and behind its last
@@ -664,7 +729,6 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
             const int edge = lane < 8 ? (lane < head ? lane : -1) : lane < 16 && tail + lane - 8 < q.len ? tail + lane - 8 : -1;
             T ev = lowest<T>();
             if (any && edge >= 0) ev = x[edge];
-            copies_wait<S - 1>();
             if (edge >= 0) img[q.off + edge] = ev;
             __syncwarp();
             const int at = q.off + grp * V, w0 = at / E, w1 = (at + V - 1) / E, ty = at + max(y, 0);
@@ -705,13 +769,14 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
             if constexpr (MODE == LOGP) {
                 const int from = lane % RP * G;
                 const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, t, from), g = __shfl_sync(~0u, et, from);
-                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; }
+                const int h = __shfl_sync(~0u, y, from);
+                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; my_y = h; }
             } else {
                 const End end = {__shfl_sync(~0u, end_l.a, row), MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
                                  MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
                 float g = 0.f, term = 0.f;
                 if (y >= 0) {
-                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, (float)w, scale, term);
+                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, wf, scale, term);
                     if (MODE == POLICY && sub == 0) sum += (double)term;
                 }
                 if (d) {
@@ -744,16 +809,19 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || NW < 16 ? 3 : 2) r
             if (++slot == S) slot = 0;
         }
         if (MODE == LOGP) {
-            const float lp = y_l >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
+            const float lp = my_y >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
             sum = (double)lp;
-            if (k.logp && lane < rows) k.logp[i * W + t0 + lane] = lp;
+            if (k.logp && lane < rows) k.logp[i * k.b.W + (int64_t)p.t * TILE + lane] = lp;
         }
         if (k.part) {
             sum = warp_sum(sum);
-            if (lane == 0) k.part[tile] = sum * w;
+            if (lane == 0) k.part[p.r] = sum * w;
         }
-        y_l = y_next;
-        end_l = end_next;
+        const bool wrapped = p.next(k);
+        ends.next(k, wrapped);
+        i += k.stride_n + wrapped;
+        walk(k, x_at, wrapped, k.b.logits_n, V, sizeof(T));
+        if (MODE != LOGP) walk(k, d_at, wrapped, k.b.grad_n, V, sizeof(T));
     }
     copies_wait<0>();
 }
@@ -888,7 +956,7 @@ __device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V
 // distributed shared memory, behind one cluster barrier a row.
 //
 // On a B200: log-probabilities of 32,768 rows of 16,384 bf16 words 199 us (5.4 TB/s), their gradient from kept statistics 353
-// us (6.1 TB/s, read and written): bound by memory. The policy loss and gradient of 16,384 rows of 65,541 words 889 us (4.8
+// us (6.1 TB/s, read and written): bound by memory. The policy loss and gradient of 16,384 rows of 65,541 words 893 us (4.8
 // TB/s): two 2^x and some 15 instructions a word at 24 warps a multiprocessor, which wait on each other at a row's end.
 // Threads a row, the fewest that hold it, since each warp pays a row's overhead (16,380 rows of 4,101 words: 68 us with
 // 32 threads, 85 with 64, 102 with 128; 8,192 of 16,384: 104 us with 128, 132 with 256). Pieces kept in registers between the
@@ -1379,14 +1447,21 @@ int allow_smem(const void* f, int bytes, uint64_t& set) {
     return bytes;
 }
 
+Rows by_tiles(Rows k, unsigned grid) {
+    k.stride = (int64_t)grid * WARPS;
+    k.stride_n = k.stride / k.tpw;
+    k.stride_t = (int32_t)(k.stride % k.tpw);
+    return k;
+}
 template <typename T, int G, int NV, int MODE, bool A>
 void group_rows(const Rows& k, cudaStream_t st) {
-    constexpr int S = NV <= 4 ? 3 : 2, SMEM = WARPS * S * NV * 512;
+    constexpr int S = NV <= 4 ? 3 : 2, SMEM = WARPS * S * (NV * 512 + 128);
     const auto f = rows_group_kernel<T, G, NV, S, MODE, A>;
     static thread_local uint64_t set = 0;
     allow_smem((const void*)f, SMEM, set);
     static const unsigned most = grid_of(f, WARPS * 32, SMEM, 1 << 20);
-    f<<<(unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most), WARPS * 32, SMEM, st>>>(k);
+    const unsigned grid = (unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most);
+    f<<<grid, WARPS * 32, SMEM, st>>>(by_tiles(k, grid));
 }
 
 template <typename T, int THREADS, int U, int S, int C, int MODE>
@@ -1413,12 +1488,13 @@ void ring_rows(const Rows& k, int pieces, cudaStream_t st) {
 
 template <typename T, int G, int NW, int MODE>
 void flat_rows(const Rows& k, cudaStream_t st) {
-    constexpr int S = 3, SMEM = WARPS * S * ((NW * 32 * 4 + 47) / 16) * 16;
+    constexpr int S = 3, SMEM = WARPS * S * (((NW * 32 * 4 + 47) / 16) * 16 + 128);
     const auto f = rows_flat_kernel<T, G, NW, S, MODE>;
     static thread_local uint64_t set = 0;
     allow_smem((const void*)f, SMEM, set);
     static const unsigned most = grid_of(f, WARPS * 32, SMEM, 1 << 20);
-    f<<<(unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most), WARPS * 32, SMEM, st>>>(k);
+    const unsigned grid = (unsigned)std::min<int64_t>((k.b.n * k.tpw + WARPS - 1) / WARPS, most);
+    f<<<grid, WARPS * 32, SMEM, st>>>(by_tiles(k, grid));
 }
 
 template <typename T, int MODE>
