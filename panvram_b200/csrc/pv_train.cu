@@ -8,7 +8,7 @@
 // overflows at the lowest or highest value of bf16 and fp32) the difference comes first: e_j = 2^((x_j - max) L).
 // The sum o over the other words is kept apart from the target's numerator e: 1 - p_y = o / (o + e) and, where e >= o,
 // log p_y = -log1p(o / e), so neither loses its digits where the model is nearly sure.
-// All statistics are in 32 bits; sums over rows are in 64 bits and in a fixed order (a partial sum per tile of rows, then
+// A row's statistics are in 32 bits, its log-probability and the differences taken of it in 64; sums over rows are in 64 bits and in a fixed order (a partial sum per tile of rows, then
 // over the tiles), so results do not change from call to call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,7 +27,7 @@ namespace {
 
 using pvb::g_cuda_err;
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int SMS = 148;
 
 // ---------------------------------------------------------------- elements
@@ -138,12 +138,18 @@ __device__ __forceinline__ void times(float (&x)[K], float f) {
     }
 }
 
-// log p of the target: t its exponent, e its numerator, o the sum of the others', m the maximum. Where the target does not
-// outweigh the others the sum is about 1 or more, and log1p of what it is above 1 is its logarithm.
-__device__ __forceinline__ float row_logp(float m, float o, float t, float e) {
+// log p of the target: x its logit, e its numerator, o the sum of the others', m the maximum (or the reference's). Where it
+// does not outweigh the others, s = o + e = 2^k g with g from 0.7 to 1.4: log p = (x log2 e - c - k) ln 2 - log g, of which
+// only the last is rounded to 32 bits, as its size is small beside log p's.
+__device__ __forceinline__ double row_logp(float m, float o, float x, float e) {
     const bool sure = e >= o;
-    const float l = log1pf(sure ? o * reciprocal(e) : (o + e) - 1.f);
-    return m == -INFINITY ? NAN : (sure ? 0.f : t * LN2) - l;            // -inf: nothing to normalise by
+    const float s = o + e;
+    const int b = __float_as_int(s), k = (b - 0x3F350000) >> 23;                 // 0.707 as bits
+    const float l = log1pf(sure ? o * reciprocal(e) : __int_as_float(b - (k << 23)) - 1.f);
+    if (m == -INFINITY || !(s < INFINITY)) return NAN;                           // nothing to normalise by, or not a number
+    if (sure) return -(double)l;
+    const double t = far(m) ? ((double)x - (double)m) * 1.4426950408889634 : (double)x * (double)LOG2E - (double)ref_of(m);
+    return (t - (double)k) * 0.6931471805599453 - (double)l - 4e-8;
 }
 
 // exp(d) - 1 and exp(d) - d - 1, near 0 by the series of the latter, where the differences would lose their digits
@@ -174,10 +180,10 @@ __device__ __forceinline__ End end_args(const Rows& k, int64_t i, int64_t t) {
 // From a counted row's log-probability its term of the sum (before the window's weight w) and its derivative, times w and
 // the upstream scale (the result).
 template <int MODE>
-__device__ __forceinline__ float row_end(const Rows& k, const End& e, float lp, float w, float scale, float& term) {
-    if (MODE == LOGP) { term = lp; return 0.f; }
+__device__ __forceinline__ float row_end(const Rows& k, const End& e, double lp, float w, float scale, float& term) {
+    if (MODE == LOGP) { term = (float)lp; return 0.f; }
     if (MODE == GRAD) { term = 0.f; return e.a * scale; }
-    const float r = expf(lp - e.old);
+    const float r = expf((float)(lp - (double)e.old));        // the difference in 64 bits: it is small beside its terms
     const float one = e.a == 0.f ? 0.f : r * e.a;
     const float two = fminf(fmaxf(r, 1.f - k.a.clip_low), 1.f + k.a.clip_high) * e.a;
     const bool free = !(one > two);                          // NaN stays
@@ -185,7 +191,7 @@ __device__ __forceinline__ float row_end(const Rows& k, const End& e, float lp, 
     term = free ? -one : -two;
     if (k.a.ref) {
         float em1, kl;
-        kl_terms(e.ref - lp, em1, kl);
+        kl_terms((float)((double)e.ref - lp), em1, kl);
         term += k.a.kl * kl;
         g -= k.a.kl * em1;
     }
@@ -508,8 +514,8 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE 
         const double w = weight_of<MODE>(k, i);
         const float wf = (float)w;
         double sum = 0;
-        // LOGP: the row of this lane's number in the tile, its maximum, others' sum, target's exponent and numerator
-        float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
+        // LOGP: the row of this lane's number in the tile, its maximum, others' sum, target's logit and numerator
+        float my_m = 0.f, my_o = 0.f, my_x = 0.f, my_e = 0.f;
         int my_y = -1;
 #pragma unroll 1
         for (int s = 0; s < G; s++) {
@@ -549,7 +555,7 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE 
 #pragma unroll
             for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
             m = fmaxf(m, xt);
-            const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
+            const float c = ref_of(m), et = ex2(exponent(xt, m, c));
             const bool any_far = __any_sync(~0u, far(m));
             float e[MODE == LOGP ? 1 : NV][K], o = 0.f;
             if constexpr (MODE == LOGP) {
@@ -582,15 +588,15 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE 
             for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
             if constexpr (MODE == LOGP) {
                 const int from = lane % RP * G;
-                const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, t, from), g = __shfl_sync(~0u, et, from);
+                const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, xt, from), g = __shfl_sync(~0u, et, from);
                 const int h = __shfl_sync(~0u, y, from);
-                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; my_y = h; }
+                if (lane / RP == s) { my_m = a; my_o = b; my_x = f; my_e = g; my_y = h; }
             } else {
                 const End end = {__shfl_sync(~0u, end_l.a, row), MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
                                  MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
                 float g = 0.f, term = 0.f;
                 if (y >= 0) {
-                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, wf, scale, term);
+                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, xt, et) : 0.0, wf, scale, term);
                     if (MODE == POLICY && sub == 0) sum += (double)term;
                 }
                 const bool some_off = __any_sync(~0u, y < 0);
@@ -612,9 +618,9 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE 
             if (!A) x += x_step;
         }
         if (MODE == LOGP) {
-            const float lp = my_y >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
-            sum = (double)lp;
-            if (k.logp && lane < rows) k.logp[i * k.b.W + (int64_t)p.t * TILE + lane] = lp;
+            const double lp = my_y >= 0 ? row_logp(my_m, my_o, my_x, my_e) : 0.0;
+            sum = lp;
+            if (k.logp && lane < rows) k.logp[i * k.b.W + (int64_t)p.t * TILE + lane] = (float)lp;
         }
         if (k.part) {
             sum = warp_sum(sum);
@@ -713,7 +719,7 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && N
         const double w = weight_of<MODE>(k, i);
         const float wf = (float)w;
         double sum = 0;
-        float my_m = 0.f, my_o = 0.f, my_t = 0.f, my_e = 0.f;
+        float my_m = 0.f, my_o = 0.f, my_x = 0.f, my_e = 0.f;
         int my_y = -1;
 #pragma unroll 1
         for (int s = 0; s < G; s++, x += RP * V) {
@@ -753,7 +759,7 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && N
             }
 #pragma unroll
             for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
-            const float c = ref_of(m), t = exponent(xt, m, c), et = ex2(t);
+            const float c = ref_of(m), et = ex2(exponent(xt, m, c));
             float e[N];
             e[N - 1] = -INFINITY;
 #pragma unroll
@@ -768,15 +774,15 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && N
             for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
             if constexpr (MODE == LOGP) {
                 const int from = lane % RP * G;
-                const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, t, from), g = __shfl_sync(~0u, et, from);
+                const float a = __shfl_sync(~0u, m, from), b = __shfl_sync(~0u, o, from), f = __shfl_sync(~0u, xt, from), g = __shfl_sync(~0u, et, from);
                 const int h = __shfl_sync(~0u, y, from);
-                if (lane / RP == s) { my_m = a; my_o = b; my_t = f; my_e = g; my_y = h; }
+                if (lane / RP == s) { my_m = a; my_o = b; my_x = f; my_e = g; my_y = h; }
             } else {
                 const End end = {__shfl_sync(~0u, end_l.a, row), MODE == POLICY ? __shfl_sync(~0u, end_l.old, row) : 0.f,
                                  MODE == POLICY ? __shfl_sync(~0u, end_l.ref, row) : 0.f};
                 float g = 0.f, term = 0.f;
                 if (y >= 0) {
-                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, t, et) : 0.f, wf, scale, term);
+                    g = row_end<MODE>(k, end, MODE == POLICY ? row_logp(m, o, xt, et) : 0.0, wf, scale, term);
                     if (MODE == POLICY && sub == 0) sum += (double)term;
                 }
                 if (d) {
@@ -809,9 +815,9 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && N
             if (++slot == S) slot = 0;
         }
         if (MODE == LOGP) {
-            const float lp = my_y >= 0 ? row_logp(my_m, my_o, my_t, my_e) : 0.f;
-            sum = (double)lp;
-            if (k.logp && lane < rows) k.logp[i * k.b.W + (int64_t)p.t * TILE + lane] = lp;
+            const double lp = my_y >= 0 ? row_logp(my_m, my_o, my_x, my_e) : 0.0;
+            sum = lp;
+            if (k.logp && lane < rows) k.logp[i * k.b.W + (int64_t)p.t * TILE + lane] = (float)lp;
         }
         if (k.part) {
             sum = warp_sum(sum);
@@ -901,16 +907,17 @@ __device__ __forceinline__ float4 block_end(const Rows& k, Meeting<NW * C>& at, 
         }
         const float xt = at.xt[turn];
         if (xt > all.m) { all.o *= rescale(all.m, xt); all.m = xt; }       // the sums leave the target out
-        const float c = ref_of(all.m), t = exponent(xt, all.m, c), e = ex2(t);
+        const float c = ref_of(all.m), e = ex2(exponent(xt, all.m, c));
         float term;
-        const float lp = row_logp(all.m, all.o, t, e), g = row_end<MODE>(k, end, lp, (float)w, scale, term);
+        const double lp = row_logp(all.m, all.o, xt, e);
+        const float g = row_end<MODE>(k, end, lp, (float)w, scale, term);
         const float inv = reciprocal(all.o + e);
         if (lane == 0) {
             if (rank == 0) {
-                if (MODE == LOGP && k.logp) k.logp[r] = lp;
+                if (MODE == LOGP && k.logp) k.logp[r] = (float)lp;
                 if (k.stat) k.stat[r] = make_float4(all.m, c, inv, all.o * inv);
                 if (MODE == POLICY && k.deriv) k.deriv[r] = g;
-                if (k.part) k.part[r] = (double)term * w;
+                if (k.part) k.part[r] = MODE == LOGP ? lp : (double)term * w;
             }
             if (grad) at.grad[turn] = make_float4(all.m, c, -g * inv, g * (all.o * inv));
         }
