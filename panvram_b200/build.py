@@ -1,5 +1,6 @@
 """Build panvram_b200's native library in-tree: panvram_b200/libpanvram_b200.so (the C ABI of
-include/panvram_b200.h) from csrc/pv_host.cpp (host reader, pooling) and csrc/pv_kernels.cu (sm_100a kernels).
+include/panvram_b200.h) from csrc/pv_host.cpp (host reader, pooling) and the csrc/*.cu (sm_100a kernels), and
+panvram_b200/_train.so, torch's view of the training step's operators (torch_ext/pv_torch.cpp), which calls it.
 
     python panvram_b200/build.py [--force] [--ptxas-info]
 
@@ -9,6 +10,7 @@ import argparse
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -16,6 +18,7 @@ CSRC = os.path.join(PKG, "csrc")
 INC = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build", "panvram_b200")
 LIB = os.path.join(PKG, "libpanvram_b200.so")
+TRAIN_LIB = os.path.join(PKG, "_train.so")
 SYNTH_LIB = os.path.join(PKG, "synth", "libpvsynth.so")
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 LIBDIR = "/usr/lib/x86_64-linux-gnu"
@@ -57,6 +60,18 @@ def build(force=False, verbose=False, ptxas_info=False):
     if force or _stale(LIB, objs):
         _run(["g++", "-shared", "-o", LIB, *objs, "-L" + os.path.join(CUDA, "lib64"), "-lcudart_static", "-ldl", "-lrt", "-lpthread",
               os.path.join(LIBDIR, "libzstd.so.1"), os.path.join(LIBDIR, "libxxhash.so.0"), os.path.join(LIBDIR, "libcrypto.so.3")], verbose)
+    # built against the torch that runs this (its C++ interface is bound to its version): the object's name says which
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(PKG, "torch_ext", "pv_torch.cpp")
+    obj = os.path.join(BUILD, f"pv_torch-{torch.__version__}.o")
+    if force or _stale(obj, [src] + HEADERS):
+        inc = [INC, *cpp_extension.include_paths(), os.path.join(CUDA, "include"), sysconfig.get_paths()["include"]]
+        log += _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", *(f for i in inc for f in ("-isystem", i)),
+                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-c", src, "-o", obj], verbose)
+    if force or _stale(TRAIN_LIB, [obj, LIB]):
+        _run(["g++", "-shared", "-o", TRAIN_LIB, obj, "-L" + PKG, "-lpanvram_b200", "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+              "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
     # the cohort synthesizer (test and benchmark data; not linked into the decode library)
     src = os.path.join(PKG, "synth", "pv_synth.cpp")
     if force or _stale(SYNTH_LIB, [src] + HEADERS):

@@ -184,3 +184,16 @@ def test_parameters_are_refused_and_no_grad_parameters_work(P, cuda):
         P.clip_grads([p], 1.0)
     (p * 3).sum().backward()
     assert float(P.clip_grads([p.grad], 1.0)) == pytest.approx(3 * math.sqrt(5), rel=5 * E32)
+
+
+def test_a_clipped_tensor_counts_as_changed(P, cuda):
+    """autograd refuses a saved tensor that clipping has written since"""
+    a, w = torch.ones(4, device=cuda), torch.ones(4, device=cuda, requires_grad=True)
+    y = (a * w).sum()
+    P.clip_grads([a], 0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        b = torch.ones(4, device=cuda)
+        P.clip_grads([b], 1.0)
+        assert b.max() < 0.51

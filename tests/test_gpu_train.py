@@ -160,7 +160,7 @@ def test_unaligned_base_leaves_neighbours_alone(P, cuda, V, off):
     """logits that start anywhere in a buffer whose other values are NaN; the gradient written by the C entry point into
     a buffer of its own, whose other values stay"""
     import ctypes
-    from panvram_b200 import _C, train
+    from panvram_b200 import _C
     for kind in TYPES:
         n, W = 2, 9
         x, t, _ = make(cuda, n, W, V, kind, "ids")
@@ -173,11 +173,14 @@ def test_unaligned_base_leaves_neighbours_alone(P, cuda, V, off):
         for goff in (off, 0, 4):
             gbuf = torch.full((n * W * V + 64,), 7.0, dtype=x.dtype, device=cuda)
             d = gbuf[goff:goff + n * W * V].view(n, W, V)
-            b = train._batch(a, t, None, 1, None)
-            stat = train._logprobs(b, cuda, False, True)[1]
+            st = torch.cuda.current_stream().cuda_stream
+            b = _C.Scored(a.data_ptr(), None, t.data_ptr(), None, n, W, V, *a.stride()[:2], 0, 0, *t.stride(), 0, 0, -100, 1,
+                          list(TYPES).index(kind), 8, 0)
+            stat = torch.empty(_C._lib.pv_score_stat_bytes(ctypes.byref(b)), dtype=torch.uint8, device=cuda)
+            logp = torch.empty(n, W, device=cuda)
+            assert _C._lib.pv_logprobs(ctypes.byref(b), logp.data_ptr(), None, stat.data_ptr() or None, None, 0, st) == 0
             b.grad, b.grad_n, b.grad_w = d.data_ptr(), d.stride(0), d.stride(1)
-            assert _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), W, 1, stat.data_ptr() if stat is not None else None, None,
-                                             torch.cuda.current_stream().cuda_stream) == 0
+            assert _C._lib.pv_logprobs_grad(ctypes.byref(b), up.data_ptr(), W, 1, stat.data_ptr() or None, None, st) == 0
             close(d, *grad_of(x, p, y, ok, up.double()))
             assert (gbuf[:goff] == 7).all() and (gbuf[goff + n * W * V:] == 7).all()
 
@@ -511,6 +514,54 @@ def test_saved_logits_changed_in_place_are_refused(P, cuda):
     y.mul_(2)
     with pytest.raises(RuntimeError, match="inplace"):
         loss.backward()
+
+
+@pytest.mark.parametrize("V", [5, 128, 2045, 2048, 4096, 70000])
+@pytest.mark.parametrize("how", ["host", "unaligned", "recomputed"])
+def test_saved_tensors_brought_back_elsewhere(P, cuda, V, how):
+    """hooks on saved tensors bring the logits, tokens and the rest back in other memory, at another alignment and laid out
+    otherwise; what lay at the old addresses is overwritten meanwhile"""
+    n, W = 4, 6
+    x0, t0, m0 = make(cuda, n, W, V, "bf16", "ids")
+    m0 = (torch.rand(n, W, device=cuda) < 0.8).float() if m0 is None else m0
+    ref = torch.randn(n, device=cuda)
+    adv, old = torch.randn(n, device=cuda), torch.randn(n, W, device=cuda) * 0.1 - 3
+    losses = {"logp": lambda x, t, m, o, a: P.window_logprobs(x, t, mask=m).mul(o).sum(),
+              "pair": lambda x, t, m, o, a: P.preference_loss(x, t, ref, mask=m),
+              "policy": lambda x, t, m, o, a: P.policy_loss(x, t, o, a, o * 0.9, kl=0.1, mask=m)}
+
+    def unaligned(t):
+        if t.numel() == 0:
+            return t
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda)[1:]
+        return buf.view(t.shape).copy_(t)
+    for name, f in losses.items():
+        for up in (1.0, 0.5):
+            leaf = x0.clone().requires_grad_()
+            (f(leaf * 1, t0, m0, old, adv) * up).backward()
+            want = leaf.grad
+            leaf = x0.clone().requires_grad_()
+            fresh = [z.clone() for z in (t0, m0, old, adv)]
+            if how == "recomputed":
+                from torch.utils.checkpoint import checkpoint
+                loss = checkpoint(lambda z, *r: f(z * 1, *r), leaf, *fresh, use_reentrant=False)
+            else:
+                pack = (lambda z: z.cpu()) if how == "host" else (lambda z: z.clone())
+                back = (lambda z: z.to(cuda)) if how == "host" else unaligned
+                with torch.autograd.graph.saved_tensors_hooks(pack, back):
+                    x = leaf * 1
+                    loss = f(x, *fresh)
+                x.detach().fill_(math.nan)
+                for z in fresh:
+                    z.zero_()
+            junk = [torch.full_like(x0, math.nan) for _ in range(4)]
+            (loss * up).backward()
+            del junk
+            # another form of the kernels may have run. Either's log-probabilities are off by run_of(V) < 2^-12, a position's
+            # weight by that times what its terms add up to (their sum may cancel: the absolute part), probabilities by that
+            # again; then each rounds to bf16 once
+            tol = want.float().abs() * (2.0 ** -7 + 2.0 ** -9) + want.float().abs().max() * 2.0 ** -11
+            assert ((leaf.grad.float() - want.float()).abs() <= tol).all(), (name, up)
 
 
 def test_streams_and_graph(P, cuda):

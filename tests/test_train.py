@@ -92,6 +92,14 @@ def test_refusals_of_gradient_lists():
         P.clip_grads([torch.nn.Parameter(A.clone())], 1.0)
 
 
+def test_refusals_of_what_is_no_tensor():
+    for call in (lambda: P.preference_loss(X, T, None), lambda: P.policy_loss(X, T, [0.0], A), lambda: P.policy_loss(X, T, L, 1.0),
+                 lambda: P.policy_loss(X, T, L, A, ref_logp=0.5, kl=0.1), lambda: P.clip_grads([A], 1.0, out=[None]),
+                 lambda: P.grad_norm(["A"]), lambda: P.window_logprobs(X, T, mask=[[1, 1, 1], [1, 1, 1]])):
+        with pytest.raises(ValueError):
+            call()
+
+
 def _scored(**kw):
     b = _C.Scored(64, None, 64, None, 2, 3, 4, 12, 4, 0, 0, 3, 1, 0, 0, 4, 1, 2, 1, 0)
     for k, v in kw.items():
