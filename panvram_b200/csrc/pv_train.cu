@@ -441,15 +441,17 @@ __device__ __noinline__ float sum_far(const uint4* raw, int step, float by, floa
 // the ring; the arguments of its rows are loaded before the first of them is waited for. The target's logit is read out of
 // the ring and -inf put in its place: the sum of the others and their maximum follow without a comparison an element.
 //
-// On a B200, 524,288 rows of 128 bf16 words: log-probabilities 35 us (3.8 TB/s), policy loss and gradient 54 us (5.0 TB/s
+// On a B200, 524,288 rows of 128 bf16 words: log-probabilities 35 us (3.8 TB/s), policy loss and gradient 58 us (4.6 TB/s
 // read and written). Bound by instructions: a step has about 250 of its own (targets, addresses, shuffles, the row's end)
-// beside 4 a word, so 32 words a lane is little; 64 words, half the lanes, lose more by the warps that no longer fit (1,048,576
-// rows: 146 us, and 112 us with 32). Three blocks a multiprocessor for log-probabilities (64 us, two 69), two where the
-// numerators are kept for the gradient (112 us, three spill: 153).
+// beside 4 a word. So lanes hold 32 words (64, half the lanes, lose more by the warps that no longer fit: 1,048,576 rows take
+// 146 us, and 112 with 32), and 3 or 6 pieces where a quarter of 4 or 8 would be empty (131,072 rows of 1,536: 150 us with 6,
+// 179 with 8). Three blocks a multiprocessor for log-probabilities (64 us, two 69), two where the numerators are kept for the
+// gradient (112 us, three spill: 153). A row that starts anywhere costs half as much again (282 words of 4 bytes 180 us, 284
+// aligned ones 136); loading its ends a step ahead does not help (195).
 // A: rows of whole pieces, logits' and gradient's alike. Else (G 16 or more) the elements before a row's first whole piece and
 // behind its last are held by a lane each, as the rows start anywhere.
 template <typename T, int G, int NV, int S, int MODE, bool A>
-__global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE == LOGP) ? 3 : 2) rows_group_kernel(Rows k) {
+__global__ void __launch_bounds__(WARPS * 32, (NV < 3 && A) || ((NV == 3 || NV == 4) && MODE == LOGP) ? 3 : 2) rows_group_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G;
     static_assert(A || G >= 16, "a lane for each element at a row's ends");
     extern __shared__ uint4 rings[];                         // [WARPS][S][NV][32]
@@ -641,8 +643,8 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 4 && A) || (NV == 4 && MODE 
 // lane by lane; of a first or last word that it shares with its neighbour it masks the half that is not its own. The gradient
 // replaces the logits in the image and leaves as the stretch came.
 //
-// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 20 us, policy loss and gradient 34 us, bound by the work of a
-// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 57 and 100 us, bound by
+// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 21 us, policy loss and gradient 37 us, bound by the work of a
+// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 57 and 108 us, bound by
 // instructions as the rows above, with a load and a mask a word more.
 template <typename T> __device__ __forceinline__ float word_max(uint32_t a, float m);
 template <> __device__ __forceinline__ float word_max<float>(uint32_t a, float m) { return fmaxf(m, __uint_as_float(a)); }
@@ -1518,17 +1520,25 @@ void short_rows(const Rows& k, const Plan& p, cudaStream_t st) {
     } else if (!whole) {
         if (p.pieces <= 16) group_rows<T, 16, 1, MODE, false>(k, st);
         else if (p.pieces <= 32) group_rows<T, 16, 2, MODE, false>(k, st);
+        else if (p.pieces <= 48) group_rows<T, 16, 3, MODE, false>(k, st);
         else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, false>(k, st);
+        else if (p.pieces <= 96) group_rows<T, 32, 3, MODE, false>(k, st);
         else if (p.pieces <= 128) group_rows<T, 32, 4, MODE, false>(k, st);
+        else if (p.pieces <= 192) group_rows<T, 32, 6, MODE, false>(k, st);
         else group_rows<T, 32, 8, MODE, false>(k, st);
     } else if (p.pieces <= 1) group_rows<T, 1, 1, MODE, true>(k, st);
     else if (p.pieces <= 2) group_rows<T, 1, 2, MODE, true>(k, st);
     else if (p.pieces <= 4) group_rows<T, 1, 4, MODE, true>(k, st);
     else if (p.pieces <= 8) group_rows<T, 2, 4, MODE, true>(k, st);
+    else if (p.pieces <= 12) group_rows<T, 4, 3, MODE, true>(k, st);
     else if (p.pieces <= 16) group_rows<T, 4, 4, MODE, true>(k, st);
+    else if (p.pieces <= 24) group_rows<T, 8, 3, MODE, true>(k, st);
     else if (p.pieces <= 32) group_rows<T, 8, 4, MODE, true>(k, st);
+    else if (p.pieces <= 48) group_rows<T, 16, 3, MODE, true>(k, st);
     else if (p.pieces <= 64) group_rows<T, 16, 4, MODE, true>(k, st);
+    else if (p.pieces <= 96) group_rows<T, 32, 3, MODE, true>(k, st);
     else if (p.pieces <= 128) group_rows<T, 32, 4, MODE, true>(k, st);
+    else if (p.pieces <= 192) group_rows<T, 32, 6, MODE, true>(k, st);
     else group_rows<T, 32, 8, MODE, true>(k, st);
 }
 
