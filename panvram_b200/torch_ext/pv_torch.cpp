@@ -87,6 +87,7 @@ void check_floats(const Tensor& t, const char* name, const pv_scored& b, const T
     TORCH_CHECK_VALUE(shape && t.scalar_type() == at::kFloat && t.layout() == at::kStrided, name, ": a float32 tensor ", one ? "[n]" : "",
                       one && each ? " or " : "", each ? "[n, W]" : "");
     TORCH_CHECK_VALUE(t.device() == logits.device(), name, ": on ", t.device(), ", the logits on ", logits.device());
+    TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a view whose negation torch has put off, or zeros without memory; pass t.clone()");
 }
 float number(double v, const char* name, double low, double high = std::numeric_limits<double>::infinity()) {
     const bool ok = v >= low && v <= high && !std::isinf(v);
@@ -141,10 +142,11 @@ struct BatchNode : Node {
         TORCH_CHECK(!t.defined() || t.device() == device, "panvram_b200: a saved tensor came back on ", t.device(), ", it was on ", device);
         return t;
     }
-    variable_list apply(variable_list&& up) override {
+    variable_list apply(variable_list&& ups) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        Tensor l = back(logits), t = back(tokens), m = back(mask), g;
-        if (!up[0].defined()) return {Tensor()};
+        const Tensor saved = back(logits), t = back(tokens), m = back(mask);
+        Tensor l = saved, up = ups[0], g;
+        if (!up.defined()) return {Tensor()};
         {
             at::AutoGradMode off(false);
             const c10::cuda::CUDAGuard guard(device);
@@ -154,11 +156,13 @@ struct BatchNode : Node {
             if (b.V > 1 && l.stride(2) != 1) l = l.contiguous();
             pv_scored now = b;
             place(now, l, t, m);
-            g = grad(now, l, t, up[0]);
+            // torch may have put a negation or the zeros themselves off
+            up = up._is_zerotensor() ? at::zeros(up.sizes(), l.options().dtype(at::kFloat)) : up.resolve_neg();
+            g = grad(now, l, t, up);
         }
         if (at::GradMode::is_enabled())
             torch::autograd::set_history(g, std::make_shared<torch::autograd::Error>("panvram_b200: no second derivative",
-                                                                                     torch::autograd::collect_next_edges(l)));
+                                                                                     torch::autograd::collect_next_edges(saved)));
         return {g};
     }
     void release_variables() override {
@@ -360,6 +364,7 @@ struct List {
             TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && type_of(t.scalar_type()) >= 0, name, ": bf16, fp16 or fp32 tensors");
             TORCH_CHECK_VALUE(t.is_contiguous() || t.is_non_overlapping_and_dense(), name, ": tensors that are dense in memory (no gaps, no expanded dimensions)");
             TORCH_CHECK_VALUE(t.device() == ts[0].device(), name, ": on one device");
+            TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a view whose negation torch has put off, or zeros without memory");
             ptr.push_back((uint64_t)t.data_ptr());
             numel.push_back(t.numel());
             type.push_back((uint8_t)type_of(t.scalar_type()));

@@ -28,7 +28,12 @@ def _shared(logits, tokens, mask, shift, ignore):
         raise ValueError("tokens: a uint8 or int64 tensor [n, W]")
     if mask is not None and not isinstance(mask, torch.Tensor):
         raise ValueError("mask: a bool, uint8 or float32 tensor [n, W]")
-    return mask, int(shift), None if ignore is None else int(ignore)
+    shift, ignore = int(shift), None if ignore is None else int(ignore)
+    if not 0 <= shift < 1 << 31:
+        raise ValueError("shift: 0 or more")
+    if ignore is not None and not -1 << 63 <= ignore < 1 << 63:
+        raise ValueError("ignore: a 64-bit integer")
+    return mask, shift, ignore
 
 
 def _floats(**tensors):

@@ -517,6 +517,24 @@ def test_saved_logits_changed_in_place_are_refused(P, cuda):
         loss.backward()
 
 
+def test_negations_that_torch_put_off(P, cuda):
+    """a real view of a conjugate holds the sign beside its memory: refused as a constant, applied to an upstream gradient"""
+    x, t, _ = make(cuda, 2, 6, 16, "fp32")
+    x.requires_grad_()
+    old = torch.complex(torch.zeros(2, 6, device=cuda), torch.rand(2, 6, device=cuda)).conj().imag
+    assert old.is_neg()
+    with pytest.raises(ValueError, match="old_logp.*negation"):
+        P.policy_loss(x, t, old, torch.ones(2, device=cuda))
+    one = torch.complex(torch.zeros(1, device=cuda), torch.ones(1, device=cuda)).conj().imag
+    with pytest.raises(ValueError, match="negation"):
+        P.clip_grads([one], 0.5)
+    a, = torch.autograd.grad(P.window_logprobs(x, t), x, old)
+    b, = torch.autograd.grad(P.window_logprobs(x, t), x, old.clone())
+    assert torch.equal(a, b) and a.abs().max() > 0
+    loss = P.policy_loss(x, t, old.clone(), torch.ones(2, device=cuda))
+    assert "PolicyLoss" in loss.grad_fn.name() and loss.grad_fn.next_functions[0][0].variable is x
+
+
 @pytest.mark.parametrize("V", [5, 128, 2045, 2048, 4096, 70000])
 @pytest.mark.parametrize("how", ["host", "unaligned", "recomputed"])
 def test_saved_tensors_brought_back_elsewhere(P, cuda, V, how):

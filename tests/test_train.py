@@ -25,7 +25,7 @@ def _calls(logits=X, tokens=T, **kw):
     ({"logits": torch.zeros(2, 3, 1).expand(2, 3, 4)}, "logits"),
     ({"tokens": T[:, :2]}, "tokens"), ({"tokens": T.int()}, "tokens"), ({"tokens": T.bool()}, "tokens"), ({"tokens": None}, "tokens"),
     ({"mask": T[:1]}, "mask"), ({"mask": T.long()}, "mask"), ({"mask": X.half()[..., 0]}, "mask"), ({"mask": True}, "mask"),
-    ({"shift": -1}, "shift"), ({"shift": 1 << 31}, "shift"),
+    ({"shift": -1}, "shift"), ({"shift": 1 << 31}, "shift"), ({"shift": 1 << 70}, "shift"), ({"ignore": 1 << 63}, "ignore"),
 ])
 def test_shared_refusals(kw, what):
     for call in _calls(**kw):
