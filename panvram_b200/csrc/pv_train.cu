@@ -644,21 +644,49 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 3 && A) || ((NV == 3 || NV =
 // replaces the logits in the image and leaves as the stretch came.
 //
 // On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 21 us, policy loss and gradient 37 us, bound by the work of a
-// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 57 and 108 us, bound by
-// instructions as the rows above, with a load and a mask a word more.
-template <typename T> __device__ __forceinline__ float word_max(uint32_t a, float m);
-template <> __device__ __forceinline__ float word_max<float>(uint32_t a, float m) { return fmaxf(m, __uint_as_float(a)); }
-template <> __device__ __forceinline__ float word_max<__nv_bfloat16>(uint32_t a, float m) {
-    return fmaxf(m, fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u)));
+// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 55 and 98 us, bound by
+// instructions as the rows above, with a load and two comparisons a word more. 12 words a lane where a third of 17 would be
+// empty (95 words: 47 and 84 us, with 17 55 and 103). Three blocks a multiprocessor for log-probabilities (33 words 35 us, two
+// 40), and for a gradient of up to 16 numerators a lane (11 floats 26 us, two 31).
+template <typename T> __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);        // element by element
+template <> __device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
 }
-template <> __device__ __forceinline__ float word_max<__half>(uint32_t a, float m) {
-    const float2 f = __half22float2(*(const __half2*)&a);
-    return fmaxf(m, fmaxf(f.x, f.y));
+template <> __device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+    return *(const uint32_t*)&m;
+}
+template <> __device__ __forceinline__ uint32_t word_max<__half>(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&m;
+}
+
+// the numerators' sum over a lane's words; FAR: about a maximum beyond 2^29 (or none, by 0)
+template <typename T, bool FAR, int NW>
+__device__ __forceinline__ float sum_words(const uint32_t (&raw)[NW], float by, float c) {
+    constexpr int E = 4 / (int)sizeof(T);
+    uint64_t v = pair(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < (NW * E + 1) / 2; q++) {
+        float x[2];
+        if (E == 2) {
+            unpack_word<T>(raw[E == 2 ? q : 0], x[0], x[1]);
+        } else {
+            x[0] = __uint_as_float(raw[E == 1 ? 2 * q : 0]);
+            x[1] = 2 * q + 1 < NW ? __uint_as_float(raw[2 * q + 1 < NW ? 2 * q + 1 : 0]) : -INFINITY;
+        }
+        if (FAR) less(x, by);
+        numerators(x, c);
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(v), "l"(pair(x[0], x[1])));
+    }
+    float a, b;
+    halves(v, a, b);
+    return a + b;
 }
 
 // NW: words a lane
 template <typename T, int G, int NW, int S, int MODE>
-__global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && NW < 16) ? 3 : 2) rows_flat_kernel(Rows k) {
+__global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && NW * (4 / sizeof(T)) <= 16) ? 3 : 2) rows_flat_kernel(Rows k) {
     constexpr int K = K_OF<T>, RP = 32 / G, E = 4 / (int)sizeof(T), N = (NW * E + 1) / 2 * 2;      // E: elements a word
     constexpr int SLOT = (NW * 32 * 4 + 47) / 16;            // 16-byte pieces of an image
     extern __shared__ uint4 rings[];                         // [WARPS][S][SLOT]
@@ -739,39 +767,47 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && N
             if (any && edge >= 0) ev = x[edge];
             if (edge >= 0) img[q.off + edge] = ev;
             __syncwarp();
-            const int at = q.off + grp * V, w0 = at / E, w1 = (at + V - 1) / E, ty = at + max(y, 0);
+            // the row's words, this lane's, which of them (first: word 0; last: -1 none) another row has a part of
+            const int at = q.off + grp * V, w0 = at / E, words = (at + V - 1) / E - w0 + 1, ty = at + max(y, 0);
+            const int mine = (words - sub + G - 1) / G, last = E == 2 && (at + V) % 2 && (words - 1) % G == sub ? (words - 1) / G : -1;
+            const bool first = E == 2 && sub == 0 && at % 2;
+            uint32_t* const own = (uint32_t*)base + w0 + sub;
             float xt = 0.f;
             if (y >= 0) xt = f32(img[ty]);
             __syncwarp();
             if (y >= 0 && sub == 0) img[ty] = lowest<T>();
             __syncwarp();
-            uint32_t raw[NW];
-            float m = xt;
-            if (y < 0) m = 0.f;
+            uint32_t raw[NW], most = Traits<T>::LOW;
+            const int cnt = y >= 0 ? mine : 0;
 #pragma unroll
             for (int j = 0; j < NW; j++) {
-                const int v = w0 + sub + j * G;
                 raw[j] = Traits<T>::LOW;
-                if (y >= 0 && v <= w1) raw[j] = ((const uint32_t*)base)[v];
-                if (E == 2) {
-                    if (j == 0 && sub == 0 && at % 2) raw[j] = raw[j] & 0xFFFF0000u | Traits<T>::LOW & 0xFFFFu;
-                    if (v == w1 && (at + V) % 2) raw[j] = raw[j] & 0xFFFFu | Traits<T>::LOW & 0xFFFF0000u;
-                }
-                m = word_max<T>(raw[j], m);
+                if (j < cnt) raw[j] = own[j * G];
+                if (j == 0 && first) raw[j] = raw[j] & 0xFFFF0000u | Traits<T>::LOW & 0xFFFFu;
+                if (E == 2 && j == last) raw[j] = raw[j] & 0xFFFFu | Traits<T>::LOW & 0xFFFF0000u;
+                most = word_max<T>(raw[j], most);
             }
+            float m, m2;
+            unpack_word<T>(most, m, m2);
+            m = y < 0 ? 0.f : fmaxf(fmaxf(m, m2), xt);
 #pragma unroll
             for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
             const float c = ref_of(m), et = ex2(exponent(xt, m, c));
-            float e[N];
-            e[N - 1] = -INFINITY;
+            const bool any_far = __any_sync(~0u, far(m));
+            float e[MODE == LOGP ? 1 : N], o;
+            if constexpr (MODE == LOGP) {
+                o = any_far ? sum_words<T, true>(raw, far(m) ? m : 0.f, c) : sum_words<T, false>(raw, 0.f, c);
+            } else {
+                e[N - 1] = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < NW; j++) {
-                if (E == 1) e[j] = __uint_as_float(raw[j]);
-                else unpack_word<T>(raw[j], e[2 * j < N ? 2 * j : 0], e[2 * j + 1 < N ? 2 * j + 1 : 0]);
+                for (int j = 0; j < NW; j++) {
+                    if (E == 1) e[j] = __uint_as_float(raw[j]);
+                    else unpack_word<T>(raw[j], e[2 * j < N ? 2 * j : 0], e[2 * j + 1 < N ? 2 * j + 1 : 0]);
+                }
+                if (any_far) less(e, far(m) ? m : 0.f);
+                numerators(e, c);
+                o = sum_of(e);
             }
-            if (__any_sync(~0u, far(m))) less(e, far(m) ? m : 0.f);
-            numerators(e, c);
-            float o = sum_of(e);
 #pragma unroll
             for (int h = G / 2; h; h >>= 1) o += __shfl_xor_sync(~0u, o, h);
             if constexpr (MODE == LOGP) {
@@ -788,19 +824,19 @@ __global__ void __launch_bounds__(WARPS * 32, MODE == LOGP || (MODE == GRAD && N
                     if (MODE == POLICY && sub == 0) sum += (double)term;
                 }
                 if (d) {
-                    const float inv = reciprocal(o + et), f = -g * inv;
+                    // a row that is not counted: numerators of 0
+                    const float inv = reciprocal(o + et), f = y < 0 ? 0.f : -g * inv;
                     times(e, f);
                     __syncwarp();
+                    const int out = row < rows ? mine : 0;
 #pragma unroll
                     for (int j = 0; j < NW; j++) {
-                        const int v = w0 + sub + j * G;
-                        uint32_t z = E == 1 ? __float_as_uint(e[j]) : pack_word<T>(e[2 * j < N ? 2 * j : 0], e[2 * j + 1 < N ? 2 * j + 1 : 0]);
-                        if (y < 0) z = 0u;
-                        if (row < rows && v <= w1) {
-                            const bool low = E == 1 || !(j == 0 && sub == 0 && at % 2), high = E == 1 || !(v == w1 && (at + V) % 2);
-                            if (low && high) ((uint32_t*)base)[v] = z;
-                            else if (low) ((uint16_t*)base)[2 * v] = (uint16_t)z;
-                            else if (high) ((uint16_t*)base)[2 * v + 1] = (uint16_t)(z >> 16);
+                        const uint32_t z = E == 1 ? __float_as_uint(e[j]) : pack_word<T>(e[2 * j < N ? 2 * j : 0], e[2 * j + 1 < N ? 2 * j + 1 : 0]);
+                        if (j < out) {
+                            const bool low = !(j == 0 && first), high = E == 1 || j != last;
+                            if (low && high) own[j * G] = z;
+                            else if (low) *(uint16_t*)(own + j * G) = (uint16_t)z;
+                            else if (high) *((uint16_t*)(own + j * G) + 1) = (uint16_t)(z >> 16);
                         }
                     }
                     __syncwarp();
@@ -1513,9 +1549,13 @@ void short_rows(const Rows& k, const Plan& p, cudaStream_t st) {
         const int words = sizeof(T) == 4 ? (int)k.b.V : (int)k.b.V / 2 + 1;
         if (words <= 4) flat_rows<T, 1, 4, MODE>(k, st);
         else if (words <= 8) flat_rows<T, 1, 8, MODE>(k, st);
+        else if (words <= 12) flat_rows<T, 1, 12, MODE>(k, st);
         else if (words <= 17) flat_rows<T, 1, 17, MODE>(k, st);
+        else if (words <= 24) flat_rows<T, 2, 12, MODE>(k, st);
         else if (words <= 34) flat_rows<T, 2, 17, MODE>(k, st);
+        else if (words <= 48) flat_rows<T, 4, 12, MODE>(k, st);
         else if (words <= 68) flat_rows<T, 4, 17, MODE>(k, st);
+        else if (words <= 96) flat_rows<T, 8, 12, MODE>(k, st);
         else flat_rows<T, 8, 17, MODE>(k, st);
     } else if (!whole) {
         if (p.pieces <= 16) group_rows<T, 16, 1, MODE, false>(k, st);

@@ -105,7 +105,8 @@ SHAPES = [(1, 1, 1, 0), (1, 1, 5, 1), (1, 2, 5, 1), (3, 7, 5, 1), (2, 33, 9, 1),
           (3, 37, 64, 1), (2, 50, 65, 0), (4, 100, 128, 1), (2, 17, 129, 1), (2, 33, 255, 1), (2, 20, 512, 1), (2, 19, 1000, 1), (2, 11, 1024, 0),
           (2, 9, 1025, 1), (2, 9, 2048, 1), (3, 5, 2049, 0), (2, 5, 4101, 1), (1, 4, 8192, 1), (2, 3, 16384, 1), (1, 3, 16391, 1), (1, 3, 33000, 0),
           (1, 3, 65541, 1), (1, 2, 70001, 1), (1, 3, 140007, 1), (2, 5, 7, 9),
-          (2, 40, 96, 1), (2, 35, 192, 1), (2, 21, 282, 1), (2, 19, 384, 0), (2, 19, 577, 1), (2, 17, 768, 1), (2, 9, 1500, 0), (2, 9, 1536, 1)]
+          (2, 40, 96, 1), (2, 35, 192, 1), (2, 21, 282, 1), (2, 19, 384, 0), (2, 19, 577, 1), (2, 17, 768, 1), (2, 9, 1500, 0), (2, 9, 1536, 1),
+          (2, 75, 21, 1), (3, 41, 45, 1), (2, 37, 85, 0), (2, 35, 171, 1)]
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
