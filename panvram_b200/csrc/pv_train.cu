@@ -275,19 +275,31 @@ template <> __device__ __forceinline__ uint4 pack<__half>(const float (&x)[8]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T> __device__ __forceinline__ float piece_max(const uint4& r);
-template <> __device__ __forceinline__ float piece_max<float>(const uint4& r) {
-    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+template <typename T> __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);        // element by element
+template <> __device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
 }
-template <> __device__ __forceinline__ float piece_max<__nv_bfloat16>(const uint4& r) {
-    const __nv_bfloat162* w = (const __nv_bfloat162*)&r;
-    const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+template <> __device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+    return *(const uint32_t*)&m;
 }
-template <> __device__ __forceinline__ float piece_max<__half>(const uint4& r) {
-    const __half2* w = (const __half2*)&r;
-    const __half2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+template <> __device__ __forceinline__ uint32_t word_max<__half>(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&m;
+}
+
+// of all words in some pieces: packed, and widened once
+template <typename T, int N>
+__device__ __forceinline__ float pieces_max(const uint4 (&r)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const uint32_t v = word_max<T>(word_max<T>(r[j].x, r[j].y), word_max<T>(r[j].z, r[j].w));
+        m = j ? word_max<T>(m, v) : v;
+    }
+    float a, b;
+    unpack_word<T>(m, a, b);
+    return fmaxf(a, b);
 }
 
 // A row of V elements seen as aligned 16-byte pieces: piece v holds elements v K - off ... + K, off = how far into its
@@ -551,9 +563,7 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 3 && A) || ((NV == 3 || NV =
                 raw[j] = own[j * 32];
                 if (!A && sub + j * G >= n) raw[j] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
             }
-            float m = fmaxf(piece_max<T>(raw[0]), ex);
-#pragma unroll
-            for (int j = 1; j < NV; j++) m = fmaxf(m, piece_max<T>(raw[j]));
+            float m = fmaxf(pieces_max<T>(raw), ex);
 #pragma unroll
             for (int h = G / 2; h; h >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, h));
             m = fmaxf(m, xt);
@@ -648,19 +658,6 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 3 && A) || ((NV == 3 || NV =
 // instructions as the rows above, with a load and two comparisons a word more. 12 words a lane where a third of 17 would be
 // empty (95 words: 47 and 84 us, with 17 55 and 103). Three blocks a multiprocessor for log-probabilities (33 words 35 us, two
 // 40), and for a gradient of up to 16 numerators a lane (11 floats 26 us, two 31).
-template <typename T> __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);        // element by element
-template <> __device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
-    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-}
-template <> __device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
-    return *(const uint32_t*)&m;
-}
-template <> __device__ __forceinline__ uint32_t word_max<__half>(uint32_t a, uint32_t b) {
-    const __half2 m = __hmax2(*(const __half2*)&a, *(const __half2*)&b);
-    return *(const uint32_t*)&m;
-}
-
 // the numerators' sum over a lane's words; FAR: about a maximum beyond 2^29 (or none, by 0)
 template <typename T, bool FAR, int NW>
 __device__ __forceinline__ float sum_words(const uint32_t (&raw)[NW], float by, float c) {
@@ -1156,9 +1153,7 @@ __global__ void __launch_bounds__(THREADS, RING_WARPS<S * U> / (THREADS / 32)) r
                             raw[h] = make_uint4(Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW, Traits<T>::LOW);
                             if (q > 1 || p0 + (j * U + u) * THREADS < n) raw[h] = from[(u + h) * THREADS];
                         }
-                        float m = piece_max<T>(raw[0]);
-#pragma unroll
-                        for (int h = 1; h < q; h++) m = fmaxf(m, piece_max<T>(raw[h]));
+                        const float m = pieces_max<T>(raw);
                         bool plain = true;
                         if (__any_sync(~0u, m > run.m + HEADROOM || far(run.m))) {
                             raise(run, m);
