@@ -518,6 +518,43 @@ def test_saved_logits_changed_in_place_are_refused(P, cuda):
         loss.backward()
 
 
+def test_threads_on_streams_of_their_own(P, cuda):
+    """calls leave the interpreter's lock: four threads at once, each on its stream, give what one gives alone"""
+    import threading
+    cases = []
+    for V in (5, 128, 577, 9001):
+        x, t, _ = make(cuda, 4, 50, V, "bf16", "ids")
+        cases.append((x, t, torch.randn(4, device=cuda), torch.full((4, 50), -3.0, device=cuda)))
+
+    def step(x, t, a, old):
+        x = x.detach().requires_grad_()
+        pair = P.preference_loss(x, t, a)
+        pol = P.policy_loss(x, t, old, a)
+        g = torch.autograd.grad(pair, x)[0], torch.autograd.grad(pol, x)[0]
+        return pair.detach(), pol.detach(), *g, P.clip_grads(list(g), 0.1)
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    out = step(*cases[i])
+                torch.cuda.current_stream().synchronize()
+                got[i] = out
+        except Exception as e:                                       # noqa: BLE001  (raised again below)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    assert not errors and len(got) == 4, errors
+    for i in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])), i
+
+
 def test_negations_that_torch_put_off(P, cuda):
     """a real view of a conjugate holds the sign beside its memory: refused as a constant, applied to an upstream gradient"""
     x, t, _ = make(cuda, 2, 6, 16, "fp32")
