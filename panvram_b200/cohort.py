@@ -596,7 +596,10 @@ class Sampler:
     copy of the generator's seed and offset that the graph advances), so a replay needs no generator bookkeeping on the
     device; if the generator is used or reseeded between calls, the next call reloads its state. With a torch release
     that restatement was not checked against (TORCH_DRAWS_CHECKED), the graph captures torch's own randint / rand
-    instead, and torch advances the generator at each replay."""
+    instead, and torch advances the generator at each replay.
+
+    Every call overwrites the same windows and coordinates, and counts as a change of them in place: a backward pass that
+    still needs the call before's is refused by autograd."""
 
     def __init__(self, cohort, n, W, generator, reverse_complement, tokens, return_coords):
         if generator is None or generator.device.type != "cuda":
@@ -644,13 +647,14 @@ class Sampler:
 
     def __call__(self):
         with torch.cuda.device(self.cohort.device):
-            if not self.native:                          # torch's draws in the graph: torch advances the generator
-                self.graph.replay()
-                return (self.x, self.coords) if self.return_coords else self.x
-            self._load_rng()
-            self.graph.replay()
-        self._offset += self._inc
-        self.generator.set_offset(self._offset)
+            if self.native:
+                self._load_rng()
+            self.graph.replay()                          # not native: torch's draws in the graph, torch advances the generator
+        # written behind autograd's back: what was saved of the call before is refused
+        torch.autograd.graph.increment_version((self.x, self.coords) if self.return_coords else self.x)
+        if self.native:
+            self._offset += self._inc
+            self.generator.set_offset(self._offset)
         return (self.x, self.coords) if self.return_coords else self.x
 
     def status(self):

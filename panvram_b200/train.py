@@ -15,7 +15,7 @@ Kernels run on torch's current stream of the logits' (gradients') device, withou
 allocator on that stream. Logits are bf16, fp16 or fp32 [n, W, V] with any strides between windows and positions; their
 gradient has their type, and no second derivative. Arguments other than the logits are constants. A loss keeps the logits,
 tokens and mask for its backward pass (hooks on saved tensors apply): with Cohort.sampler, run it before the sampler's next
-call overwrites its windows. A clipped list counts as changed in place."""
+call overwrites its windows (autograd refuses it afterwards). A clipped list counts as changed in place."""
 import torch
 
 from . import _C, _train  # noqa: F401  (_C loads the library that _train calls; _train: torch_ext/pv_torch.cpp)

@@ -740,3 +740,23 @@ def test_training_step_from_the_sampler(P, cohort, cuda):
     for w, p in zip(want, double.parameters()):
         # the model's own 32-bit (TF32 off) products bound this, not the loss: sums of 2,400 rows
         assert (w.double() - p.grad).norm() <= 1e-3 * p.grad.norm() + 1e-7
+
+
+def test_a_sampler_marks_its_windows_as_changed(P, cohort, cuda):
+    """a backward pass behind the sampler's next call would pair that call's tokens with this one's logits: refused"""
+    s = cohort.sampler(4, 200, torch.Generator(device=cuda).manual_seed(3), tokens=True, return_coords=True)
+    table = torch.randn(5, 8, device=cuda, requires_grad=True)
+    a, old = torch.ones(4, device=cuda), torch.full((4, 200), -2.0, device=cuda)
+    for f in (lambda x: P.window_logprobs(table[x.long()], x).sum(), lambda x: P.preference_loss(table[x.long()], x, a),
+              lambda x: P.policy_loss(table[x.long()], x, old, a), lambda x: P.policy_loss(table[x.long()].half(), x, old, a) * 2):
+        f(s()[0]).backward()                                         # before the next call: as ever
+        loss = f(s()[0])
+        x, c = s()
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        versions = x._version, c._version
+        s()
+        assert x._version > versions[0] and c._version > versions[1]
+    with torch.inference_mode():                                     # its tensors have no versions
+        s = cohort.sampler(4, 200, torch.Generator(device=cuda).manual_seed(3), tokens=True)
+        assert s().shape == (4, 200)
