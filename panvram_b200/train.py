@@ -16,9 +16,28 @@ allocator on that stream. Logits are bf16, fp16 or fp32 [n, W, V] with any strid
 gradient has their type, and no second derivative. Arguments other than the logits are constants. A loss keeps the logits,
 tokens and mask for its backward pass (hooks on saved tensors apply): with Cohort.sampler, run it before the sampler's next
 call overwrites its windows (autograd refuses it afterwards). A clipped list counts as changed in place."""
+import os
+
 import torch
 
-from . import _C, _train  # noqa: F401  (_C loads the library that _train calls; _train: torch_ext/pv_torch.cpp)
+from . import _C
+
+_train = None               # torch_ext/pv_torch.cpp, loaded by the first call: the data path does without it
+
+
+def _ext():
+    """the compiled side (bound to one torch release, unlike the library that it calls and _C has loaded)"""
+    global _train
+    if _train is None:
+        try:
+            from . import _train as ext
+        except ImportError as e:
+            path = os.path.join(os.path.dirname(_C.LIB_PATH), "_train.so")
+            why = "is missing" if not os.path.exists(path) else f"does not load under torch {torch.__version__}"
+            raise ImportError(f"panvram_b200: the training step's operators are in {path}, which {why}; build it: "
+                              "python panvram_b200/build.py") from e
+        _train = ext
+    return _train
 
 
 def _shared(logits, tokens, mask, shift, ignore):
@@ -54,7 +73,7 @@ def window_logprobs(logits, tokens, mask=None, shift=1, ignore=None, reduce="tok
     t + shift; 0 where it is not counted), or with reduce="window" their sums, float32 [n] (0 for a window with none).
     Differentiable by the logits."""
     window = _by_window(reduce)
-    return _train.window_logprobs(logits, tokens, *_shared(logits, tokens, mask, shift, ignore), window)
+    return _ext().window_logprobs(logits, tokens, *_shared(logits, tokens, mask, shift, ignore), window)
 
 
 def preference_loss(logits, tokens, ref_logp, beta=0.1, label_smoothing=0.0, mask=None, shift=1, ignore=None, return_margins=False):
@@ -65,7 +84,7 @@ def preference_loss(logits, tokens, ref_logp, beta=0.1, label_smoothing=0.0, mas
     pairs (0 without any). return_margins: also the margins, float32 [n/2], which carry no gradient."""
     rest = _shared(logits, tokens, mask, shift, ignore)
     _floats(ref_logp=ref_logp)
-    out = _train.preference_loss(logits, tokens, ref_logp, float(beta), float(label_smoothing), *rest, bool(return_margins))
+    out = _ext().preference_loss(logits, tokens, ref_logp, float(beta), float(label_smoothing), *rest, bool(return_margins))
     return out if return_margins else out[0]
 
 
@@ -85,7 +104,7 @@ def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, k
     if ref_logp is not None:
         _floats(ref_logp=ref_logp)
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
-    return _train.policy_loss(logits, tokens, old_logp, advantages, ref_logp, float(low), float(high), float(kl), *rest, by_window, float(scale))
+    return _ext().policy_loss(logits, tokens, old_logp, advantages, ref_logp, float(low), float(high), float(kl), *rest, by_window, float(scale))
 
 
 def _list(ts):
@@ -97,7 +116,7 @@ def grad_norm(grads):
     each dense in memory) -> float32 scalar on their device, summed in 64 bits. An empty list is refused: it has no
     device."""
     try:
-        return _train.grad_norm(_list(grads))
+        return _ext().grad_norm(_list(grads))
     except TypeError:
         raise ValueError("grads: bf16, fp16 or fp32 tensors") from None
 
@@ -108,6 +127,6 @@ def clip_grads(grads, max_norm, out=None):
     many elements, contiguous as it is (else of its shape and strides); then always written. A tensor that is written may not share memory with another. A norm of
     infinity scales finite elements to 0, NaN makes every element NaN, as the formula says."""
     try:
-        return _train.clip_grads(_list(grads), float(max_norm), None if out is None else _list(out))
+        return _ext().clip_grads(_list(grads), float(max_norm), None if out is None else _list(out))
     except TypeError:
         raise ValueError("grads, out: bf16, fp16 or fp32 tensors") from None

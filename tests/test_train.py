@@ -179,3 +179,28 @@ def test_entry_points_refuse_bad_lists_and_shared_memory():
                    (_list([256], [8], [f]), _list([272], [8], [f])),                             # over part of itself
                    (_list([256], [8], [0]), _list([256], [8], [f]))):                            # wider, over itself
         assert clip(g, out) == _C.PV_EARG and shared in _message()
+
+
+@pytest.mark.parametrize("how", ["missing", "another torch"])
+def test_the_package_needs_its_torch_extension_only_for_the_operators(tmp_path, how):
+    """a copy of the package without _train.so, or with one that does not load: it imports, and a call names the build"""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    copy = tmp_path / "panvram_b200"
+    shutil.copytree(os.path.dirname(P.__file__), copy, ignore=shutil.ignore_patterns("__pycache__", "_train.so", "csrc", "torch_ext"))
+    if how != "missing":
+        (copy / "_train.so").write_bytes(b"not a library")
+    code = ("import torch, panvram_b200 as P\n"
+            "assert P.__file__.startswith(%r) and P.Cohort and P._C.with_cuda\n"
+            "x = torch.zeros(2, 3, 4)\n"
+            "for f in (lambda: P.window_logprobs(x, x[..., 0].byte()), lambda: P.grad_norm([x]), lambda: P.clip_grads([x], 1.0)):\n"
+            "    try:\n"
+            "        f()\n"
+            "    except ImportError as e:\n"
+            "        assert 'build.py' in str(e) and %r in str(e), e\n"
+            "    else:\n"
+            "        raise AssertionError('no error')\n" % (str(tmp_path), "missing" if how == "missing" else "does not load"))
+    r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
