@@ -40,6 +40,32 @@ def _run(cmd, verbose):
     return r.stdout + r.stderr
 
 
+def _build_train(force, verbose):
+    """_train.so, bound to the torch, the Python and the C++ ABI that run this build: its object is named by them, and a
+    stamp beside it says which one _train.so was linked from (an older object is no reason to keep another torch's)"""
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(PKG, "torch_ext", "pv_torch.cpp")
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    key = f"{torch.__version__}-{sysconfig.get_config_var('SOABI')}-abi{abi}"
+    obj, stamp = os.path.join(BUILD, f"pv_torch-{key}.o"), os.path.join(BUILD, "pv_torch.linked")
+    log = ""
+    if force or _stale(obj, [src] + HEADERS):
+        inc = [INC, *cpp_extension.include_paths(), os.path.join(CUDA, "include"), sysconfig.get_paths()["include"]]
+        log += _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", *(f for i in inc for f in ("-isystem", i)),
+                     f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-c", src, "-o", obj], verbose)
+    linked = ""
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            linked = f.read()
+    if force or linked != key or _stale(TRAIN_LIB, [obj, LIB]):
+        _run(["g++", "-shared", "-o", TRAIN_LIB, obj, "-L" + PKG, "-lpanvram_b200", "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+              "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
+        with open(stamp, "w") as f:
+            f.write(key)
+    return log
+
+
 def build(force=False, verbose=False, ptxas_info=False):
     os.makedirs(BUILD, exist_ok=True)
     objs, log = [], ""
@@ -60,18 +86,7 @@ def build(force=False, verbose=False, ptxas_info=False):
     if force or _stale(LIB, objs):
         _run(["g++", "-shared", "-o", LIB, *objs, "-L" + os.path.join(CUDA, "lib64"), "-lcudart_static", "-ldl", "-lrt", "-lpthread",
               os.path.join(LIBDIR, "libzstd.so.1"), os.path.join(LIBDIR, "libxxhash.so.0"), os.path.join(LIBDIR, "libcrypto.so.3")], verbose)
-    # built against the torch that runs this (its C++ interface is bound to its version): the object's name says which
-    import torch
-    from torch.utils import cpp_extension
-    src = os.path.join(PKG, "torch_ext", "pv_torch.cpp")
-    obj = os.path.join(BUILD, f"pv_torch-{torch.__version__}.o")
-    if force or _stale(obj, [src] + HEADERS):
-        inc = [INC, *cpp_extension.include_paths(), os.path.join(CUDA, "include"), sysconfig.get_paths()["include"]]
-        log += _run(["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", *(f for i in inc for f in ("-isystem", i)),
-                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-c", src, "-o", obj], verbose)
-    if force or _stale(TRAIN_LIB, [obj, LIB]):
-        _run(["g++", "-shared", "-o", TRAIN_LIB, obj, "-L" + PKG, "-lpanvram_b200", "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
-              "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
+    log += _build_train(force, verbose)
     # the cohort synthesizer (test and benchmark data; not linked into the decode library)
     src = os.path.join(PKG, "synth", "pv_synth.cpp")
     if force or _stale(SYNTH_LIB, [src] + HEADERS):

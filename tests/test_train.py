@@ -204,3 +204,37 @@ def test_the_package_needs_its_torch_extension_only_for_the_operators(tmp_path, 
             "        raise AssertionError('no error')\n" % (str(tmp_path), "missing" if how == "missing" else "does not load"))
     r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
+
+
+def test_the_torch_extension_is_linked_again_for_another_torch(tmp_path, monkeypatch):
+    """built under one torch, another, and the first again: each time its own object is what _train.so is linked from"""
+    import os
+    import sysconfig
+    from panvram_b200 import build as B
+    monkeypatch.setattr(B, "BUILD", str(tmp_path))
+    monkeypatch.setattr(B, "LIB", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(B, "TRAIN_LIB", str(tmp_path / "_train.so"))
+    monkeypatch.setattr(B, "SYNTH_LIB", str(tmp_path / "synth.so"))
+    clock = [2_000_000_000]                                              # later than every source
+
+    def run(cmd, verbose):
+        out = cmd[cmd.index("-o") + 1]
+        with open(out, "w") as f:
+            f.write(" ".join(c for c in cmd if c.endswith(".o") and c != out))
+        clock[0] += 10
+        os.utime(out, (clock[0], clock[0]))
+        ran.append(out)
+        return ""
+    monkeypatch.setattr(B, "_run", run)
+    real = sysconfig.get_config_var
+    for torch_version, soabi in (("2.11.0", "cpython-312"), ("2.12.0", "cpython-312"), ("2.11.0", "cpython-312"), ("2.11.0", "cpython-313")):
+        monkeypatch.setattr(torch, "__version__", torch_version)
+        monkeypatch.setattr(sysconfig, "get_config_var", lambda k: soabi if k == "SOABI" else real(k))
+        ran = []
+        B.build()
+        with open(tmp_path / "_train.so") as f:
+            linked = os.path.basename(f.read())
+        assert torch_version in linked and soabi in linked, linked
+        ran = []
+        B.build()
+        assert ran == []                                                 # nothing changed
