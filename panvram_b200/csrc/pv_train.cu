@@ -85,8 +85,12 @@ __device__ __forceinline__ int target(const pv_scored& b, int64_t i, int64_t t) 
 __device__ __forceinline__ bool far(float m) { return !(fabsf(m) < 536870912.f); }     // infinities too
 __device__ __forceinline__ float ref_of(float m) { return far(m) ? 0.f : m * LOG2E; }
 __device__ __forceinline__ float exponent(float x, float m, float c) { return far(m) ? (x - m) * LOG2E : fmaf(x, LOG2E, -c); }
-// what a sum of numerators with the maximum m is multiplied by, to be one with the maximum M >= m
-__device__ __forceinline__ float rescale(float m, float M) { return ex2(far(m) || far(M) ? (m - M) * LOG2E : ref_of(m) - ref_of(M)); }
+// What a sum of numerators with the maximum m is multiplied by, to be one with the maximum M >= m. Where only one of the two
+// is far, the other's reference, a product rounded by up to 32, has to be taken as it is.
+__device__ __forceinline__ float rescale(float m, float M) {
+    if (!far(m) && !far(M)) return ex2(ref_of(m) - ref_of(M));
+    return ex2(!far(m) ? fmaf(-M, LOG2E, ref_of(m)) : !far(M) ? fmaf(m, LOG2E, -ref_of(M)) : (m - M) * LOG2E);
+}
 
 __device__ __forceinline__ float reciprocal(float v) {          // of sums of numerators: about 1 or more, so nothing is flushed
     float r;

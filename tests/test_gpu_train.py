@@ -760,3 +760,34 @@ def test_a_sampler_marks_its_windows_as_changed(P, cohort, cuda):
     with torch.inference_mode():                                     # its tensors have no versions
         s = cohort.sampler(4, 200, torch.Generator(device=cuda).manual_seed(3), tokens=True)
         assert s().shape == (4, 200)
+
+
+@pytest.mark.parametrize("V", [2049, 4101, 16384, 65541])
+def test_maxima_on_both_sides_of_the_far_border(P, cuda, V):
+    """threads (and steps) of a row whose maxima lie just below and just above 2^29, where the reference changes its form:
+    floats there are 32 and 64 apart, so the words below weigh e^-32 and e^-64 (and more where there are many)"""
+    top = 2.0 ** 29
+    x = torch.full((1, 6, V), -top, device=cuda)
+    x[0, :, ::3] = top - 32
+    x[0, 1] = top - 32
+    x[0, 2, :64] = top - 64
+    x[0, 3:5] = -top + 32                                    # the same around -2^29
+    x[0, 3, 1::2] = -top - 64
+    x[0, 4, : V // 2] = -top
+    x[0, 5, ::7] = top + 64
+    t = torch.zeros(1, 6, dtype=torch.int64, device=cuda)
+    for i, at in enumerate((V - 1, V // 2, 5, 0, V - 1, 7)):
+        t[0, i] = at
+        if i < 3:
+            x[0, i, at] = top
+    lp, p, y, ok = oracle(x, t, None, 0)
+    x.requires_grad_(True)
+    got = P.window_logprobs(x, t, shift=0)
+    close(got, lp.detach(), tol_lp(V, lp.detach()))
+    (d,) = torch.autograd.grad(got.sum(), x)
+    want, tol = grad_of(x, p, y, ok, torch.ones(1, 6, device=cuda).double())
+    close(d, want, tol + 1e-9)
+    old = lp.detach().float()
+    (d,) = torch.autograd.grad(P.policy_loss(x, t, old, torch.ones(1, device=cuda), shift=0), x)
+    r = (lp.detach() - old.double()).exp()
+    close(d, *grad_of(x, p, y, ok, -r / 6, r / 6 * (tol_lp(V, lp.detach()) + 2 * E32 * (1 + old.abs()))))
