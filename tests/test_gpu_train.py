@@ -834,3 +834,24 @@ def test_log_probabilities_have_no_mean_error(P, cuda, V, pad, kind):
         total += float(margin) - (want - float(ref[0]))
         count += W
     assert abs(total / count) <= 2e-8
+
+
+@pytest.mark.parametrize("d", [s * v for v in (1e-3, 0.1, 0.2499, 0.25, 0.26, 0.3, 0.4, 0.5, 0.7, 0.9, 0.99, 1.0, 1.01, 1.3, 2.0, 3.0, 8.0, 20.0) for s in (1, -1)])
+def test_policy_kl_term_keeps_its_digits(P, cuda, d):
+    """exp(d) - d - 1 by itself (one word: log p is 0, d the reference's; advantage 0). Below 1 a series: its last step's
+    rounding, the steps' before it (at -1 1.2 of the sum's), d d and the product: 5 eps32. From 1 on expm1 (1 ulp = 2 eps32) less
+    d: 2 * 2.39 + 1 at 1, less elsewhere. 6, and 1 for the loss. Its derivative expm1(d), times 1 - p = 1/2 (two equal words, whose
+    log p is log1p(1) to 1 ulp: an error of d, as is d's own rounding): 4 eps32, the reciprocal's 2 and three products."""
+    x, t, z = torch.zeros(1, 1, 1, device=cuda), torch.zeros(1, 1, dtype=torch.int64, device=cuda), torch.zeros(1, 1, device=cuda)
+    ref = torch.full((1, 1), d, device=cuda)
+    v = ref.double().item()
+    want = math.expm1(v) - v if abs(v) > 0.1 else sum(v ** k / math.factorial(k) for k in range(2, 18))
+    got = float(P.policy_loss(x, t, z, z[:, 0], ref, kl=1.0, shift=0))
+    assert abs(got - want) <= 7 * E32 * want
+    x = torch.zeros(1, 1, 2, device=cuda, requires_grad=True)
+    ref = torch.full((1, 1), d - math.log(2), device=cuda)
+    v = ref.double().item() + math.log(2)
+    (g,) = torch.autograd.grad(P.policy_loss(x, t, z, z[:, 0], ref, kl=1.0, shift=0), x)
+    want = -math.expm1(v) * 0.5
+    tol = 9 * E32 * abs(want) + 0.5 * math.exp(v) * E32 * (abs(v) + 2 * math.log(2))
+    assert abs(float(g[0, 0, 0]) - want) <= tol and abs(float(g[0, 0, 1]) + want) <= tol
