@@ -203,7 +203,7 @@ __device__ __forceinline__ float row_end(const Rows& k, const End& e, double lp,
     if (MODE == LOGP) { term = (float)lp; return 0.f; }
     if (MODE == GRAD) { term = 0.f; return e.a * scale; }
     const float r = expf((float)(lp - (double)e.old));        // the difference in 64 bits: it is small beside its terms
-    const float one = e.a == 0.f ? 0.f : r * e.a;
+    const float one = e.a == 0.f && r == INFINITY ? 0.f : r * e.a;      // a ratio that overflows by an advantage of 0 is 0, NaN stays
     const float two = fminf(fmaxf(r, 1.f - k.a.clip_low), 1.f + k.a.clip_high) * e.a;
     const bool free = !(one > two);                          // NaN stays
     float g = free ? -one : 0.f;

@@ -93,7 +93,7 @@ def policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, clip=0.2, k
     old_logp (of the policy that drew the tokens) and ref_logp (of the reference model) laid out the same, float32 [n, W]:
     r = exp(logp - old_logp), and per counted position
         -min(r A, clamp(r, 1 - clip, 1 + clip) A) + kl (exp(d) - d - 1),    d = ref_logp - logp.
-    advantages A: float32 [n], or [n, W] at the logits' positions. clip: a number, or (below, above). kl > 0 needs ref_logp.
+    advantages A: float32 [n], or [n, W] at the logits' positions; where A is 0 an r that overflows counts as 0. clip: a number, or (below, above). kl > 0 needs ref_logp.
     reduce: "token", the mean over all counted positions; "window", the mean over the windows that have any of their own
     means. 0 where nothing is counted. The result is multiplied by `scale`: with 1 / (batches a step) there, and not on the
     loss, the gradient is made in the loss's own pass over bf16 or fp32 logits (whose memory it takes from then on); an

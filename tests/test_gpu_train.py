@@ -855,3 +855,24 @@ def test_policy_kl_term_keeps_its_digits(P, cuda, d):
     want = -math.expm1(v) * 0.5
     tol = 9 * E32 * abs(want) + 0.5 * math.exp(v) * E32 * (abs(v) + 2 * math.log(2))
     assert abs(float(g[0, 0, 0]) - want) <= tol and abs(float(g[0, 0, 1]) + want) <= tol
+
+
+@pytest.mark.parametrize("V", [8, 9, 128, 4096])
+def test_policy_nan_is_not_hidden_by_an_advantage_of_0(P, cuda, V):
+    """a counted position whose logits or old_logp are NaN gives NaN whatever its advantage, in the loss as in the gradient;
+    beside it positions with an overflowing ratio give 0"""
+    t = torch.zeros(1, 3, dtype=torch.int64, device=cuda)
+    adv = torch.zeros(1, device=cuda)
+    for where in ("logits", "old"):
+        x, old = torch.zeros(1, 3, V, device=cuda), torch.full((1, 3), -300.0, device=cuda)
+        if where == "logits":
+            x[0, 1, 2] = math.nan
+        else:
+            old[0, 1] = math.nan
+        loss = P.policy_loss(x.requires_grad_(), t, old, adv, shift=0)
+        (g,) = torch.autograd.grad(loss, x)
+        assert loss.isnan() and g[0, 1].isnan().all() and (g[0, ::2] == 0).all()
+        with torch.no_grad():
+            assert P.policy_loss(x, t, old, adv, shift=0).isnan()
+            m = torch.tensor([[1.0, 0.0, 1.0]], device=cuda)                 # not counted: not read
+            assert P.policy_loss(x, t, old, adv, shift=0, mask=m) == 0
