@@ -1347,7 +1347,7 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const double* part, int64_t
         const double h = (double)beta * gap;
         // log sigmoid(h) = min(h, 0) - log1p(exp(-|h|))
         const double l = log1p(exp(-fabs(h))), up = fmin(h, 0.0) - l, down = fmin(-h, 0.0) - l;
-        all += h != h ? h : -(1.0 - eps) * up - (eps == 0.f ? 0.0 : eps * down);
+        all += h != h ? h : -(eps == 1.f ? 0.0 : (1.0 - eps) * up) - (eps == 0.f ? 0.0 : eps * down);   // 0 of an infinite term is 0
         if (margins) margins[j] = (float)gap;
         const double c = (double)beta / (double)m * ((double)eps - 1.0 / (1.0 + exp(h)));
         coef[j] = (float)c;

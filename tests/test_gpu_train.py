@@ -876,3 +876,13 @@ def test_policy_nan_is_not_hidden_by_an_advantage_of_0(P, cuda, V):
             assert P.policy_loss(x, t, old, adv, shift=0).isnan()
             m = torch.tensor([[1.0, 0.0, 1.0]], device=cuda)                 # not counted: not read
             assert P.policy_loss(x, t, old, adv, shift=0, mask=m) == 0
+
+
+def test_preference_smoothing_at_its_ends_with_infinite_margins(P, cuda):
+    """label_smoothing 0 and 1 each leave out one of the two terms, also where it is infinite (a window that cannot be)"""
+    x = torch.zeros(2, 2, 8, device=cuda)
+    x[0, 0, 0] = -math.inf
+    t, r = torch.zeros(2, 2, dtype=torch.int64, device=cuda), torch.zeros(2, device=cuda)
+    for first, smoothing, want in ((x, 0.0, math.inf), (x, 1.0, 0.0), (x.flip(0), 0.0, 0.0), (x.flip(0), 1.0, math.inf)):
+        loss, margin = P.preference_loss(first, t, r, label_smoothing=smoothing, shift=0, return_margins=True)
+        assert float(loss) == want and float(margin) == (-math.inf if first is x else math.inf)
