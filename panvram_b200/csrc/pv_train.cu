@@ -1664,11 +1664,14 @@ int window_sums(const Plan& p, int64_t n, const double* part, float* sums, doubl
     return launched();
 }
 
+bool finite(float v) { return v >= 0.f && v < INFINITY; }
+
 int bad_policy(const pv_scored* b, const pv_policy_args* a) {
     if (!a) return fail(PV_EARG, "pv_policy: NULL arguments");
-    if (!(a->scale >= 0.f)) return fail(PV_EARG, "pv_policy: scale is negative");
-    if (!(a->clip_low >= 0.f) || !(a->clip_high >= 0.f)) return fail(PV_EARG, "pv_policy: clip is negative");
-    if (!(a->kl == 0.f) && !a->ref && b->n && b->W) return fail(PV_EARG, "pv_policy: a KL term without reference log-probabilities");
+    if (!finite(a->scale)) return fail(PV_EARG, "pv_policy: scale is negative or not finite");
+    if (!finite(a->clip_low) || !finite(a->clip_high)) return fail(PV_EARG, "pv_policy: clip is negative or not finite");
+    if (!finite(a->kl)) return fail(PV_EARG, "pv_policy: kl is negative or not finite");
+    if (a->kl != 0.f && !a->ref && b->n && b->W) return fail(PV_EARG, "pv_policy: a KL term without reference log-probabilities");
     return PV_OK;
 }
 
@@ -1738,6 +1741,8 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
                   void* stat, void* work, size_t work_bytes, void* stream) {
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (b->n & 1) return fail(PV_EARG, "pv_preference: an odd number of windows");
+    if (!finite(beta)) return fail(PV_EARG, "pv_preference: beta is negative or not finite");
+    if (!(smoothing >= 0.f && smoothing <= 1.f)) return fail(PV_EARG, "pv_preference: smoothing is not in [0, 1]");
     if (!loss || (b->n && (!ref || !coef))) return fail(PV_EARG, "pv_preference: NULL argument");
     const Plan p = plan_of(*b);
     const Scratch s = scratch_of(*b, p, work);

@@ -90,8 +90,8 @@ void check_floats(const Tensor& t, const char* name, const pv_scored& b, const T
     TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a view whose negation torch has put off, or zeros without memory; pass t.clone()");
 }
 float number(double v, const char* name, double low, double high = std::numeric_limits<double>::infinity()) {
-    const bool ok = v >= low && v <= high && !std::isinf(v);
-    if (std::isinf(high)) TORCH_CHECK_VALUE(ok, name, ": finite, ", low, " or more");
+    const bool ok = v >= low && v <= high && std::isfinite((float)v);
+    if (std::isinf(high)) TORCH_CHECK_VALUE(ok, name, ": finite (in 32 bits), ", low, " or more");
     TORCH_CHECK_VALUE(ok, name, ": from ", low, " to ", high);
     return (float)v;
 }
@@ -384,7 +384,7 @@ Tensor grad_norm(const std::vector<Tensor>& grads) {
 }
 
 Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::optional<std::vector<Tensor>>& out) {
-    TORCH_CHECK_VALUE(max_norm >= 0, "max_norm: 0 or more");
+    TORCH_CHECK_VALUE(max_norm >= 0 && std::isinf(max_norm) == std::isinf((float)max_norm), "max_norm: 0 or more, in float32's range or infinity");
     const List l(grads, "grads");
     std::optional<List> o;
     if (out) {

@@ -238,3 +238,28 @@ def test_the_torch_extension_is_linked_again_for_another_torch(tmp_path, monkeyp
         ran = []
         B.build()
         assert ran == []                                                 # nothing changed
+
+
+def test_refusals_of_numbers_that_32_bits_cannot_hold():
+    """1e39 is finite, but infinity to the kernels"""
+    for call, name in ((lambda: P.preference_loss(X, T, A, beta=1e39), "beta"), (lambda: P.policy_loss(X, T, L, A, clip=1e39), "clip"),
+                       (lambda: P.policy_loss(X, T, L, A, clip=(0.2, 1e39)), "clip"), (lambda: P.policy_loss(X, T, L, A, scale=1e39), "scale"),
+                       (lambda: P.policy_loss(X, T, L, A, ref_logp=L, kl=1e39), "kl"), (lambda: P.clip_grads([A], 1e39), "max_norm")):
+        with pytest.raises(ValueError, match=name):
+            call()
+    for call in (lambda: P.preference_loss(X, T, A, beta=3e38), lambda: P.clip_grads([A], float("inf"))):
+        with pytest.raises(RuntimeError, match="GPU only"):                      # accepted as far as the device
+            call()
+
+
+def test_entry_points_refuse_bad_numbers():
+    lib, b = _C._lib, _scored()
+    good = dict(old=64, adv=64, ref=64, clip_low=0.2, clip_high=0.2, kl=0.1, scale=1.0)
+    for k in ("clip_low", "clip_high", "kl", "scale"):
+        for bad in (-1.0, float("nan"), float("inf")):
+            a = _C.PolicyArgs(**{**good, k: bad})
+            assert lib.pv_policy(b, ctypes.byref(a), 64, 64, 64, 1 << 30, None) == _C.PV_EARG and k.split("_")[0] in _message()
+            assert lib.pv_policy_grad(_scored(grad=64), ctypes.byref(a), 64, None, 0, None, 0, None) == _C.PV_EARG
+    for beta, smoothing, what in ((-1.0, 0.0, "beta"), (float("nan"), 0.0, "beta"), (float("inf"), 0.0, "beta"), (0.1, -0.1, "smoothing"),
+                                  (0.1, 1.5, "smoothing"), (0.1, float("nan"), "smoothing")):
+        assert lib.pv_preference(b, 64, 1, beta, smoothing, 64, None, 64, None, 64, 1 << 30, None) == _C.PV_EARG and what in _message()
