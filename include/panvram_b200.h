@@ -422,7 +422,8 @@ const char* pv_kernels_last_error(void);
 
 /* ---- device: the operators of a training step around a model fed from the cohort (no counterpart in the reference,
  * which hands the batch out and leaves scoring, losses and clipping to the caller's framework). Device pointers;
- * asynchronous on `stream`; work: device scratch of the stated size, 16-byte aligned. Failures: pv_kernels_last_error. */
+ * asynchronous on `stream`; work: device scratch of the stated size, 16-byte aligned. Every array is aligned to its type.
+ * Failures: pv_kernels_last_error. */
 
 #define PV_T_BF16 0
 #define PV_T_FP16 1

@@ -309,7 +309,7 @@ int all(const pv_tensors* g, const pv_tensors* out, bool clip, double* part, int
 }
 
 int norm_parts(const pv_tensors* g, float* norm, void* work, size_t work_bytes, int64_t* parts, cudaStream_t st) {
-    if (!norm) return fail(PV_EARG, "norm: NULL");
+    if (!norm || (uintptr_t)norm % 4) return fail(PV_EARG, "norm: NULL or not aligned to float");
     if (!work || work_bytes < pv_grads_work_bytes(g) || ((uintptr_t)work & 15)) return fail(PV_EARG, "scratch: too small, NULL or not 16-byte aligned");
     *parts = 0;
     return all(g, nullptr, false, (double*)work, parts, 0.f, false, nullptr, st);

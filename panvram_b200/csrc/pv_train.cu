@@ -1445,6 +1445,8 @@ int launched() {
     return e == cudaSuccess ? PV_OK : fail(PV_ECUDA, cudaGetErrorString(e));
 }
 
+bool off(const void* p, int bytes) { return (uintptr_t)p % bytes != 0; }       // an address not aligned to its type
+
 const char* bad_batch(const pv_scored* b) {
     if (!b) return "batch: NULL";
     if (b->n < 0 || b->W < 0 || b->W >= (1ll << 31) || b->V < 1 || b->V >= (1ll << 30)) return "batch: n, W or V out of range";
@@ -1454,6 +1456,9 @@ const char* bad_batch(const pv_scored* b) {
     if (b->mask_bytes != 0 && b->mask_bytes != 1 && b->mask_bytes != 4) return "batch: the mask is uint8 or float";
     if (b->n > 0 && b->W > 0 && (!b->logits || !b->tokens || (b->mask_bytes && !b->mask))) return "batch: NULL logits, tokens or mask";
     if (b->n > 0 && b->W > (1ll << 62) / b->n) return "batch: n W is too large";
+    const int size = b->type == PV_T_FP32 ? 4 : 2;
+    if (off(b->logits, size) || off(b->grad, size) || off(b->tokens, b->token_bytes) || (b->mask_bytes && off(b->mask, b->mask_bytes)))
+        return "batch: an address is not aligned to its type";
     return nullptr;
 }
 
@@ -1671,6 +1676,7 @@ int bad_policy(const pv_scored* b, const pv_policy_args* a) {
     if (!finite(a->scale)) return fail(PV_EARG, "pv_policy: scale is negative or not finite");
     if (!finite(a->clip_low) || !finite(a->clip_high)) return fail(PV_EARG, "pv_policy: clip is negative or not finite");
     if (!finite(a->kl)) return fail(PV_EARG, "pv_policy: kl is negative or not finite");
+    if (off(a->old, 4) || off(a->adv, 4) || off(a->ref, 4)) return fail(PV_EARG, "pv_policy: an address is not aligned to float");
     if (a->kl != 0.f && !a->ref && b->n && b->W) return fail(PV_EARG, "pv_policy: a KL term without reference log-probabilities");
     return PV_OK;
 }
@@ -1713,6 +1719,7 @@ int pv_logprobs(const pv_scored* b, float* logp, float* sums, void* stat, void* 
     const Plan p = plan_of(*b);
     const Scratch s = scratch_of(*b, p, work);
     if (sums && check_work(s, work, work_bytes)) return PV_EARG;
+    if (off(logp, 4) || off(sums, 4) || off(stat, 16)) return fail(PV_EARG, "pv_logprobs: an address is not aligned (float, stat to 16 bytes)");
     if (b->n == 0) return PV_OK;
     Rows k = rows_of(*b, p);
     k.b.grad = nullptr;
@@ -1728,6 +1735,7 @@ int pv_logprobs_grad(const pv_scored* b, const float* up, int64_t up_n, int64_t 
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !up) return fail(PV_EARG, "pv_logprobs_grad: NULL gradient");
+    if (off(up, 4) || off(scale, 4)) return fail(PV_EARG, "pv_logprobs_grad: an address is not aligned to float");
     const Plan p = plan_of(*b);
     if (p.form > SHORT_ROWS && (!stat || ((uintptr_t)stat & 15))) return fail(PV_EARG, "pv_logprobs_grad: rows of this length need their statistics");
     Rows k = rows_of(*b, p);
@@ -1744,6 +1752,8 @@ int pv_preference(const pv_scored* b, const float* ref, int64_t ref_n, float bet
     if (!finite(beta)) return fail(PV_EARG, "pv_preference: beta is negative or not finite");
     if (!(smoothing >= 0.f && smoothing <= 1.f)) return fail(PV_EARG, "pv_preference: smoothing is not in [0, 1]");
     if (!loss || (b->n && (!ref || !coef))) return fail(PV_EARG, "pv_preference: NULL argument");
+    if (off(ref, 4) || off(loss, 4) || off(margins, 4) || off(coef, 4) || off(stat, 16))
+        return fail(PV_EARG, "pv_preference: an address is not aligned (float, stat to 16 bytes)");
     const Plan p = plan_of(*b);
     const Scratch s = scratch_of(*b, p, work);
     if (check_work(s, work, work_bytes)) return PV_EARG;
@@ -1771,6 +1781,7 @@ int pv_policy(const pv_scored* b, const pv_policy_args* a, float* loss, double* 
     if (const char* why = bad_batch(b)) return fail(PV_EARG, why);
     if (const int e = bad_policy(b, a)) return e;
     if (!loss || (b->n && !weight) || (b->n && b->W && (!a->old || !a->adv))) return fail(PV_EARG, "pv_policy: NULL argument");
+    if (off(loss, 4) || off(weight, 8)) return fail(PV_EARG, "pv_policy: an address is not aligned (loss float, weight double)");
     const Plan p = plan_of(*b);
     const Scratch s = scratch_of(*b, p, work);
     if (check_work(s, work, work_bytes)) return PV_EARG;
@@ -1799,6 +1810,7 @@ int pv_policy_grad(const pv_scored* b, const pv_policy_args* a, const double* we
     if (const int e = bad_policy(b, a)) return e;
     if (b->n == 0 || b->W == 0) return PV_OK;
     if (!b->grad || !weight || !a->old || !a->adv) return fail(PV_EARG, "pv_policy_grad: NULL argument");
+    if (off(weight, 8) || off(scale, 4)) return fail(PV_EARG, "pv_policy_grad: an address is not aligned (weight double, scale float)");
     const Plan p = plan_of(*b);
     const Scratch s = scratch_of(*b, p, work);
     if (p.form == LONG_ROWS && check_work(s, work, work_bytes)) return PV_EARG;

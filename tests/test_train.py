@@ -263,3 +263,31 @@ def test_entry_points_refuse_bad_numbers():
     for beta, smoothing, what in ((-1.0, 0.0, "beta"), (float("nan"), 0.0, "beta"), (float("inf"), 0.0, "beta"), (0.1, -0.1, "smoothing"),
                                   (0.1, 1.5, "smoothing"), (0.1, float("nan"), "smoothing")):
         assert lib.pv_preference(b, 64, 1, beta, smoothing, 64, None, 64, None, 64, 1 << 30, None) == _C.PV_EARG and what in _message()
+
+
+def test_entry_points_refuse_addresses_that_are_not_aligned():
+    """a misaligned access ends the CUDA context, so none is launched: host addresses, nothing is read"""
+    lib, ok = _C._lib, (64, 1 << 30, None)
+    for kw in ({"logits": 66}, {"grad": 66}, {"logits": 65, "type": 0}, {"tokens": 68, "token_bytes": 8}, {"mask": 66, "mask_bytes": 4}):
+        assert lib.pv_logprobs(_scored(**kw), 64, None, None, *ok) == _C.PV_EARG and "aligned" in _message()
+    assert lib.pv_score_work_bytes(_scored(logits=66, type=0)) > 0                              # 2-byte logits there are fine
+    b, g = _scored(), _scored(grad=64)
+    long = _scored(V=100000, logits_w=100000, logits_n=300000, grad=64)
+    for args in ((66, None, None), (None, 66, None), (64, None, 72)):
+        assert lib.pv_logprobs(long, *args, *ok) == _C.PV_EARG and "aligned" in _message()
+    for up, scale in ((66, None), (64, 66)):
+        assert lib.pv_logprobs_grad(g, up, 3, 1, None, scale, None) == _C.PV_EARG and "aligned" in _message()
+    for k in range(5):
+        ref, loss, margins, coef, stat = [64 + (2 if i == k else 0) for i in range(4)] + [72 if k == 4 else 64]
+        assert lib.pv_preference(long, ref, 1, 0.1, 0.0, loss, margins, coef, stat, *ok) == _C.PV_EARG and "aligned" in _message()
+    good = dict(old=64, adv=64, ref=64, clip_low=0.2, clip_high=0.2, kl=0.1, scale=1.0)
+    for k in ("old", "adv", "ref"):
+        a = ctypes.byref(_C.PolicyArgs(**{**good, k: 66}))
+        assert lib.pv_policy(b, a, 64, 64, *ok) == _C.PV_EARG and "aligned" in _message()
+        assert lib.pv_policy_grad(g, a, 64, None, 0, *ok) == _C.PV_EARG and "aligned" in _message()
+    a = ctypes.byref(_C.PolicyArgs(**good))
+    assert lib.pv_policy(b, a, 66, 64, *ok) == _C.PV_EARG and lib.pv_policy(b, a, 64, 68, *ok) == _C.PV_EARG and "aligned" in _message()
+    assert lib.pv_policy_grad(g, a, 68, None, 0, *ok) == _C.PV_EARG and lib.pv_policy_grad(g, a, 64, 66, 0, *ok) == _C.PV_EARG
+    grads = _list([64], [4], [2])
+    assert lib.pv_grad_norm(ctypes.byref(grads), 66, 64, 1 << 20, None) == _C.PV_EARG and "aligned" in _message()
+    assert lib.pv_clip_grads(ctypes.byref(grads), None, 1.0, 66, 64, 1 << 20, None) == _C.PV_EARG and "aligned" in _message()
