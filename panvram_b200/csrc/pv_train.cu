@@ -1449,13 +1449,14 @@ bool off(const void* p, int bytes) { return (uintptr_t)p % bytes != 0; }       /
 
 const char* bad_batch(const pv_scored* b) {
     if (!b) return "batch: NULL";
-    if (b->n < 0 || b->W < 0 || b->W >= (1ll << 31) || b->V < 1 || b->V >= (1ll << 30)) return "batch: n, W or V out of range";
+    // scratch, statistics and offsets are up to 32 bytes a position and 16 a window: no size below wraps round in 64 bits
+    if (b->n < 0 || b->n > (1ll << 56) || b->W < 0 || b->W >= (1ll << 31) || b->V < 1 || b->V >= (1ll << 30)) return "batch: n, W or V out of range";
     if (b->shift < 0) return "batch: shift is negative";
     if (b->type < PV_T_BF16 || b->type > PV_T_FP32) return "batch: logits are bf16, fp16 or fp32";
     if (b->token_bytes != 1 && b->token_bytes != 8) return "batch: tokens are uint8 or int64";
     if (b->mask_bytes != 0 && b->mask_bytes != 1 && b->mask_bytes != 4) return "batch: the mask is uint8 or float";
     if (b->n > 0 && b->W > 0 && (!b->logits || !b->tokens || (b->mask_bytes && !b->mask))) return "batch: NULL logits, tokens or mask";
-    if (b->n > 0 && b->W > (1ll << 62) / b->n) return "batch: n W is too large";
+    if (b->n > 0 && b->W > (1ll << 56) / b->n) return "batch: n W is too large";
     const int size = b->type == PV_T_FP32 ? 4 : 2;
     if (off(b->logits, size) || off(b->grad, size) || off(b->tokens, b->token_bytes) || (b->mask_bytes && off(b->mask, b->mask_bytes)))
         return "batch: an address is not aligned to its type";

@@ -57,6 +57,7 @@ pv_scored batch_of(const Tensor& logits, const Tensor& tokens, const MaybeTensor
     const int64_t n = logits.size(0), W = logits.size(1), V = logits.size(2);
     TORCH_CHECK_VALUE(V >= 1 && (V == 1 || logits.stride(2) == 1), "logits: at least one word, and a position's words contiguous");
     TORCH_CHECK_VALUE(W < (int64_t(1) << 31) && V < (int64_t(1) << 30), "logits: W below 2^31 and V below 2^30");
+    TORCH_CHECK_VALUE(n <= (int64_t(1) << 56) / std::max<int64_t>(W, 1), "logits: n W up to 2^56");
     const bool ids = tokens.scalar_type() == at::kLong;
     TORCH_CHECK_VALUE(tokens.dim() == 2 && tokens.size(0) == n && tokens.size(1) == W && tokens.layout() == at::kStrided &&
                           (ids || tokens.scalar_type() == at::kByte),

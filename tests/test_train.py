@@ -291,3 +291,18 @@ def test_entry_points_refuse_addresses_that_are_not_aligned():
     grads = _list([64], [4], [2])
     assert lib.pv_grad_norm(ctypes.byref(grads), 66, 64, 1 << 20, None) == _C.PV_EARG and "aligned" in _message()
     assert lib.pv_clip_grads(ctypes.byref(grads), None, 1.0, 66, 64, 1 << 20, None) == _C.PV_EARG and "aligned" in _message()
+
+
+@pytest.mark.parametrize("n, W", [(1 << 62, 0), (1 << 61, 0), (1 << 61, 1), (1 << 31, (1 << 31) - 1)])
+def test_sizes_whose_bytes_wrap_round_are_refused(n, W):
+    """expanded tensors may have such shapes; scratch of n W doubles would come out as few bytes or none"""
+    lib, b = _C._lib, _scored(n=n, W=W, V=1 << 20)
+    assert lib.pv_score_work_bytes(b) == 0 and lib.pv_score_stat_bytes(b) == 0
+    for call in (lambda: lib.pv_logprobs(b, None, 64, None, 64, 1 << 40, None),
+                 lambda: lib.pv_preference(b, 64, 0, 0.1, 0.0, 64, None, 64, None, 64, 1 << 40, None)):
+        assert call() == _C.PV_EARG and _message().startswith("batch")
+    x = torch.zeros(1, 1, 1).expand(n, W, 1) if W else torch.zeros(n, 0, 1)
+    t = torch.zeros(1, 1, dtype=torch.uint8).expand(n, W) if W else torch.zeros(n, 0, dtype=torch.uint8)
+    for call in _calls(x, t):
+        with pytest.raises(ValueError, match="n W"):
+            call()
