@@ -33,6 +33,14 @@ int type_of(at::ScalarType t) {
     return t == at::kBFloat16 ? PV_T_BF16 : t == at::kHalf ? PV_T_FP16 : t == at::kFloat ? PV_T_FP32 : -1;
 }
 
+// the kernels take a tensor's memory as it lies
+void check_memory(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a view whose negation torch has put off, or zeros without memory; pass t.clone()");
+    TORCH_CHECK_VALUE(t.has_storage() && (t.numel() == 0 || t.storage().data() != nullptr), name,
+                      ": a tensor without memory of its own (in a wrapper class, as sharded tensors are, or in a function transform such as vmap); "
+                      "pass the tensor inside, a shard's local part");
+}
+
 void check_device(const Tensor& t, const char* what) {
     TORCH_CHECK(t.is_cuda(), "panvram_b200 runs on the GPU only: ", what, " on ", t.device());
     TORCH_CHECK(at::cuda::getDeviceProperties(t.get_device())->major >= 10, "panvram_b200 is built for sm_100a (B200); ",
@@ -67,10 +75,13 @@ pv_scored batch_of(const Tensor& logits, const Tensor& tokens, const MaybeTensor
                               (mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte || mask->scalar_type() == at::kFloat),
                           "mask: a bool, uint8 or float32 tensor [n, W]");
     TORCH_CHECK_VALUE(shift >= 0 && shift < (int64_t(1) << 31), "shift: 0 or more");
+    TORCH_CHECK(!logits._fw_grad(0).defined(), "panvram_b200: no forward-mode derivative");
+    check_memory(logits, "logits");
+    check_memory(tokens, "tokens");
+    if (mask) check_memory(*mask, "mask");
     check_device(logits, "logits");
     TORCH_CHECK_VALUE(tokens.device() == logits.device(), "tokens: on ", tokens.device(), ", the logits on ", logits.device());
     if (mask) TORCH_CHECK_VALUE(mask->device() == logits.device(), "mask: on ", mask->device(), ", the logits on ", logits.device());
-    TORCH_CHECK(!logits._fw_grad(0).defined(), "panvram_b200: no forward-mode derivative");
     pv_scored b = {};
     b.n = n; b.W = W; b.V = V;
     place(b, logits, tokens, mask ? *mask : Tensor());
@@ -88,7 +99,7 @@ void check_floats(const Tensor& t, const char* name, const pv_scored& b, const T
     TORCH_CHECK_VALUE(shape && t.scalar_type() == at::kFloat && t.layout() == at::kStrided, name, ": a float32 tensor ", one ? "[n]" : "",
                       one && each ? " or " : "", each ? "[n, W]" : "");
     TORCH_CHECK_VALUE(t.device() == logits.device(), name, ": on ", t.device(), ", the logits on ", logits.device());
-    TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a view whose negation torch has put off, or zeros without memory; pass t.clone()");
+    check_memory(t, name);
 }
 float number(double v, const char* name, double low, double high = std::numeric_limits<double>::infinity()) {
     const bool ok = v >= low && v <= high && std::isfinite((float)v);
@@ -365,7 +376,7 @@ struct List {
             TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided && type_of(t.scalar_type()) >= 0, name, ": bf16, fp16 or fp32 tensors");
             TORCH_CHECK_VALUE(t.is_contiguous() || t.is_non_overlapping_and_dense(), name, ": tensors that are dense in memory (no gaps, no expanded dimensions)");
             TORCH_CHECK_VALUE(t.device() == ts[0].device(), name, ": on one device");
-            TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a view whose negation torch has put off, or zeros without memory");
+            check_memory(t, name);
             ptr.push_back((uint64_t)t.data_ptr());
             numel.push_back(t.numel());
             type.push_back((uint8_t)type_of(t.scalar_type()));

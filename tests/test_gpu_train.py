@@ -886,3 +886,25 @@ def test_preference_smoothing_at_its_ends_with_infinite_margins(P, cuda):
     for first, smoothing, want in ((x, 0.0, math.inf), (x, 1.0, 0.0), (x.flip(0), 0.0, 0.0), (x.flip(0), 1.0, math.inf)):
         loss, margin = P.preference_loss(first, t, r, label_smoothing=smoothing, shift=0, return_margins=True)
         assert float(loss) == want and float(margin) == (-math.inf if first is x else math.inf)
+
+
+def test_transforms_and_tensors_without_memory_are_refused(P, cuda):
+    """as on the CPU (test_train.py), and several upstream gradients at once"""
+    from test_train import Wrapped
+    x, t, _ = make(cuda, 2, 6, 16, "fp32")
+    a = torch.zeros(2, device=cuda)
+    for call, name in ((lambda: P.window_logprobs(Wrapped(x), t), "logits"), (lambda: P.preference_loss(x, t, Wrapped(a)), "ref_logp"),
+                       (lambda: torch.vmap(lambda z: P.window_logprobs(z, t))(x[None].repeat(3, 1, 1, 1)), "logits"),
+                       (lambda: torch.func.grad(lambda z: P.preference_loss(z, t, a))(x), "logits"),
+                       (lambda: P.clip_grads([Wrapped(x)], 1.0), "grads")):
+        with pytest.raises(ValueError, match=name + ": a tensor without memory"):
+            call()
+    with pytest.raises(ValueError, match="logits.*negation"):
+        P.window_logprobs(torch._neg_view(x), t)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            P.window_logprobs(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), t)
+    x.requires_grad_()
+    out = P.window_logprobs(x, t)
+    with pytest.raises(RuntimeError, match="storage|memory"):
+        torch.autograd.grad(out, x, torch.ones(3, 2, 6, device=cuda), is_grads_batched=True)

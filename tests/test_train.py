@@ -306,3 +306,37 @@ def test_sizes_whose_bytes_wrap_round_are_refused(n, W):
     for call in _calls(x, t):
         with pytest.raises(ValueError, match="n W"):
             call()
+
+
+class Wrapped(torch.Tensor):
+    """a tensor class that holds another one and has no memory itself"""
+
+    @staticmethod
+    def __new__(cls, inside):
+        return torch.Tensor._make_wrapper_subclass(cls, inside.size(), strides=inside.stride(), dtype=inside.dtype, device=inside.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+        raise NotImplementedError(str(f))
+
+
+def test_tensors_without_memory_are_refused_by_name():
+    for call, name in ((lambda: P.window_logprobs(Wrapped(X), T), "logits"), (lambda: P.window_logprobs(X, Wrapped(T)), "tokens"),
+                       (lambda: P.window_logprobs(X, T, Wrapped(T)), "mask"), (lambda: P.grad_norm([Wrapped(X)]), "grads"),
+                       (lambda: P.clip_grads([A, Wrapped(X)], 1.0), "grads"), (lambda: P.clip_grads([X], 1.0, out=[Wrapped(X)]), "out"),
+                       (lambda: torch.vmap(lambda z: P.window_logprobs(z, T))(X[None].repeat(3, 1, 1, 1)), "logits"),
+                       (lambda: torch.vmap(lambda z: P.policy_loss(X, z, L, A))(T[None].repeat(3, 1, 1)), "tokens"),
+                       (lambda: torch.func.grad(lambda z: P.window_logprobs(z, T).sum())(X), "logits"),
+                       (lambda: torch.vmap(lambda z: P.grad_norm([z]))(X), "grads")):
+        with pytest.raises(ValueError, match=name + ": a tensor without memory"):
+            call()
+
+
+def test_negated_logits_and_forward_mode_are_refused():
+    for call in _calls(torch._neg_view(X)):
+        with pytest.raises(ValueError, match="logits.*negation"):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        for call in _calls(torch.autograd.forward_ad.make_dual(X, torch.ones_like(X))):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
