@@ -908,3 +908,9 @@ def test_transforms_and_tensors_without_memory_are_refused(P, cuda):
     out = P.window_logprobs(x, t)
     with pytest.raises(RuntimeError, match="storage|memory"):
         torch.autograd.grad(out, x, torch.ones(3, 2, 6, device=cuda), is_grads_batched=True)
+
+
+@pytest.mark.parametrize("how", ["host", "unaligned", "recomputed"])
+def test_saved_tensors_brought_back_to_a_form_that_reads_twice(P, cuda, how):
+    """9,216 pieces fit the policy loss's ring; brought back astride one more they are read twice, with scratch of their own"""
+    test_saved_tensors_brought_back_elsewhere(P, cuda, 73728, how)
