@@ -169,8 +169,8 @@ __device__ __forceinline__ double row_logp(float m, float o, float x, float e) {
 // the second is 9 times smaller than the first); from 1 on it loses 2.4 at most.
 __device__ __forceinline__ void kl_terms(float d, float& em1, float& kl) {
     if (fabsf(d) < 1.f) {
-        constexpr float F[11] = {0.5f, 1.f / 6, 1.f / 24, 1.f / 120, 1.f / 720, 1.f / 5040, 1.f / 40320, 1.f / 362880, 1.f / 3628800,
-                                 1.f / 39916800, 1.f / 479001600};              // the next is 2e-10 of the sum
+        constexpr float F[11] = {1.f / 2, 1.f / 6, 1.f / 24, 1.f / 120, 1.f / 720, 1.f / 5040, 1.f / 40320, 1.f / 362880,
+                                 1.f / 3628800, 1.f / 39916800, 1.f / 479001600};      // the next is 2e-10 of the sum
         float p = F[10];
 #pragma unroll
         for (int j = 9; j >= 0; j--) p = fmaf(d, p, F[j]);
@@ -473,8 +473,11 @@ __device__ __noinline__ float sum_far(const uint4* raw, int step, float by, floa
 // the ring and -inf put in its place: the sum of the others and their maximum follow without a comparison an element.
 //
 // On a B200, 524,288 rows of 128 bf16 words: log-probabilities 35 us (3.8 TB/s), policy loss and gradient 58 us (4.6 TB/s
-// read and written). Bound by instructions: a step has about 250 of its own (targets, addresses, shuffles, the row's end)
-// beside 4 a word. So lanes hold 32 words (64, half the lanes, lose more by the warps that no longer fit: 1,048,576 rows take
+// read and written); 1,048,576 of 16 words 19 and 32 us. Bound by instructions: counted, a step of 8 rows of 128 words takes
+// 321 of them for log-probabilities, 373 for a gradient and 577 for the policy loss (targets, addresses, shuffles, the rows'
+// ends) where the words themselves, 32 a lane, take 4 each or 8 with a gradient; of 32 rows of 16 words 426, 427 and 733; of 2 of
+// 401 words that start anywhere 376, 499 and 676. Issue slots are 49 to 63 % taken, the rest is their latency at 5 to 7 warps
+// a scheduler. So lanes hold 32 words (64, half the lanes, lose more by the warps that no longer fit: 1,048,576 rows take
 // 146 us, and 112 with 32), and 3 or 6 pieces where a quarter of 4 or 8 would be empty (131,072 rows of 1,536: 150 us with 6,
 // 179 with 8). Three blocks a multiprocessor for log-probabilities (64 us, two 69), two where the numerators are kept for the
 // gradient (112 us, three spill: 153). A row that starts anywhere costs half as much again (282 words of 4 bytes 180 us, 284
@@ -672,9 +675,10 @@ __global__ void __launch_bounds__(WARPS * 32, (NV < 3 && A) || ((NV == 3 || NV =
 // lane by lane; of a first or last word that it shares with its neighbour it masks the half that is not its own. The gradient
 // replaces the logits in the image and leaves as the stretch came.
 //
-// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 21 us, policy loss and gradient 37 us, bound by the work of a
-// row's own (its target, log-probability and loss: over 100 instructions); 524,288 of 101 words 55 and 98 us, bound by
-// instructions as the rows above, with a load and two comparisons a word more. 12 words a lane where a third of 17 would be
+// On a B200, 1,048,576 rows of 5 bf16 words: log-probabilities 21 us, gradient 24 us, policy loss and gradient 37 us, bound by the
+// instructions of a step, whatever its words: counted, 539, 597 and 820 for 32 rows (the stretch and its ends, the image, the
+// targets, the rows' ends), issue slots 72, 68 and 56 % taken, the rest latency at 7 to 4 warps a scheduler. 524,288 of 101
+// words 56 and 98 us, bound by instructions as the rows above, with a load and two comparisons a word more. 12 words a lane where a third of 17 would be
 // empty (95 words: 47 and 84 us, with 17 55 and 103). Three blocks a multiprocessor for log-probabilities (33 words 35 us, two
 // 40), and for a gradient of up to 16 numerators a lane (11 floats 26 us, two 31).
 // the numerators' sum over a lane's words; FAR: about a maximum beyond 2^29 (or none, by 0)
@@ -1033,11 +1037,14 @@ __device__ __forceinline__ void grad_piece(const uint4& raw, T* d, int e0, int V
 // C: blocks of a cluster that share a row, each a span of its pieces; they leave each other what their warps found in
 // distributed shared memory, behind one cluster barrier a row.
 //
-// On a B200: log-probabilities of 32,768 rows of 16,384 bf16 words 199 us (5.4 TB/s), their gradient from kept statistics 353
-// us (6.1 TB/s, read and written): bound by memory. The policy loss and gradient of 16,384 rows of 65,541 words 893 us (4.8
-// TB/s): two 2^x and some 15 instructions a word at 24 warps a multiprocessor, which wait on each other at a row's end.
+// On a B200: log-probabilities of 32,768 rows of 16,384 bf16 words 197 us (5.5 TB/s), their gradient from kept statistics 357
+// us (6.0 TB/s, read and written): bound by memory. The policy loss and gradient of 16,384 rows of 65,541 words 897 us (4.8
+// TB/s): two 2^x and, counted, 16 instructions a word at 24 warps a multiprocessor, which wait on each other at a row's end
+// (the most frequent stall), and take 51 % of the issue slots.
 // Threads a row, the fewest that hold it, since each warp pays a row's overhead (16,380 rows of 4,101 words: 68 us with
-// 32 threads, 85 with 64, 102 with 128; 8,192 of 16,384: 104 us with 128, 132 with 256). Pieces kept in registers between the
+// 32 threads, 85 with 64, 102 with 128; 8,192 of 16,384: 102 us with 128, 132 with 256). 128 threads have 16 pieces each, in four
+// steps of four, the others' 18 in six of three: 8,192 rows of 16,384 words take 102 us in four steps and 104 in six, but
+// of 16,389 words 132 us with 256 threads, where 128 in six steps would take 107. Pieces kept in registers between the
 // passes, so that copies go on during both, lost to their warps' latency (16,384 words: 523 us, and 397 us from the ring).
 
 // warps that a multiprocessor holds with P pieces a thread in the ring, 32 at most (64 registers a thread)
